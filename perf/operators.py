@@ -126,7 +126,7 @@ def _padded(dim):
 def _regions(n_pages, n_kv, dim, n_slots, block):
     """Byte offset, type and shape of the parts of a cache buffer, each on a multiple of 256 bytes."""
     dp, sub = _padded(dim), PAGE // block
-    parts = [("k", torch.uint8, (n_pages, n_kv, PAGE, dp)), ("v", torch.uint8, (n_pages, n_kv, dp, PAGE)),
+    parts = [("k", torch.uint8, (n_pages, n_kv, dp // 64, PAGE, 64)), ("v", torch.uint8, (n_pages, n_kv, dp, PAGE)),
              ("k_scale", torch.float32, (n_pages, n_kv, sub)), ("v_scale", torch.float32, (n_pages, n_kv, sub)),
              ("pos", torch.int32, (n_pages, n_kv, PAGE)), ("sums", torch.float32, (n_pages, n_kv, PAGE)),
              ("tail", torch.float32, (n_slots, n_kv, 2, block, dim)), ("tag", torch.int32, (n_slots, n_kv, 2, 2))]
@@ -153,6 +153,11 @@ def _typed(codes, type_):
 
 def _decode(codes, type_):
     return _typed(codes, type_).float()
+
+
+def _wide(codes):
+    """Rows of key codes [..., dim] as the cache holds them: [..., columns / 64, 64], zeros behind the last."""
+    return torch.nn.functional.pad(codes, (0, _padded(codes.shape[-1]) - codes.shape[-1])).unflatten(-1, (-1, 64))
 
 
 # ---------------------------------------------------------------- what the caller has in hand
@@ -193,7 +198,7 @@ def prepare(case, seed):
             scale = (amax / CODE_MAX[type_]).clamp_min(FLOOR)
             codes = _encode(x, scale.repeat_interleave(block, -1)[..., None], type_)
             if part == "k":
-                view["k"][p:p + n, :, :, :dim] = codes
+                view["k"][p:p + n] = _wide(codes).transpose(2, 3)
             else:
                 view["v"][p:p + n, :, :dim, :] = codes.transpose(2, 3)
             view[part + "_scale"][p:p + n] = scale
@@ -296,8 +301,8 @@ def _plain_write(st):
         again = _encode(keep[s_old, :, j_old], scale[s_old, first_blk[s_old]][..., None], type_)
         at_old = fsub[s_old] * block + j_old
         if name == "k":
-            view["k"][page, :, slot % PAGE, :dim] = codes
-            view["k"][fpage[s_old], :, at_old, :dim] = again
+            view["k"][page, :, :, slot % PAGE] = _wide(codes)
+            view["k"][fpage[s_old], :, :, at_old] = _wide(again)
         else:
             view["v"][page, :, :dim, slot % PAGE] = codes
             view["v"][fpage[s_old], :, :dim, at_old] = again
@@ -318,7 +323,7 @@ def _gathered(st):
     at = st["pages"][:, :n].long().clamp_min(0)
     rep = c["block"]
     scale = lambda x: x[at].permute(0, 2, 1, 3).repeat_interleave(rep, -1).flatten(2)[..., None]  # noqa: E731
-    k = _decode(view["k"][at][..., :c["dim"]], c["type"]).permute(0, 2, 1, 3, 4).flatten(2, 3) * scale(view["k_scale"])
+    k = _decode(view["k"][at].permute(0, 2, 1, 4, 3, 5).flatten(-2)[..., :c["dim"]], c["type"]).flatten(2, 3) * scale(view["k_scale"])
     v = _decode(view["v"][at][..., :c["dim"], :], c["type"]).permute(0, 2, 1, 4, 3).flatten(2, 3) * scale(view["v_scale"])
     return k, v, view["pos"][at].permute(0, 2, 1, 3).flatten(2)
 
@@ -418,13 +423,13 @@ def _plain_evict(st):
     at = (to[w], w[1], tok[w[2], w[3]] % PAGE)
     for name in ("k", "v"):
         old = view[name + "_scale"][page, head, slot // block]
-        codes = view["k"][page, head, slot, :dim] if name == "k" else view["v"][page, head, :dim, slot]
+        codes = view["k"][page, head, :, slot].flatten(-2)[..., :dim] if name == "k" else view["v"][page, head, :dim, slot]
         x = _decode(codes, type_) * old[..., None]
         amax = torch.where(live[..., None], x.abs(), torch.zeros((), device=x.device)).amax((-1, -2))
         new = torch.where(whole, old[..., 0], (amax / CODE_MAX[type_]).clamp_min(FLOOR))
         fresh = torch.where(whole[..., None, None], codes, _encode(x, new[..., None, None], type_))
         if name == "k":
-            view["k"][at[0], at[1], at[2], :dim] = fresh[w]
+            view["k"][at[0], at[1], :, at[2]] = _wide(fresh[w])
         else:
             view["v"][at[0], at[1], :dim, at[2]] = fresh[w]
         view[name + "_scale"][at[0], at[1], at[2] // block] = new[..., None].expand_as(src)[w]
@@ -545,7 +550,7 @@ def _exact_tokens(st, s, h, name):
     length = int(st["lens"][s])
     at = st["pages"][s, :-(-length // PAGE)].long()
     codes = view[name][at, h]
-    codes = codes[..., :c["dim"]] if name == "k" else codes[:, :c["dim"]].transpose(1, 2)
+    codes = codes.transpose(1, 2).flatten(2)[..., :c["dim"]] if name == "k" else codes[:, :c["dim"]].transpose(1, 2)
     value = _decode(codes.contiguous(), c["type"]).double().reshape(-1, c["dim"])
     scale = view[name + "_scale"][at, h].double().reshape(-1)
     return (value * scale.repeat_interleave(c["block"])[:, None])[:length]
