@@ -57,6 +57,9 @@ typedef enum {
     INFR_DTYPE_TQ2_0 = 35,  /* 256 / 66 B: [u8 qs[64]][f16 d]  w = d*(q-1), 2-bit ternary codes         :356 */
     INFR_DTYPE_MXFP4 = 39,  /* 32 / 17 B: [u8 e][u8 qs[16]]  w = table[q] * 2^(e-128)             :361 */
     INFR_DTYPE_NVFP4 = 40,  /* 64 / 36 B: [u8 d[4]][u8 qs[32]]  w = table[q] * ue4m3(d[i/16]) / 2     :363 */
+    INFR_DTYPE_I8 = 24,     /* codes of an 8-bit KV cache: value = code * scale, codes -127..127 */
+    INFR_DTYPE_I32 = 26,    /* token ids, positions and the other integer tables (never a weight) */
+    INFR_DTYPE_F8_E4M3 = 64, /* codes of an 8-bit KV cache (OCP e4m3, no infinities); outside GGML's ids */
     INFR_DTYPE_BF16 = 30, /* plain rows, as F16 */
     INFR_DTYPE_Q2_0 = 42  /* 64 / 18 B:   [f16 d][u8 qs[16]] ternary-style 2-bit codes    :357-358 */
 } infr_dtype;
@@ -264,6 +267,111 @@ int infr_hip_embed_gather(infr_hip_t *be, int dtype, const infr_hip_buffer_t *ta
                           const infr_hip_buffer_t *ids, size_t rows, size_t ne, float scale,
                           infr_hip_buffer_t *dst);
 
+/* ---- the 8-bit KV cache: what a decoder layer has between its q/k/v Linears and its output Linear.
+ * No counterpart in the reference: its runner keeps the cache and the attention on another backend.
+ *
+ * The cache is ONE buffer of `n_pages` pages of 64 tokens, each page for all `n_kv` KV heads. Keys and values
+ * are 8-bit codes; `block` (16, 32 or 64) tokens of one head share an f32 scale:
+ *   I8       scale = max(amax / 127, 2^-96), code = x / scale to the nearest, ties to even
+ *   F8_E4M3  scale = max(amax / 448, 2^-96), code = e4m3(x / scale), to the nearest, ties to even
+ * A block that holds a value which is not finite has the scale NaN and zero codes: what sees any of its tokens
+ * is NaN. infr_hip_kv8_layout gives the parts' offsets; with DP = head_dim rounded up to 64 they are
+ *   k        u8  [n_pages][n_kv][DP / 64][64 tokens][64]
+ *   v        u8  [n_pages][n_kv][DP][64 tokens]
+ *   k_scale, v_scale  f32 [n_pages][n_kv][64 / block]
+ *   pos      i32 [n_pages][n_kv][64]    position of each token, as written
+ *   sums     f32 [n_pages][n_kv][64]    attention weight each token has drawn (ScoreKv8); 0 when written
+ *   tail     f32 [n_slots][n_kv][2][block][head_dim]  rows of the block that is open, K then V
+ *   tag      i32 [n_slots][n_kv][2][2]  which block of the cache the tail holds (-1: none; set by WriteKv8), its rows
+ * A fresh cache comes zeroed from infr_hip_alloc; nothing but `tag` has to be (a tag is believed).
+ *
+ * A batch is described by i32 tables in device memory, read by the kernels at each execute:
+ *   q_start [n_seq + 1]  rows q_start[s] .. q_start[s + 1] of the call belong to sequence s (ascending; rows behind
+ *                        the last sequence are left as they are)
+ *   lens    [n_seq]      tokens sequence s has in the cache, this call's rows among them: row i of n is token
+ *                        len - n + i
+ *   pages   [n_seq][max_pages]  page of token t is pages[s][t / 64]; entries behind the last token are not read
+ *   pos     [rows]       position of each row; along a sequence's tokens positions ascend strictly
+ *   slots   [n_seq]      tail slot of each sequence (WriteKv8), one sequence's own as long as it lives
+ * Sequences may share pages that none of them writes in the call. `max_q` bounds the rows of one sequence.
+ * Nothing outside the buffers is touched whatever the tables hold. A sequence whose tables contradict each other
+ * or the shapes (len < n, n > max_q, q_start outside [0, rows], len > 64 max_pages) gets nothing written, and its rows
+ * (up to max_q of them) read as NaN. Tokens on a page outside [0, n_pages) are not written and have no sums; rows of a
+ * sequence that has such tokens read as NaN, and EvictKv8 leaves the sequence as it is. */
+typedef struct {
+    /* the cache */
+    uint32_t n_pages, n_kv, head_dim /* 1..256 */, n_slots, block;
+    int dtype; /* INFR_DTYPE_I8 or INFR_DTYPE_F8_E4M3 */
+    /* the batch */
+    uint32_t rows, n_seq, max_q, max_pages;
+    /* where the rows lie, in floats: first element and distance of two rows (0: side by side). q, k and v may so be
+     * parts of one Linear's output. x is k (WriteKv8) or q */
+    uint32_t x_off, x_stride, v_off, v_stride;
+    /* AttentionKv8, ScoreKv8 */
+    uint32_t n_head; /* a multiple of n_kv: query heads h * n_head / n_kv .. read KV head h */
+    float scale, softcap /* 0: none */;
+    uint32_t window; /* 0: none */
+    int causal;
+    int has_first, has_prefix, has_slopes, has_lse;
+    float decay; /* ScoreKv8 */
+    /* EvictKv8 */
+    uint32_t keep, sink, recent;
+} infr_hip_kv8_params_t;
+
+typedef struct {
+    uint64_t k, v, k_scale, v_scale, pos, sums, tail, tag; /* byte offsets */
+    uint64_t bytes;                                        /* of the whole buffer */
+} infr_hip_kv8_layout_t;
+
+/* The operands of the four calls; those a call does not take stay NULL. */
+typedef struct {
+    const infr_hip_buffer_t *x, *v;
+    infr_hip_buffer_t *cache;
+    const infr_hip_buffer_t *pos, *pages, *q_start, *lens, *slots;
+    const infr_hip_buffer_t *first, *prefix, *slopes;
+    infr_hip_buffer_t *lse, *dst;
+    const infr_hip_buffer_t *pages_out;
+    infr_hip_buffer_t *lens_out, *kept;
+} infr_hip_kv8_operands_t;
+
+/* Host only. INFR_HIP_ERR_UNSUPPORTED for a geometry the kernels do not take. */
+int infr_hip_kv8_layout(const infr_hip_kv8_params_t *p, infr_hip_kv8_layout_t *out);
+/* Host only: whether the op `kind` (INFR_OP_WRITE_KV8 ..) takes these parameters; infr_hip_compile and the four calls
+ * refuse with INFR_HIP_ERR_UNSUPPORTED what this refuses. `why` (may be NULL) receives a static text or NULL. */
+int infr_hip_kv8_supported(int kind, const infr_hip_kv8_params_t *p, const char **why);
+
+/* WriteKv8: rows x (K) and v, f32 [rows][n_kv * head_dim], become tokens of the cache, with their positions and
+ * sums of 0. Operands x, v, cache, pos, pages, q_start, lens, slots. The codes of a block are those of all its tokens
+ * quantized at once, however many calls they came in; tokens of a block whose rows the tail has no longer (the
+ * sequence was cut back behind a block that had closed, or moved to other pages) count at their cached values. */
+int infr_hip_write_kv8(infr_hip_t *be, const infr_hip_kv8_params_t *p, const infr_hip_kv8_operands_t *o);
+
+/* AttentionKv8: dst[r, h] = sum over the tokens j that row r sees of exp(s_rj - lse[r, h]) * value_j, f32
+ * [rows][n_head * head_dim], with
+ *   s_rj = scale * q_r . key_j;  softcap > 0: s = softcap * tanh(s / softcap);  slopes: s -= slopes[h] * |pos_r - pos_j|
+ *   lse  = log of the sum of exp(s_rj), f32 [rows][n_head] (optional output).
+ * Row r sees token j of its sequence when all of these hold:
+ *   not causal, or j <= the row's own token, or the position of j < prefix[s]   (i32 [n_seq], optional: prefix mask)
+ *   window == 0, or pos_r - pos_j < window
+ *   pos_j >= first[r]                                   (i32 [rows], optional: where the row's document begins)
+ * A row that sees nothing is 0 with lse = -inf. Operands x (q), cache, dst, pos, pages, q_start, lens, then by has_*
+ * first, prefix, slopes (f32 [n_head]), lse. Sums are f32 and f32 operands keep 22 bits in the matrix products. */
+int infr_hip_attention_kv8(infr_hip_t *be, const infr_hip_kv8_params_t *p, const infr_hip_kv8_operands_t *o);
+
+/* ScoreKv8: sums_j = decay * sums_j + the weights exp(s_rj - lse[r, h]) that the call's rows and the heads of j's
+ * group give token j, with s and the masks of AttentionKv8 and its lse as input (decay 0: the old sums are not read).
+ * Operands as for AttentionKv8, without dst. Sequences of one call must not share pages here. */
+int infr_hip_score_kv8(infr_hip_t *be, const infr_hip_kv8_params_t *p, const infr_hip_kv8_operands_t *o);
+
+/* EvictKv8: cuts each sequence down to `keep` tokens per KV head: the first `sink`, the last `recent` and, of those
+ * between, the ones with the largest sums (equal sums: the earlier token), in their order, on the pages pages_out
+ * [n_seq][ceil(keep / 64)], with their positions and sums. pages_out must not name a page that the call reads. A block
+ * whose tokens come whole and in place from one block keeps its codes; others are quantized again from their cached
+ * values. lens_out[s] (i32) is the new length, -1 for a sequence whose tables are wrong (nothing of it is written);
+ * kept (i32 [n_seq][n_kv][keep]) the tokens that stayed, -1 behind the last. Operands cache, pages, lens, pages_out,
+ * lens_out, kept; params the cache's, n_seq, max_pages, keep, sink, recent. */
+int infr_hip_evict_kv8(infr_hip_t *be, const infr_hip_kv8_params_t *p, const infr_hip_kv8_operands_t *o);
+
 /* ---- graph level: Backend::compile / execute (backend.rs:560-577) over a flat C mirror of
  * infr_core::graph::Graph restricted to the ops of this path ---- */
 typedef enum {
@@ -275,7 +383,12 @@ typedef enum {
     INFR_OP_GATED_ACT = 5,       /* Op::GatedAct, graph.rs:697-735; lib.rs:1890-1944 */
     INFR_OP_GATED_ACT_FUSED = 6, /* Op::GatedActFused, graph.rs:736-748; lib.rs:1945-1971 */
     INFR_OP_ADD = 7,             /* Op::Add, graph.rs:749-755; lib.rs:1972-1988 */
-    INFR_OP_EMBED_GATHER = 8     /* Op::EmbedGather, graph.rs:853-865; lib.rs:2084-2111 */
+    INFR_OP_EMBED_GATHER = 8,    /* Op::EmbedGather, graph.rs:853-865; lib.rs:2084-2111 */
+    /* the 8-bit KV cache */
+    INFR_OP_WRITE_KV8 = 9,
+    INFR_OP_ATTENTION_KV8 = 10,
+    INFR_OP_SCORE_KV8 = 11,
+    INFR_OP_EVICT_KV8 = 12
 } infr_hip_op_kind;
 
 typedef struct {
@@ -305,6 +418,12 @@ typedef struct {
     int has_clamp;
     float clamp;
     float scale; /* EmbedGather */
+    /* Ops of the 8-bit KV cache: the operands of infr_hip_kv8_operands_t as tensor ids (x and dst above), those the
+     * op takes by its kind and kv.has_*. AttentionKv8 writes dst, ScoreKv8 the cache, EvictKv8 the cache, lens_out
+     * and kept, WriteKv8 the cache. */
+    uint32_t kv_v, kv_cache, kv_pos, kv_pages, kv_q_start, kv_lens, kv_slots, kv_first, kv_prefix, kv_slopes, kv_lse;
+    uint32_t kv_pages_out, kv_lens_out, kv_kept;
+    infr_hip_kv8_params_t kv;
 } infr_hip_op_t;
 
 /* Backend::compile: validates and stores the op list (the reference's GraphPlan clones the

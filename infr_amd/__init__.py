@@ -4,7 +4,8 @@
 ``include/infr_hip.h``; ``infr_amd.build`` compiles the HIP sources into ``libinfr_hip.so``.
 """
 from .backend import (  # noqa: F401
-    Activation, Add, Bindings, Buffer, BufferUsage, DType, EmbedGather, GatedAct, GatedActFused, Graph, HipBackend,
-    InfrError, Linear, MoeFfn, Plan, RmsNorm, RmsNormAdd, Status, TensorDesc, TensorId, block_layout,
-    load_library, synth_normal_f32, synth_weight,
+    Activation, Add, AttentionKv8, Bindings, Buffer, BufferUsage, DType, EmbedGather, EvictKv8, GatedAct, GatedActFused,
+    Graph, HipBackend, InfrError, Kv8, Kv8Batch, Linear, MoeFfn, Plan, RmsNorm, RmsNormAdd, ScoreKv8, Status,
+    TensorDesc, TensorId, WriteKv8, block_layout, kv8_supported, load_library, synth_normal_f32,
+    synth_weight,
 )

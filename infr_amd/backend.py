@@ -40,7 +40,9 @@ class DType(IntEnum):
     MXFP4 = 39
     NVFP4 = 40
     BF16 = 30    # plain rows, as F16
-    I32 = 26     # token ids (never a weight here)
+    I8 = 24      # codes of an 8-bit KV cache
+    I32 = 26     # token ids, positions, tables (never a weight here)
+    F8E4M3 = 64  # codes of an 8-bit KV cache (outside GGML's ids)
     Q2_0 = 42
 
 
@@ -101,6 +103,26 @@ def _moe_params(ne, n_expert, n_used, n_ff_exp, rows, scale, router_dtype, gate_
                       int(has_ep_band))
 
 
+class _Kv8Params(C.Structure):
+    _fields_ = [("n_pages", C.c_uint32), ("n_kv", C.c_uint32), ("head_dim", C.c_uint32), ("n_slots", C.c_uint32),
+                ("block", C.c_uint32), ("dtype", C.c_int),
+                ("rows", C.c_uint32), ("n_seq", C.c_uint32), ("max_q", C.c_uint32), ("max_pages", C.c_uint32),
+                ("x_off", C.c_uint32), ("x_stride", C.c_uint32), ("v_off", C.c_uint32), ("v_stride", C.c_uint32),
+                ("n_head", C.c_uint32), ("scale", C.c_float), ("softcap", C.c_float), ("window", C.c_uint32),
+                ("causal", C.c_int), ("has_first", C.c_int), ("has_prefix", C.c_int), ("has_slopes", C.c_int),
+                ("has_lse", C.c_int), ("decay", C.c_float),
+                ("keep", C.c_uint32), ("sink", C.c_uint32), ("recent", C.c_uint32)]
+
+
+class _Kv8Layout(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("k", "v", "k_scale", "v_scale", "pos", "sums", "tail", "tag", "bytes")]
+
+
+class _Kv8Operands(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "v", "cache", "pos", "pages", "q_start", "lens", "slots", "first",
+                                          "prefix", "slopes", "lse", "dst", "pages_out", "lens_out", "kept")]
+
+
 class _Op(C.Structure):
     _fields_ = [("kind", C.c_int), ("x", C.c_uint32), ("weight", C.c_uint32), ("dst", C.c_uint32),
                 ("m", C.c_uint32), ("in_f", C.c_uint32), ("out_f", C.c_uint32),
@@ -111,7 +133,12 @@ class _Op(C.Structure):
                 ("moe", _MoeParams),
                 ("aux", C.c_uint32), ("eps", C.c_float), ("act", C.c_int), ("up_off", C.c_uint32),
                 ("up_stride", C.c_uint32), ("gate_stride", C.c_uint32), ("gate_block_width", C.c_uint32),
-                ("has_clamp", C.c_int), ("clamp", C.c_float), ("scale", C.c_float)]
+                ("has_clamp", C.c_int), ("clamp", C.c_float), ("scale", C.c_float),
+                ("kv_v", C.c_uint32), ("kv_cache", C.c_uint32), ("kv_pos", C.c_uint32), ("kv_pages", C.c_uint32),
+                ("kv_q_start", C.c_uint32), ("kv_lens", C.c_uint32), ("kv_slots", C.c_uint32),
+                ("kv_first", C.c_uint32), ("kv_prefix", C.c_uint32), ("kv_slopes", C.c_uint32), ("kv_lse", C.c_uint32),
+                ("kv_pages_out", C.c_uint32), ("kv_lens_out", C.c_uint32), ("kv_kept", C.c_uint32),
+                ("kv", _Kv8Params)]
 
 
 class _Caps(C.Structure):
@@ -155,6 +182,12 @@ SYMBOLS = {
     "infr_hip_moe_ffn": (C.c_int, [_vp, C.POINTER(_MoeParams), _vp, _vp, _vp, _vp, _vp, _vp,
                                    C.POINTER(_MoeOptional), _vp, _vp, _vp]),
     "infr_hip_embed_gather": (C.c_int, [_vp, C.c_int, _vp, C.c_size_t, _vp, C.c_size_t, C.c_size_t, C.c_float, _vp]),
+    "infr_hip_kv8_layout": (C.c_int, [C.POINTER(_Kv8Params), C.POINTER(_Kv8Layout)]),
+    "infr_hip_kv8_supported": (C.c_int, [C.c_int, C.POINTER(_Kv8Params), C.POINTER(C.c_char_p)]),
+    "infr_hip_write_kv8": (C.c_int, [_vp, C.POINTER(_Kv8Params), C.POINTER(_Kv8Operands)]),
+    "infr_hip_attention_kv8": (C.c_int, [_vp, C.POINTER(_Kv8Params), C.POINTER(_Kv8Operands)]),
+    "infr_hip_score_kv8": (C.c_int, [_vp, C.POINTER(_Kv8Params), C.POINTER(_Kv8Operands)]),
+    "infr_hip_evict_kv8": (C.c_int, [_vp, C.POINTER(_Kv8Params), C.POINTER(_Kv8Operands)]),
     "infr_hip_compile": (C.c_int, [_vp, C.POINTER(_Op), C.c_size_t, C.POINTER(_vp)]),
     "infr_hip_plan_free": (None, [_vp, _vp]),
     "infr_hip_execute": (C.c_int, [_vp, _vp, C.POINTER(_vp), C.c_size_t]),
@@ -401,6 +434,166 @@ class EmbedGather:
     scale: float = 1.0
 
 
+@dataclass(frozen=True)
+class Kv8:
+    """Geometry of an 8-bit KV cache (include/infr_hip.h): pages of 64 tokens, `block` tokens of a head to a scale."""
+    n_pages: int
+    n_kv: int
+    head_dim: int
+    n_slots: int
+    dtype: DType = DType.I8
+    block: int = 16
+
+    def layout(self) -> dict:
+        """Byte offset of each part of the cache buffer, and ``bytes``, its size."""
+        out = _Kv8Layout()
+        rc = load_library().infr_hip_kv8_layout(C.byref(_kv8_params(self)), C.byref(out))
+        if rc != 0:
+            raise InfrError(rc, f"kv8: geometry {self} is not supported")
+        return {n: getattr(out, n) for n, _ in _Kv8Layout._fields_}
+
+    def nbytes(self) -> int:
+        return self.layout()["bytes"]
+
+
+@dataclass(frozen=True)
+class Kv8Batch:
+    """Shape of a call's batch: rows in all, sequences, most rows of one sequence, width of the page table."""
+    rows: int
+    n_seq: int
+    max_q: int
+    max_pages: int
+
+
+@dataclass
+class WriteKv8:
+    """Rows of keys and values become tokens of the cache (infr_hip_write_kv8). Offsets and strides in floats."""
+    k: TensorId
+    v: TensorId
+    cache: TensorId
+    pos: TensorId
+    pages: TensorId
+    q_start: TensorId
+    lens: TensorId
+    slots: TensorId
+    geom: Kv8
+    batch: Kv8Batch
+    k_off: int = 0
+    k_stride: int = 0
+    v_off: int = 0
+    v_stride: int = 0
+
+
+@dataclass
+class AttentionKv8:
+    """Attention of the batch's rows over the cache (infr_hip_attention_kv8); ``scale`` None: 1 / sqrt(head_dim)."""
+    q: TensorId
+    cache: TensorId
+    dst: TensorId
+    pos: TensorId
+    pages: TensorId
+    q_start: TensorId
+    lens: TensorId
+    geom: Kv8
+    batch: Kv8Batch
+    n_head: int
+    scale: float | None = None
+    softcap: float = 0.0
+    window: int = 0
+    causal: bool = True
+    first: TensorId | None = None
+    prefix: TensorId | None = None
+    slopes: TensorId | None = None
+    lse: TensorId | None = None
+    q_off: int = 0
+    q_stride: int = 0
+
+
+@dataclass
+class ScoreKv8:
+    """Attention weights summed up per cached token (infr_hip_score_kv8); ``lse`` is AttentionKv8's."""
+    q: TensorId
+    cache: TensorId
+    lse: TensorId
+    pos: TensorId
+    pages: TensorId
+    q_start: TensorId
+    lens: TensorId
+    geom: Kv8
+    batch: Kv8Batch
+    n_head: int
+    scale: float | None = None
+    softcap: float = 0.0
+    window: int = 0
+    causal: bool = True
+    first: TensorId | None = None
+    prefix: TensorId | None = None
+    slopes: TensorId | None = None
+    decay: float = 1.0
+    q_off: int = 0
+    q_stride: int = 0
+
+
+@dataclass
+class EvictKv8:
+    """The cache cut down to ``keep`` tokens per KV head, on other pages (infr_hip_evict_kv8)."""
+    cache: TensorId
+    pages: TensorId
+    lens: TensorId
+    pages_out: TensorId
+    lens_out: TensorId
+    kept: TensorId
+    geom: Kv8
+    n_seq: int
+    max_pages: int
+    keep: int
+    sink: int = 0
+    recent: int = 0
+
+
+def _kv8_params(geom: Kv8, op=None) -> _Kv8Params:
+    p = _Kv8Params(n_pages=geom.n_pages, n_kv=geom.n_kv, head_dim=geom.head_dim, n_slots=geom.n_slots,
+                   block=geom.block, dtype=int(geom.dtype))
+    if op is None:
+        return p
+    if isinstance(op, EvictKv8):
+        p.n_seq, p.max_pages, p.keep, p.sink, p.recent = op.n_seq, op.max_pages, op.keep, op.sink, op.recent
+        return p
+    b = op.batch
+    p.rows, p.n_seq, p.max_q, p.max_pages = b.rows, b.n_seq, b.max_q, b.max_pages
+    if isinstance(op, WriteKv8):
+        p.x_off, p.x_stride, p.v_off, p.v_stride = op.k_off, op.k_stride, op.v_off, op.v_stride
+        return p
+    p.x_off, p.x_stride, p.n_head = op.q_off, op.q_stride, op.n_head
+    p.scale = op.scale if op.scale is not None else 1.0 / geom.head_dim ** 0.5
+    p.softcap, p.window, p.causal = op.softcap, op.window, int(op.causal)
+    p.has_first, p.has_prefix, p.has_slopes = op.first is not None, op.prefix is not None, op.slopes is not None
+    p.has_lse = op.lse is not None
+    if isinstance(op, ScoreKv8):
+        p.decay = op.decay
+    return p
+
+
+# the fields of the 8-bit cache's ops that name tensors, with the C operand each is; the ids of x and dst are
+# infr_hip_op_t's own, the others' fields carry the prefix kv_
+_KV8_OPERANDS = {"k": "x", "q": "x", **{n: n for n in (
+    "v", "cache", "pos", "pages", "q_start", "lens", "slots", "first", "prefix", "slopes", "lse", "dst", "pages_out",
+    "lens_out", "kept")}}
+_KV8_KINDS = {WriteKv8: 9, AttentionKv8: 10, ScoreKv8: 11, EvictKv8: 12}
+
+
+def kv8_supported(op) -> str | None:
+    """None when the library takes the parameters of this op of the 8-bit KV cache, else what it does not take."""
+    why = C.c_char_p()
+    rc = load_library().infr_hip_kv8_supported(_KV8_KINDS[type(op)], C.byref(_kv8_params(op.geom, op)), C.byref(why))
+    return None if rc == 0 else (why.value or b"invalid").decode()
+
+
+def _kv8_operands(op):
+    """(C operand name, tensor) of each operand the op carries."""
+    return [(c, getattr(op, n)) for n, c in _KV8_OPERANDS.items() if getattr(op, n, None) is not None]
+
+
 @dataclass
 class Graph:
     """Ordered op list over declared tensors (crates/infr-core/src/graph.rs:1317-1460)."""
@@ -607,6 +800,11 @@ class HipBackend:
                 o.m, o.in_f, o.scale = op.rows, op.ne, op.scale
                 o.w_numel = g.desc(op.table).numel()
                 o.w_dtype = int(g.desc(op.table).dtype)
+            elif type(op) in _KV8_KINDS:
+                o.kind = _KV8_KINDS[type(op)]
+                o.kv = _kv8_params(op.geom, op)
+                for name, t in _kv8_operands(op):
+                    setattr(o, name if name in ("x", "dst") else "kv_" + name, t.id)
             else:
                 raise InfrError(Status.Unsupported, f"op {type(op).__name__} is not on this path")
         h = _vp()
@@ -698,6 +896,14 @@ class HipBackend:
         self._check(self._lib.infr_hip_moe_ffn(
             self._h, C.byref(p), x._h, rx._h, router._h, gate._h, up._h if up is not None else None, down._h,
             C.byref(opt), dst._h, sel_idx._h if sel_idx else None, sel_w._h if sel_w else None))
+
+    def run_kv8(self, op) -> None:
+        """One op of the 8-bit KV cache, directly: a WriteKv8, AttentionKv8, ScoreKv8 or EvictKv8 whose operands
+        are Buffers instead of tensor ids."""
+        entry = {WriteKv8: self._lib.infr_hip_write_kv8, AttentionKv8: self._lib.infr_hip_attention_kv8,
+                 ScoreKv8: self._lib.infr_hip_score_kv8, EvictKv8: self._lib.infr_hip_evict_kv8}[type(op)]
+        operands = _Kv8Operands(**{name: b._h for name, b in _kv8_operands(op)})
+        self._check(entry(self._h, C.byref(_kv8_params(op.geom, op)), C.byref(operands)))
 
     # -- measurement --
     def stream_read_gbs(self, buf: Buffer, nbytes: int | None = None, reps: int = 10, nontemporal: bool = False) -> float:

@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "kernels.hpp"
+#include "kv8.hpp"
 
 struct infr_hip_buffer {
     void* ptr = nullptr;
@@ -88,6 +89,9 @@ struct infr_hip {
     // MoE scratch
     void* moe_ws = nullptr;
     size_t moe_ws_bytes = 0;
+    // AttentionKv8's partial results
+    void* kv8_ws = nullptr;
+    size_t kv8_ws_bytes = 0;
     // Counts reallocations of the scratch above. A recorded launch sequence carries the scratch
     // addresses in its kernel arguments, so a plan replays only while the epoch it was recorded
     // under is still current (Internal scratch is the backend's to keep valid, backend.rs:8-13).
@@ -460,6 +464,267 @@ int check_embed(infr_hip_t* be, int dtype, const infr_hip_buffer_t* table, size_
     return INFR_HIP_OK;
 }
 
+// ---- the 8-bit KV cache ----
+
+static bool is_kv8(int kind) { return kind >= INFR_OP_WRITE_KV8 && kind <= INFR_OP_EVICT_KV8; }
+
+// The parts of a cache buffer; null when the kernels take the geometry, else what they do not.
+static const char* kv8_layout(const infr_hip_kv8_params_t& p, infr_hip_kv8_layout_t* out) {
+    if (p.dtype != INFR_DTYPE_I8 && p.dtype != INFR_DTYPE_F8_E4M3) return "cache dtype is neither I8 nor F8_E4M3";
+    if (p.head_dim == 0 || p.head_dim > 256) return "head_dim is not 1..256";
+    if (p.block != 16 && p.block != 32 && p.block != 64) return "block is not 16, 32 or 64";
+    // (block numbers are 32-bit in the tags, and every size below stays far inside 64 bits)
+    if (p.n_pages == 0 || p.n_pages > (1u << 28) || p.n_kv == 0 || p.n_kv > 4096 || p.n_slots > (1u << 24))
+        return "n_pages, n_kv or n_slots out of range";
+    const uint64_t dp = (p.head_dim + 63) / 64 * 64, heads = (uint64_t)p.n_pages * p.n_kv, slots = (uint64_t)p.n_slots * p.n_kv;
+    uint64_t at = 0;
+    auto part = [&](uint64_t bytes) {
+        const uint64_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    out->k = part(heads * dp * infr::kPage);
+    out->v = part(heads * dp * infr::kPage);
+    out->k_scale = part(heads * (infr::kPage / p.block) * 4);
+    out->v_scale = part(heads * (infr::kPage / p.block) * 4);
+    out->pos = part(heads * infr::kPage * 4);
+    out->sums = part(heads * infr::kPage * 4);
+    out->tail = part(slots * 2 * p.block * p.head_dim * 4);
+    out->tag = part(slots * 2 * 2 * 4);
+    out->bytes = at;
+    return nullptr;
+}
+
+// What does not depend on buffers: null, or what is not supported.
+static const char* kv8_shape(int kind, const infr_hip_kv8_params_t& p) {
+    infr_hip_kv8_layout_t l;
+    if (const char* msg = kv8_layout(p, &l)) return msg;
+    if (p.n_seq == 0 || p.n_seq > 65535) return "n_seq is not 1..65535";
+    if (p.max_pages == 0 || p.max_pages > 0x7FFFFFFFu / infr::kPage) return "max_pages out of range";
+    if (kind == INFR_OP_EVICT_KV8) {
+        if (p.keep == 0 || p.keep > 0x7FFFFFFFu - infr::kPage) return "keep out of range";
+        if ((uint64_t)p.sink + p.recent > p.keep) return "sink + recent exceeds keep";
+        return nullptr;
+    }
+    if (p.rows == 0 || p.rows > 0x7FFFFFFFu || p.max_q == 0 || p.max_q > p.rows) return "rows or max_q out of range";
+    if (kind == INFR_OP_WRITE_KV8) {
+        const uint32_t width = p.n_kv * p.head_dim;
+        if (p.n_slots == 0) return "a cache that is written needs tail slots";
+        if ((p.x_stride && p.x_stride < width) || (p.v_stride && p.v_stride < width)) return "row stride below a row's length";
+        return nullptr;
+    }
+    if (p.n_head == 0 || p.n_head > 65535 || p.n_head % p.n_kv != 0) return "n_head is not a multiple of n_kv";
+    if ((uint64_t)p.max_q * (p.n_head / p.n_kv) > 0x7FFFFFFFu) return "max_q out of range";
+    if (p.x_stride && p.x_stride < (uint64_t)p.n_head * p.head_dim) return "row stride below a row's length";
+    if (!(p.softcap >= 0.0f) || p.softcap > 3.0e38f || !(p.scale >= -3.0e38f && p.scale <= 3.0e38f)) return "scale or softcap out of range";
+    if (p.window > 0x7FFFFFFFu) return "window out of range";
+    if (kind == INFR_OP_SCORE_KV8 && !(p.decay >= -3.0e38f && p.decay <= 3.0e38f)) return "decay out of range";
+    return nullptr;
+}
+
+// Operands of a cache op, validated: what the launch takes, and the device ranges it reads and writes.
+struct Kv8Args {
+    infr::Kv8Cache c{};
+    infr::Kv8Batch b{};
+    infr::Kv8Attn a{};
+    infr::Kv8Evict e{};
+    const float *x = nullptr, *v = nullptr;
+    size_t x_stride = 0, v_stride = 0;
+    const int32_t* slots = nullptr;
+    float *dst = nullptr, *lse = nullptr;
+    struct Range { const uint8_t* lo; size_t bytes; };
+    Range rd[12], wr[4];
+    int n_rd = 0, n_wr = 0;
+};
+
+static int check_kv8(infr_hip_t* be, int kind, const infr_hip_kv8_params_t& p, const infr_hip_kv8_operands_t& o, Kv8Args* out) {
+    static const char* const names[] = {"write_kv8", "attention_kv8", "score_kv8", "evict_kv8"};
+    const std::string op = names[kind - INFR_OP_WRITE_KV8];
+    if (const char* msg = kv8_shape(kind, p)) return fail(be, INFR_HIP_ERR_UNSUPPORTED, op + ": " + msg);
+    infr_hip_kv8_layout_t l;
+    (void)kv8_layout(p, &l);
+    *out = Kv8Args{};
+    std::string bad;
+    auto take = [&](const infr_hip_buffer_t* b, const char* name, uint64_t bytes, uint64_t align, bool writes) -> uint8_t* {
+        if (!b) bad = std::string(name) + " is unbound";
+        else if (b->len < bytes) bad = std::string(name) + " is too small for the shape";
+        else if (reinterpret_cast<uintptr_t>(b->ptr) % align != 0) bad = std::string(name) + " is misaligned";
+        else {
+            uint8_t* at = static_cast<uint8_t*>(b->ptr);
+            if (writes) out->wr[out->n_wr++] = {at, (size_t)bytes};
+            else out->rd[out->n_rd++] = {at, (size_t)bytes};
+            return at;
+        }
+        return nullptr;
+    };
+    auto rows_bytes = [&](uint64_t off, uint64_t stride, uint64_t width) {
+        return (off + (p.rows - 1) * (stride ? stride : width) + width) * 4;
+    };
+    auto i32 = [&](const infr_hip_buffer_t* b, const char* name, uint64_t n) {
+        return reinterpret_cast<const int32_t*>(take(b, name, n * 4, 4, false));
+    };
+    uint8_t* cache = take(o.cache, "cache", l.bytes, 16, kind != INFR_OP_ATTENTION_KV8);
+    infr::Kv8Cache& c = out->c;
+    c.k = cache + l.k;
+    c.v = cache + l.v;
+    c.ks = reinterpret_cast<float*>(cache + l.k_scale);
+    c.vs = reinterpret_cast<float*>(cache + l.v_scale);
+    c.pos = reinterpret_cast<int32_t*>(cache + l.pos);
+    c.sums = reinterpret_cast<float*>(cache + l.sums);
+    c.tail = reinterpret_cast<float*>(cache + l.tail);
+    c.tag = reinterpret_cast<int32_t*>(cache + l.tag);
+    c.n_pages = (int32_t)p.n_pages;
+    c.n_kv = (int32_t)p.n_kv;
+    c.dim = (int32_t)p.head_dim;
+    c.dp = (int32_t)((p.head_dim + 63) / 64 * 64);
+    c.n_slots = (int32_t)p.n_slots;
+    c.block = (int32_t)p.block;
+    c.f8 = p.dtype == INFR_DTYPE_F8_E4M3;
+    const int32_t* pages = i32(o.pages, "pages", (uint64_t)p.n_seq * p.max_pages);
+    const int32_t* lens = i32(o.lens, "lens", p.n_seq);
+    if (kind == INFR_OP_EVICT_KV8) {
+        const uint64_t out_pages = ((uint64_t)p.keep + infr::kPage - 1) / infr::kPage;
+        infr::Kv8Evict& e = out->e;
+        e.pages = pages;
+        e.lens = lens;
+        e.pages_out = i32(o.pages_out, "pages_out", p.n_seq * out_pages);
+        e.lens_out = reinterpret_cast<int32_t*>(take(o.lens_out, "lens_out", (uint64_t)p.n_seq * 4, 4, true));
+        e.kept = reinterpret_cast<int32_t*>(take(o.kept, "kept", (uint64_t)p.n_seq * p.n_kv * p.keep * 4, 4, true));
+        e.n_seq = (int32_t)p.n_seq;
+        e.max_pages = (int32_t)p.max_pages;
+        e.out_pages = (int32_t)out_pages;
+        e.keep = (int32_t)p.keep;
+        e.sink = (int32_t)p.sink;
+        e.recent = (int32_t)p.recent;
+    } else {
+        infr::Kv8Batch& b = out->b;
+        b.pos = i32(o.pos, "pos", p.rows);
+        b.pages = pages;
+        b.q_start = i32(o.q_start, "q_start", (uint64_t)p.n_seq + 1);
+        b.lens = lens;
+        b.rows = (int32_t)p.rows;
+        b.n_seq = (int32_t)p.n_seq;
+        b.max_q = (int32_t)p.max_q;
+        b.max_pages = (int32_t)p.max_pages;
+        const uint64_t width = (uint64_t)(kind == INFR_OP_WRITE_KV8 ? p.n_kv : p.n_head) * p.head_dim;
+        out->x = reinterpret_cast<const float*>(take(o.x, kind == INFR_OP_WRITE_KV8 ? "k" : "q", rows_bytes(p.x_off, p.x_stride, width), 4, false)) + p.x_off;
+        out->x_stride = p.x_stride ? p.x_stride : (size_t)width;
+        if (kind == INFR_OP_WRITE_KV8) {
+            out->v = reinterpret_cast<const float*>(take(o.v, "v", rows_bytes(p.v_off, p.v_stride, width), 4, false)) + p.v_off;
+            out->v_stride = p.v_stride ? p.v_stride : (size_t)width;
+            out->slots = i32(o.slots, "slots", p.n_seq);
+        } else {
+            const uint64_t lse_bytes = (uint64_t)p.rows * p.n_head * 4;
+            infr::Kv8Attn& a = out->a;
+            a.q = out->x;
+            a.q_stride = out->x_stride;
+            a.n_head = (int32_t)p.n_head;
+            a.group = (int32_t)(p.n_head / p.n_kv);
+            a.scale = p.scale;
+            a.softcap = p.softcap;
+            a.window = (int32_t)p.window;
+            a.causal = p.causal;
+            if (p.has_first) a.first = i32(o.first, "first", p.rows);
+            if (p.has_prefix) a.prefix = i32(o.prefix, "prefix", p.n_seq);
+            if (p.has_slopes) a.slopes = reinterpret_cast<const float*>(take(o.slopes, "slopes", (uint64_t)p.n_head * 4, 4, false));
+            const bool scores = kind == INFR_OP_SCORE_KV8;
+            if (scores || p.has_lse) out->lse = reinterpret_cast<float*>(take(o.lse, "lse", lse_bytes, 4, !scores));
+            if (!scores) out->dst = reinterpret_cast<float*>(take(o.dst, "dst", (uint64_t)p.rows * width * 4, 4, true));
+        }
+    }
+    if (!bad.empty()) return fail(be, INFR_HIP_ERR_INVALID, op + ": " + bad);
+    // an output over an input or over another output: the kernels read and write in no fixed order
+    for (int i = 0; i < out->n_wr; ++i) {
+        const auto& w = out->wr[i];
+        auto meets = [&](const Kv8Args::Range& r) { return w.lo < r.lo + r.bytes && r.lo < w.lo + w.bytes; };
+        for (int j = 0; j < out->n_rd; ++j)
+            if (meets(out->rd[j])) return fail(be, INFR_HIP_ERR_INVALID, op + ": an output overlaps an input");
+        for (int j = 0; j < i; ++j)
+            if (meets(out->wr[j])) return fail(be, INFR_HIP_ERR_INVALID, op + ": two outputs overlap");
+    }
+    return INFR_HIP_OK;
+}
+
+// The operands of a plan's op out of the bindings, those its kind and flags name.
+static infr_hip_kv8_operands_t kv8_operands(const infr_hip_op_t& op, infr_hip_buffer_t* const* bindings) {
+    infr_hip_kv8_operands_t o{};
+    o.cache = bindings[op.kv_cache];
+    o.pages = bindings[op.kv_pages];
+    o.lens = bindings[op.kv_lens];
+    if (op.kind == INFR_OP_EVICT_KV8) {
+        o.pages_out = bindings[op.kv_pages_out];
+        o.lens_out = bindings[op.kv_lens_out];
+        o.kept = bindings[op.kv_kept];
+        return o;
+    }
+    o.x = bindings[op.x];
+    o.pos = bindings[op.kv_pos];
+    o.q_start = bindings[op.kv_q_start];
+    if (op.kind == INFR_OP_WRITE_KV8) {
+        o.v = bindings[op.kv_v];
+        o.slots = bindings[op.kv_slots];
+        return o;
+    }
+    if (op.kv.has_first) o.first = bindings[op.kv_first];
+    if (op.kv.has_prefix) o.prefix = bindings[op.kv_prefix];
+    if (op.kv.has_slopes) o.slopes = bindings[op.kv_slopes];
+    if (op.kind == INFR_OP_SCORE_KV8 || op.kv.has_lse) o.lse = bindings[op.kv_lse];
+    if (op.kind == INFR_OP_ATTENTION_KV8) o.dst = bindings[op.dst];
+    return o;
+}
+
+// Largest tensor id a plan's op names.
+static uint32_t kv8_max_tensor(const infr_hip_op_t& op) {
+    uint32_t m = std::max({op.kv_cache, op.kv_pages, op.kv_lens});
+    if (op.kind == INFR_OP_EVICT_KV8) return std::max({m, op.kv_pages_out, op.kv_lens_out, op.kv_kept});
+    m = std::max({m, op.x, op.kv_pos, op.kv_q_start});
+    if (op.kind == INFR_OP_WRITE_KV8) return std::max({m, op.kv_v, op.kv_slots});
+    if (op.kv.has_first) m = std::max(m, op.kv_first);
+    if (op.kv.has_prefix) m = std::max(m, op.kv_prefix);
+    if (op.kv.has_slopes) m = std::max(m, op.kv_slopes);
+    if (op.kind == INFR_OP_SCORE_KV8 || op.kv.has_lse) m = std::max(m, op.kv_lse);
+    return op.kind == INFR_OP_ATTENTION_KV8 ? std::max(m, op.dst) : m;
+}
+
+// Scratch an op of this shape needs.
+static size_t kv8_scratch(int kind, const infr_hip_kv8_params_t& p) {
+    return kind == INFR_OP_ATTENTION_KV8
+               ? infr::attention_kv8_scratch((int)p.head_dim, (int)p.n_kv, (int)(p.n_head / p.n_kv), (int)p.n_seq, (int)p.max_q, (int)p.max_pages)
+               : 0;
+}
+
+static int ensure_kv8_ws(infr_hip_t* be, size_t bytes) {
+    if (bytes <= be->kv8_ws_bytes) return INFR_HIP_OK;
+    int current = be->device;
+    (void)hipGetDevice(&current);
+    HIP_TRY(be, hipStreamSynchronize(be->stream));
+    ++be->scratch_epoch;
+    if (be->kv8_ws) (void)hipFree(be->kv8_ws);
+    be->kv8_ws = nullptr;
+    be->kv8_ws_bytes = 0;
+    HIP_TRY(be, hipSetDevice(be->device));
+    const hipError_t e = hipMalloc(&be->kv8_ws, bytes);
+    (void)hipSetDevice(current);
+    if (e != hipSuccess) {
+        be->kv8_ws = nullptr;
+        return fail(be, INFR_HIP_ERR_BACKEND, "attention_kv8: hipMalloc(" + std::to_string(bytes) + "): " + hipGetErrorString(e));
+    }
+    be->kv8_ws_bytes = bytes;
+    return INFR_HIP_OK;
+}
+
+static int enqueue_kv8(infr_hip_t* be, int kind, const infr_hip_kv8_params_t& p, const Kv8Args& k) {
+    if (kv8_scratch(kind, p) > be->kv8_ws_bytes) return fail(be, INFR_HIP_ERR_OTHER, "attention_kv8: scratch was not sized");
+    switch (kind) {
+    case INFR_OP_WRITE_KV8: infr::launch_write_kv8(k.c, k.b, k.slots, k.x, k.x_stride, k.v, k.v_stride, be->stream); break;
+    case INFR_OP_ATTENTION_KV8: infr::launch_attention_kv8(k.c, k.b, k.a, k.dst, k.lse, be->kv8_ws, be->stream); break;
+    case INFR_OP_SCORE_KV8: infr::launch_score_kv8(k.c, k.b, k.a, k.lse, p.decay, be->stream); break;
+    default: infr::launch_evict_kv8(k.c, k.e, be->stream); break;
+    }
+    HIP_TRY(be, hipGetLastError());
+    return INFR_HIP_OK;
+}
+
 int check_latch(infr_hip_t* be) {
     if (g_shutdown_signo.load(std::memory_order_relaxed) != 0)
         return fail(be, INFR_HIP_ERR_ABORTED, "shutdown requested");
@@ -524,6 +789,7 @@ void infr_hip_destroy(infr_hip_t* be) {
         (void)hipFree(be->act.bsums16);
     }
     if (be->moe_ws) (void)hipFree(be->moe_ws);
+    if (be->kv8_ws) (void)hipFree(be->kv8_ws);
     if (be->ev0) (void)hipEventDestroy(be->ev0);
     if (be->ev1) (void)hipEventDestroy(be->ev1);
     if (be->stream) (void)hipStreamDestroy(be->stream);
@@ -932,6 +1198,41 @@ int infr_hip_moe_ffn(infr_hip_t* be, const infr_hip_moe_params_t* p, const infr_
     return enqueue_moe(be, s, b);
 }
 
+static int run_kv8(infr_hip_t* be, int kind, const infr_hip_kv8_params_t* p, const infr_hip_kv8_operands_t* o) {
+    if (!be) return INFR_HIP_ERR_INVALID;
+    if (!p || !o) return fail(be, INFR_HIP_ERR_INVALID, "kv8: null argument");
+    if (int rc = check_latch(be)) return rc;
+    Kv8Args k;
+    if (int rc = check_kv8(be, kind, *p, *o, &k)) return rc;
+    if (int rc = ensure_kv8_ws(be, kv8_scratch(kind, *p))) return rc;
+    return enqueue_kv8(be, kind, *p, k);
+}
+
+int infr_hip_kv8_layout(const infr_hip_kv8_params_t* p, infr_hip_kv8_layout_t* out) {
+    if (!p || !out) return INFR_HIP_ERR_INVALID;
+    std::memset(out, 0, sizeof *out);
+    return kv8_layout(*p, out) ? INFR_HIP_ERR_UNSUPPORTED : INFR_HIP_OK;
+}
+int infr_hip_kv8_supported(int kind, const infr_hip_kv8_params_t* p, const char** why) {
+    if (why) *why = nullptr;
+    if (!p || !is_kv8(kind)) return INFR_HIP_ERR_INVALID;
+    const char* msg = kv8_shape(kind, *p);
+    if (why) *why = msg;
+    return msg ? INFR_HIP_ERR_UNSUPPORTED : INFR_HIP_OK;
+}
+int infr_hip_write_kv8(infr_hip_t* be, const infr_hip_kv8_params_t* p, const infr_hip_kv8_operands_t* o) {
+    return run_kv8(be, INFR_OP_WRITE_KV8, p, o);
+}
+int infr_hip_attention_kv8(infr_hip_t* be, const infr_hip_kv8_params_t* p, const infr_hip_kv8_operands_t* o) {
+    return run_kv8(be, INFR_OP_ATTENTION_KV8, p, o);
+}
+int infr_hip_score_kv8(infr_hip_t* be, const infr_hip_kv8_params_t* p, const infr_hip_kv8_operands_t* o) {
+    return run_kv8(be, INFR_OP_SCORE_KV8, p, o);
+}
+int infr_hip_evict_kv8(infr_hip_t* be, const infr_hip_kv8_params_t* p, const infr_hip_kv8_operands_t* o) {
+    return run_kv8(be, INFR_OP_EVICT_KV8, p, o);
+}
+
 // ---- plan / execute ----
 
 int infr_hip_compile(infr_hip_t* be, const infr_hip_op_t* ops, size_t n_ops, infr_hip_plan_t** out) {
@@ -942,7 +1243,7 @@ int infr_hip_compile(infr_hip_t* be, const infr_hip_op_t* ops, size_t n_ops, inf
     p->ops.assign(ops, ops + n_ops);
     // batch_need: one small-batch op's activations; a group of several distinct activation tensors
     // grows the scratch when it is scheduled (the levels depend on the bound addresses)
-    size_t act_need = 0, moe_need = 0, batch_need = 0;
+    size_t act_need = 0, moe_need = 0, batch_need = 0, kv8_need = 0;
     for (const auto& op : p->ops) {
         if (op.kind == INFR_OP_LINEAR) {
             if ((!is_quant(op.w_dtype) && !is_plain(op.w_dtype)) || op.m == 0 || op.in_f == 0 || op.out_f == 0 ||
@@ -990,6 +1291,13 @@ int infr_hip_compile(infr_hip_t* be, const infr_hip_op_t* ops, size_t n_ops, inf
                 return fail(be, INFR_HIP_ERR_UNSUPPORTED, "compile: EmbedGather op with unsupported dtype/shape");
             }
             p->max_tensor = std::max({p->max_tensor, op.x, op.weight, op.dst});
+        } else if (is_kv8(op.kind)) {
+            if (const char* msg = kv8_shape(op.kind, op.kv)) {
+                delete p;
+                return fail(be, INFR_HIP_ERR_UNSUPPORTED, std::string("compile: 8-bit KV cache op: ") + msg);
+            }
+            p->max_tensor = std::max(p->max_tensor, kv8_max_tensor(op));
+            kv8_need = std::max(kv8_need, kv8_scratch(op.kind, op.kv));
         } else {
             delete p;
             return fail(be, INFR_HIP_ERR_UNSUPPORTED, "compile: op kind " + std::to_string(op.kind));
@@ -1001,6 +1309,10 @@ int infr_hip_compile(infr_hip_t* be, const infr_hip_op_t* ops, size_t n_ops, inf
         return rc;
     }
     if (int rc = ensure_moe_ws(be, moe_need)) {
+        delete p;
+        return rc;
+    }
+    if (int rc = ensure_kv8_ws(be, kv8_need)) {
         delete p;
         return rc;
     }
@@ -1017,6 +1329,7 @@ size_t infr_hip_plan_launches(const infr_hip_plan_t* plan) {
         if (st.op < 0) n += st.m > 1 ? 2 : 1;                              // grouped launch (+ grouped quantize)
         else if (plan->ops[st.op].kind == INFR_OP_MOE_FFN) n += plan->ops[st.op].moe.rows == 1 ? 3 : 4;
         else if (is_elementwise(plan->ops[st.op].kind) || plan->ops[st.op].kind == INFR_OP_EMBED_GATHER) n += 1;
+        else if (is_kv8(plan->ops[st.op].kind)) n += plan->ops[st.op].kind == INFR_OP_WRITE_KV8 ? 1 : 2;
         else n += 2;                                                       // quantize + GEMM
     }
     return n;
@@ -1088,6 +1401,15 @@ static int schedule_plan(infr_hip_t* be, infr_hip_plan_t* plan, infr_hip_buffer_
             rd[i] = {fspan(ea[i].x, ea[i].x_elems)};
             if (ea[i].aux) rd[i].push_back(fspan(ea[i].aux, ea[i].aux_elems));
             wr[i] = {fspan(ea[i].dst, ea[i].dst_elems)};
+        } else if (is_kv8(op.kind)) {
+            Kv8Args k;
+            if (int rc = check_kv8(be, op.kind, op.kv, kv8_operands(op, bindings), &k)) return rc;
+            for (int j = 0; j < k.n_rd; ++j) rd[i].push_back(Span{k.rd[j].lo, k.rd[j].lo + k.rd[j].bytes});
+            for (int j = 0; j < k.n_wr; ++j) {
+                // rows behind the last sequence and pages of others keep what they held: a write that reads
+                wr[i].push_back(Span{k.wr[j].lo, k.wr[j].lo + k.wr[j].bytes});
+                rd[i].push_back(wr[i].back());
+            }
         } else {
             if (int rc = check_linear(be, op.w_dtype, bindings[op.weight], op.w_numel, op.w_off,
                                       bindings[op.x], op.m, op.in_f, op.out_f, &la[i]))
@@ -1691,6 +2013,11 @@ static int enqueue_plan(infr_hip_t* be, infr_hip_plan_t* plan, infr_hip_buffer_t
                                       static_cast<const int32_t*>(bindings[op.x]->ptr), op.m, op.in_f, op.scale,
                                       static_cast<float*>(bindings[op.dst]->ptr), be->stream);
             HIP_TRY(be, hipGetLastError());
+        } else if (st.op >= 0 && is_kv8(plan->ops[st.op].kind)) {
+            const auto& op = plan->ops[st.op];
+            Kv8Args k;
+            if (int rc = check_kv8(be, op.kind, op.kv, kv8_operands(op, bindings), &k)) return rc;
+            if (int rc = enqueue_kv8(be, op.kind, op.kv, k)) return rc;
         } else if (st.op >= 0 && is_elementwise(plan->ops[st.op].kind)) {
             ElementwiseArgs ea;
             if (int rc = check_elementwise(be, plan->ops[st.op], bindings, &ea)) return rc;
@@ -1757,6 +2084,7 @@ int infr_hip_execute(infr_hip_t* be, infr_hip_plan_t* plan, infr_hip_buffer_t* c
     // Validate and schedule before recording so a bad binding cannot leave a capture open.
     for (const auto& op : plan->ops) {
         const bool moe = op.kind == INFR_OP_MOE_FFN;
+        if (is_kv8(op.kind)) continue;  // check_kv8 names the operands it misses
         // elementwise ops name their second operand per kind; check_elementwise validates it
         if (!bindings[op.x] || !bindings[op.dst] || ((op.kind == INFR_OP_LINEAR || op.kind == INFR_OP_EMBED_GATHER) && !bindings[op.weight]) ||
             (moe && (!bindings[op.router_x] || !bindings[op.router] || !bindings[op.gate_exps] ||

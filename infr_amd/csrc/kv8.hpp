@@ -1,0 +1,154 @@
+// The 8-bit KV cache and what its kernels share: geometry, the parts of the cache buffer, the tables
+// of a batch, the codes of the two types and the search for the sequence a workgroup works on.
+//
+// The cache is one buffer of `n_pages` pages of 64 tokens, each for all KV heads. Its parts, each on a
+// multiple of 256 bytes, in this order (DP = head_dim rounded up to 64):
+//   K codes    u8  [n_pages][n_kv][DP/64][64 tokens][64]   64 bytes of a token side by side: the four lanes
+//                                                          that feed a token to the MFMA read one segment
+//   V codes    u8  [n_pages][n_kv][DP][64 tokens]          tokens side by side: P.V's MFMA sums over tokens
+//   K scales   f32 [n_pages][n_kv][64/block], V scales the same
+//   positions  i32 [n_pages][n_kv][64]
+//   sums       f32 [n_pages][n_kv][64]                     accumulated attention weight of each token
+//   tail       f32 [n_slots][n_kv][2][block][head_dim]     the rows of the block that is open, K then V
+//   tag        i32 [n_slots][n_kv][2][2]                   which block of the cache the tail holds, how many rows
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace infr {
+
+constexpr int kPage = 64;
+constexpr float kMinScale = 0x1p-96f;
+
+struct Kv8Cache {
+    uint8_t *k, *v;
+    float *ks, *vs;
+    int32_t* pos;
+    float* sums;
+    float* tail;
+    int32_t* tag;
+    int32_t n_pages, n_kv, dim, dp, n_slots, block, f8;
+};
+
+// The tables that describe a batch, all in device memory.
+struct Kv8Batch {
+    const int32_t* pos;      // [rows]
+    const int32_t* pages;    // [n_seq][max_pages]
+    const int32_t* q_start;  // [n_seq + 1]
+    const int32_t* lens;     // [n_seq]
+    int32_t rows, n_seq, max_q, max_pages;
+};
+
+// What AttentionKv8 and ScoreKv8 have in common.
+struct Kv8Attn {
+    const float* q;
+    size_t q_stride;          // floats from row to row
+    int32_t n_head, group;    // query heads, and per KV head
+    float scale, softcap;     // softcap 0: none
+    int32_t window;           // 0: none
+    int32_t causal;
+    const int32_t* first;     // [rows] or null
+    const int32_t* prefix;    // [n_seq] or null
+    const float* slopes;      // [n_head] or null
+};
+
+struct Kv8Evict {
+    const int32_t* pages;
+    const int32_t* lens;
+    const int32_t* pages_out;  // [n_seq][out_pages]
+    int32_t* lens_out;
+    int32_t* kept;             // [n_seq][n_kv][keep]
+    int32_t n_seq, max_pages, out_pages, keep, sink, recent;
+};
+
+void launch_write_kv8(const Kv8Cache& c, const Kv8Batch& b, const int32_t* slots, const float* k, size_t k_stride,
+                      const float* v, size_t v_stride, hipStream_t stream);
+// f32 scratch an attention launch needs, in bytes.
+size_t attention_kv8_scratch(int dim, int n_kv, int group, int n_seq, int max_q, int max_pages);
+void launch_attention_kv8(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, void* scratch,
+                          hipStream_t stream);
+void launch_score_kv8(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, const float* lse, float decay,
+                      hipStream_t stream);
+void launch_evict_kv8(const Kv8Cache& c, const Kv8Evict& e, hipStream_t stream);
+
+#ifdef __HIPCC__
+// ---- device side ----
+
+struct Kv8Seq {
+    int r0, n, len;  // first row, rows, cached tokens
+    bool ok;
+};
+// Sequence s of the batch. Tables that contradict each other or the shapes give ok = false and, in r0 / n,
+// at most max_q rows that lie inside the batch; no other row or page of that sequence is touched.
+__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Batch& b, int s) {
+    const int r0 = b.q_start[s], r1 = b.q_start[s + 1], len = b.lens[s];
+    Kv8Seq q;
+    const int c0 = min(max(r0, 0), b.rows), c1 = min(max(r1, c0), b.rows);
+    q.r0 = c0;
+    q.n = min(c1 - c0, b.max_q);
+    q.len = len;
+    q.ok = r0 == c0 && r1 == c1 && c1 - c0 <= b.max_q && len >= q.n && len <= b.max_pages * kPage;
+    return q;
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
+
+// Scale of a block from the largest absolute value's bits; a value that is not finite makes it NaN.
+__device__ __forceinline__ float kv8_scale(uint32_t amax_bits, bool f8) {
+    if (amax_bits >= 0x7F800000u) return __builtin_nanf("");
+    return fmaxf(__builtin_bit_cast(float, amax_bits) / (f8 ? 448.0f : 127.0f), kMinScale);
+}
+// Nearest code of x / scale, ties to even. |x / scale| stays below the largest code's rounding border: the
+// scale is amax / code_max rounded once and the quotient is rounded once more.
+__device__ __forceinline__ uint32_t kv8_code(float x, float scale, bool f8) {
+    if (!(scale < __builtin_inff())) return 0;  // a NaN scale
+    const float y = x / scale;
+    if (f8) return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false) & 0xFFu;
+    return (uint32_t)(int)fminf(fmaxf(rintf(y), -127.0f), 127.0f) & 0xFFu;
+}
+__device__ __forceinline__ float kv8_value(uint32_t code, bool f8) {
+    return f8 ? __builtin_amdgcn_cvt_f32_fp8((int)code, 0) : (float)(int)(int8_t)code;
+}
+
+// Byte offset of key code d of token t of (page, head) / of value code d.
+__device__ __forceinline__ size_t k_at(const Kv8Cache& c, int page, int h, int t, int d) {
+    return ((((size_t)page * c.n_kv + h) * (c.dp / 64) + d / 64) * kPage + t) * 64 + d % 64;
+}
+__device__ __forceinline__ size_t v_at(const Kv8Cache& c, int page, int h, int t, int d) {
+    return (((size_t)page * c.n_kv + h) * c.dp + d) * kPage + t;
+}
+
+// Inclusive prefix sum over the 64 lanes of a wave.
+__device__ __forceinline__ int wave_scan(int x) {
+    const int lane = (int)(threadIdx.x & 63);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    return x;
+}
+
+// The sequence that work item `idx` belongs to, where sequence s has count(s) >= 0 of them, and in *rest its
+// number within the sequence; -1 when there are fewer items. Every lane of the wave calls it with the same idx.
+template <typename F>
+__device__ __forceinline__ int find_seq(int n_seq, int idx, int* rest, F count) {
+    const int lane = (int)(threadIdx.x & 63);
+    for (int base = 0; base < n_seq; base += 64) {
+        const int n = base + lane < n_seq ? count(base + lane) : 0;
+        const int sum = wave_scan(n);
+        const unsigned long long hit = __ballot(idx < sum);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            *rest = idx - (__shfl(sum, l) - __shfl(n, l));
+            return base + l;
+        }
+        idx -= __shfl(sum, 63);
+    }
+    return -1;
+}
+#endif  // __HIPCC__
+
+}  // namespace infr

@@ -1,0 +1,152 @@
+// WriteKv8: a call's new key and value rows into the 8-bit cache.
+//
+// A block of `block` tokens of one head has one scale, so a token that joins an open block can change the codes
+// of those before it. The open block's rows are therefore kept in f32 (the tail of the sequence's slot) and the
+// block is quantized from them as a whole each time: its codes are those of its tokens taken at once, whatever
+// pieces they came in. Tokens of a block whose rows the tail no longer holds (a sequence cut back behind a block
+// that had closed, or one that moved to other pages) are taken at their cached values.
+//
+// One workgroup per (page that gets tokens, head, K or V): 64 tokens x 64 columns at a time, four lanes to a
+// token, 16 columns each, so that a token's 64 columns are one 256-byte read and its key codes one 64-byte
+// segment; value codes turn in LDS. Bound by HBM on 8 bytes read and 2 written per column of a token; a single
+// token per sequence is bound by the launch.
+#include <algorithm>
+
+#include "kv8.hpp"
+
+namespace infr {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kTurn = kPage + 4;  // LDS row of value codes: 4 bytes of padding keep the columns off one bank
+
+// Pages of sequence s that get tokens.
+__device__ __forceinline__ int pages_written(const Kv8Batch& b, int s) {
+    const Kv8Seq q = kv8_seq(b, s);
+    return q.ok && q.n > 0 ? (q.len - 1) / kPage - (q.len - q.n) / kPage + 1 : 0;
+}
+
+__global__ __launch_bounds__(kThreads) void write_kv8_kernel(Kv8Cache c, Kv8Batch b, const int32_t* __restrict__ slots,
+                                                             const float* __restrict__ kx, size_t k_stride,
+                                                             const float* __restrict__ vx, size_t v_stride) {
+    __shared__ uint32_t amax[kPage];
+    __shared__ __align__(16) uint8_t turn[64 * kTurn];
+    int rest = 0;
+    const int s = find_seq(b.n_seq, (int)blockIdx.x, &rest, [&](int i) { return pages_written(b, i); });
+    if (s < 0) return;
+    const int h = blockIdx.y;
+    const bool is_v = blockIdx.z != 0;
+    const Kv8Seq q = kv8_seq(b, s);
+    const int slot0 = q.len - q.n;                       // first new token
+    const int pi = slot0 / kPage + rest;                 // page of the sequence
+    const int page = b.pages[(size_t)s * b.max_pages + pi];
+    const int tail_slot = slots[s];
+    const bool page_ok = page >= 0 && page < c.n_pages;
+    const bool tail_ok = tail_slot >= 0 && tail_slot < c.n_slots;
+    const bool f8 = c.f8 != 0;
+    const int tid = threadIdx.x, t = tid >> 2, col = (tid & 3) * 16;
+    const int subs = kPage / c.block, sub = t / c.block;
+    const int tok = pi * kPage + t;                      // token of this thread
+    // the block that was open before the call, and what of it the tail holds
+    const int open = slot0 / c.block * c.block, have = slot0 - open;
+    const float* x = is_v ? vx : kx;
+    const size_t stride = is_v ? v_stride : k_stride;
+    const size_t tail_at = (((size_t)tail_slot * c.n_kv + h) * 2 + (is_v ? 1 : 0)) * c.block * c.dim;
+    int32_t* tag = tail_ok ? c.tag + (((size_t)tail_slot * c.n_kv + h) * 2 + (is_v ? 1 : 0)) * 2 : nullptr;
+    const bool raw = rest == 0 && tail_ok && have > 0 && page_ok && tag[0] == page * subs + open % kPage / c.block && tag[1] >= have;
+    float* scales = is_v ? c.vs : c.ks;
+    const size_t scale_at = ((size_t)page * c.n_kv + h) * subs + sub;
+    const bool touched = tok / c.block >= slot0 / c.block && tok / c.block <= (q.len - 1) / c.block;
+    const bool is_new = tok >= slot0 && tok < q.len, is_old = touched && tok < slot0;
+    const float old_scale = is_old && !raw && page_ok ? scales[scale_at] : 0.0f;
+
+    // value of column d of this thread's token: zero behind the sequence's end and the row's
+    auto value = [&](int d) -> float {
+        if (d >= c.dim) return 0.0f;
+        if (is_new) return x[(size_t)(q.r0 + tok - slot0) * stride + (size_t)h * c.dim + d];
+        if (!is_old) return 0.0f;
+        if (raw) return c.tail[tail_at + (size_t)(tok - open) * c.dim + d];
+        const size_t at = is_v ? v_at(c, page, h, t, d) : k_at(c, page, h, t, d);
+        return kv8_value((is_v ? c.v : c.k)[at], f8) * old_scale;
+    };
+
+    float r[4][16];  // this thread's columns: 16 of each 64
+    uint32_t top = 0;
+    if (page_ok)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j * 64 < c.dp)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    r[j][e] = value(j * 64 + col + e);
+                    top = max(top, abs_bits(r[j][e]));
+                }
+    top = max(top, (uint32_t)__shfl_xor((int)top, 1));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 2));
+    if ((tid & 3) == 0) amax[t] = top;
+    __syncthreads();
+    for (int o = 0; o < c.block; ++o) top = max(top, amax[sub * c.block + o]);
+    const float scale = kv8_scale(top, f8);
+    if (page_ok && touched && t % c.block == 0 && (tid & 3) == 0) scales[scale_at] = scale;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (j * 64 >= c.dp || !page_ok) continue;
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e / 4] |= kv8_code(r[j][e], scale, f8) << (8 * (e % 4));
+        if (!is_v) {
+            if (touched) *reinterpret_cast<uint4*>(c.k + k_at(c, page, h, t, j * 64 + col)) = make_uint4(w[0], w[1], w[2], w[3]);
+            continue;
+        }
+        __syncthreads();  // (page_ok and dp are the workgroup's)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) turn[(col + e) * kTurn + t] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
+        __syncthreads();
+        // thread -> 16 tokens of one column; blocks are whole 16s, so a segment is written or left as a whole
+        const int d = tid >> 2, t0 = (tid & 3) * 16;
+        const int first = (pi * kPage + t0) / c.block;
+        if (first >= slot0 / c.block && first <= (q.len - 1) / c.block) {
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(turn + d * kTurn + t0);
+            *reinterpret_cast<uint4*>(c.v + v_at(c, page, h, t0, j * 64 + d)) = make_uint4(src[0], src[1], src[2], src[3]);
+        }
+    }
+    if (!is_v && page_ok && is_new && (tid & 3) == 0) {
+        const size_t at = ((size_t)page * c.n_kv + h) * kPage + t;
+        c.pos[at] = b.pos[q.r0 + tok - slot0];
+        c.sums[at] = 0.0f;
+    }
+    // The run's first workgroup, which has read the tail, leaves the rows of the block that is open now in it.
+    if (rest != 0 || !tail_ok) return;
+    __syncthreads();
+    const int last = (q.len - 1) / c.block * c.block;    // first token of that block
+    const int lpage = b.pages[(size_t)s * b.max_pages + last / kPage];
+    const bool lpage_ok = lpage >= 0 && lpage < c.n_pages;
+    if (last == open && is_old && !raw && page_ok)       // rows only the cache had, at their values there
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (j * 64 + col + e < c.dim) c.tail[tail_at + (size_t)(tok - open) * c.dim + j * 64 + col + e] = r[j][e];
+    const int from = max(last, slot0), n = (q.len - from) * c.dim;
+    for (int i = tid; i < n; i += kThreads) {
+        const int o = i / c.dim, d = i % c.dim;
+        c.tail[tail_at + (size_t)(from - last + o) * c.dim + d] = x[(size_t)(q.r0 + from - slot0 + o) * stride + (size_t)h * c.dim + d];
+    }
+    if (tid == 0) {
+        tag[0] = lpage_ok ? lpage * subs + last % kPage / c.block : -1;
+        tag[1] = q.len - last;
+    }
+}
+
+}  // namespace
+
+void launch_write_kv8(const Kv8Cache& c, const Kv8Batch& b, const int32_t* slots, const float* k, size_t k_stride,
+                      const float* v, size_t v_stride, hipStream_t stream) {
+    // a run of n rows touches at most n and at most n / 64 + 2 pages
+    const unsigned pages = (unsigned)std::min<size_t>((size_t)b.rows, (size_t)b.rows / kPage + 2 * (size_t)b.n_seq);
+    hipLaunchKernelGGL(write_kv8_kernel, dim3(pages, (unsigned)c.n_kv, 2), dim3(kThreads), 0, stream, c, b, slots, k,
+                       k_stride, v, v_stride);
+}
+
+}  // namespace infr
