@@ -687,9 +687,9 @@ static uint32_t kv8_max_tensor(const infr_hip_op_t& op) {
 }
 
 // Scratch an op of this shape needs.
-static size_t kv8_scratch(int kind, const infr_hip_kv8_params_t& p) {
+static size_t kv8_scratch(const infr_hip_t* be, int kind, const infr_hip_kv8_params_t& p) {
     return kind == INFR_OP_ATTENTION_KV8
-               ? infr::attention_kv8_scratch((int)p.head_dim, (int)p.n_kv, (int)(p.n_head / p.n_kv), (int)p.n_seq, (int)p.max_q, (int)p.max_pages)
+               ? infr::attention_kv8_scratch(be->props.multiProcessorCount, (int)p.head_dim, (int)p.n_kv, (int)(p.n_head / p.n_kv), (int)p.n_seq, (int)p.max_q, (int)p.max_pages)
                : 0;
 }
 
@@ -714,10 +714,10 @@ static int ensure_kv8_ws(infr_hip_t* be, size_t bytes) {
 }
 
 static int enqueue_kv8(infr_hip_t* be, int kind, const infr_hip_kv8_params_t& p, const Kv8Args& k) {
-    if (kv8_scratch(kind, p) > be->kv8_ws_bytes) return fail(be, INFR_HIP_ERR_OTHER, "attention_kv8: scratch was not sized");
+    if (kv8_scratch(be, kind, p) > be->kv8_ws_bytes) return fail(be, INFR_HIP_ERR_OTHER, "attention_kv8: scratch was not sized");
     switch (kind) {
     case INFR_OP_WRITE_KV8: infr::launch_write_kv8(k.c, k.b, k.slots, k.x, k.x_stride, k.v, k.v_stride, be->stream); break;
-    case INFR_OP_ATTENTION_KV8: infr::launch_attention_kv8(k.c, k.b, k.a, k.dst, k.lse, be->kv8_ws, be->stream); break;
+    case INFR_OP_ATTENTION_KV8: infr::launch_attention_kv8(k.c, k.b, k.a, k.dst, k.lse, be->kv8_ws, be->props.multiProcessorCount, be->stream); break;
     case INFR_OP_SCORE_KV8: infr::launch_score_kv8(k.c, k.b, k.a, k.lse, p.decay, be->stream); break;
     default: infr::launch_evict_kv8(k.c, k.e, be->stream); break;
     }
@@ -1204,7 +1204,7 @@ static int run_kv8(infr_hip_t* be, int kind, const infr_hip_kv8_params_t* p, con
     if (int rc = check_latch(be)) return rc;
     Kv8Args k;
     if (int rc = check_kv8(be, kind, *p, *o, &k)) return rc;
-    if (int rc = ensure_kv8_ws(be, kv8_scratch(kind, *p))) return rc;
+    if (int rc = ensure_kv8_ws(be, kv8_scratch(be, kind, *p))) return rc;
     return enqueue_kv8(be, kind, *p, k);
 }
 
@@ -1297,7 +1297,7 @@ int infr_hip_compile(infr_hip_t* be, const infr_hip_op_t* ops, size_t n_ops, inf
                 return fail(be, INFR_HIP_ERR_UNSUPPORTED, std::string("compile: 8-bit KV cache op: ") + msg);
             }
             p->max_tensor = std::max(p->max_tensor, kv8_max_tensor(op));
-            kv8_need = std::max(kv8_need, kv8_scratch(op.kind, op.kv));
+            kv8_need = std::max(kv8_need, kv8_scratch(be, op.kind, op.kv));
         } else {
             delete p;
             return fail(be, INFR_HIP_ERR_UNSUPPORTED, "compile: op kind " + std::to_string(op.kind));

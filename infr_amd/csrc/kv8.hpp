@@ -65,10 +65,10 @@ struct Kv8Evict {
 
 void launch_write_kv8(const Kv8Cache& c, const Kv8Batch& b, const int32_t* slots, const float* k, size_t k_stride,
                       const float* v, size_t v_stride, hipStream_t stream);
-// f32 scratch an attention launch needs, in bytes.
-size_t attention_kv8_scratch(int dim, int n_kv, int group, int n_seq, int max_q, int max_pages);
+// f32 scratch an attention launch needs on a device of `cus` compute units, in bytes.
+size_t attention_kv8_scratch(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages);
 void launch_attention_kv8(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, void* scratch,
-                          hipStream_t stream);
+                          int cus, hipStream_t stream);
 void launch_score_kv8(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, const float* lse, float decay,
                       hipStream_t stream);
 void launch_evict_kv8(const Kv8Cache& c, const Kv8Evict& e, hipStream_t stream);

@@ -1,5 +1,5 @@
 // AttentionKv8 and ScoreKv8, one wave per query row and head: lane t holds token t of a page.
-#include "kv8.hpp"
+#include "kv8_attn.hpp"
 
 namespace infr {
 
@@ -38,55 +38,6 @@ __device__ __forceinline__ float dot_of(const Kv8Cache& c, const float* q, int p
     return acc * c.ks[((size_t)page * c.n_kv + h) * (kPage / c.block) + t / c.block];
 }
 
-__global__ __launch_bounds__(64) void attention_rows_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a, float* __restrict__ dst,
-                                                            float* __restrict__ lse) {
-    const int s = blockIdx.z, head = blockIdx.y, i = blockIdx.x, lane = threadIdx.x, h = head / a.group;
-    const Kv8Seq q = kv8_seq(b, s);
-    if (i >= q.n) return;
-    float* out = dst + ((size_t)(q.r0 + i) * a.n_head + head) * c.dim;
-    const float* qr = a.q + (size_t)(q.r0 + i) * a.q_stride + (size_t)head * c.dim;
-    float o[4] = {0, 0, 0, 0}, m = -__builtin_inff(), l = 0.0f;
-    bool bad = !q.ok;
-    if (q.ok) {
-        const RowSees sees = row_sees(b, a, q, s, i);
-        for (int p = 0; p * kPage < q.len; ++p) {
-            const int page = b.pages[(size_t)s * b.max_pages + p];
-            if (page < 0 || page >= c.n_pages) {
-                bad = true;
-                break;
-            }
-            const int j = p * kPage + lane;
-            const int kpos = c.pos[((size_t)page * c.n_kv + h) * kPage + lane];
-            const bool see = sees(j, kpos);
-            const float x = see ? score_of(a, dot_of(c, qr, page, h, lane), head, sees.pos, kpos) : -__builtin_inff();
-            float top = x;
-            bool nan = see && x != x;
-            for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
-            if (__ballot(nan)) bad = true;
-            if (!__ballot(see)) continue;
-            const float m2 = fmaxf(m, top), keep = expf(m - m2);
-            const float w = see ? expf(x - m2) : 0.0f;
-            float sum = w;
-            for (int k = 1; k < 64; k <<= 1) sum += __shfl_xor(sum, k);
-            l = l * keep + sum;
-            m = m2;
-            for (int e = 0; e < 4; ++e) {
-                const int d = e * 64 + lane;
-                o[e] *= keep;
-                for (int t = 0; t < 64; ++t) {
-                    const float wt = __shfl(w, t);
-                    if (wt == 0.0f || d >= c.dim) continue;
-                    const float vs = c.vs[((size_t)page * c.n_kv + h) * (kPage / c.block) + t / c.block];
-                    o[e] = __builtin_fmaf(wt, kv8_value(c.v[v_at(c, page, h, t, d)], c.f8 != 0) * vs, o[e]);
-                }
-            }
-        }
-    }
-    for (int e = 0; e < 4; ++e)
-        if (e * 64 + lane < c.dim) out[e * 64 + lane] = bad ? __builtin_nanf("") : l > 0.0f ? o[e] / l : l == 0.0f ? 0.0f : l;
-    if (lse && lane == 0) lse[(size_t)(q.r0 + i) * a.n_head + head] = bad ? __builtin_nanf("") : m + logf(l);
-}
-
 __global__ __launch_bounds__(64) void score_rows_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a, const float* __restrict__ lse,
                                                         float decay) {
     const int s = blockIdx.z, h = blockIdx.y, p = blockIdx.x, lane = threadIdx.x;
@@ -112,12 +63,13 @@ __global__ __launch_bounds__(64) void score_rows_kernel(Kv8Cache c, Kv8Batch b, 
 
 }  // namespace
 
-size_t attention_kv8_scratch(int, int, int, int, int, int) { return 0; }
+size_t attention_kv8_scratch(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages) {
+    return step_scratch(cus, dim, n_kv, group, n_seq, max_q, max_pages);
+}
 
-void launch_attention_kv8(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, void*,
+void launch_attention_kv8(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, void* scratch, int cus,
                           hipStream_t stream) {
-    hipLaunchKernelGGL(attention_rows_kernel, dim3((unsigned)b.max_q, (unsigned)a.n_head, (unsigned)b.n_seq), dim3(64), 0,
-                       stream, c, b, a, dst, lse);
+    launch_attention_step(c, b, a, dst, lse, static_cast<float*>(scratch), cus, stream);
 }
 
 void launch_score_kv8(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, const float* lse, float decay,

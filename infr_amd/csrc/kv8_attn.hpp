@@ -1,0 +1,16 @@
+// The two forms of AttentionKv8: few rows per sequence (kv8_step.hip) and many (kv8_prompt.hip).
+#pragma once
+
+#include <algorithm>
+
+#include "kv8.hpp"
+
+namespace infr {
+
+int step_target(int cus);
+size_t step_items(int cus, int n_kv, int group, int n_seq, int max_q, int max_pages);
+size_t step_scratch(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages);
+void launch_attention_step(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch,
+                           int cus, hipStream_t stream);
+
+}  // namespace infr

@@ -1,0 +1,117 @@
+// Device pieces that the kernels reading the 8-bit KV cache share: codes to f16, f32 operands as two f16
+// numbers, the scores' softcap, bias and masks.
+//
+// Matrix products run on the f16 MFMA. Every code of either type is exact in f16; an f32 operand x goes in as
+// hi + lo, hi = f16(x) and lo = f16(x - hi), two products instead of one, so that 22 bits of it count (f16 alone
+// would leave 11, which shows in an f32 result). Query rows are scaled by a power of two that puts their largest
+// value at 2^14, softmax weights by 2^10, so that the smallest f16 number stands far below what counts.
+//
+// Layouts follow from S^T = K Q^T: with tokens as the MFMA's rows and query rows as its columns, a lane's scores
+// all belong to one query row, the softmax statistics of a row live in the lanes that hold its output, and the
+// weights are P.V's operand where they stand: no exchange between lanes but the maximum's.
+#pragma once
+
+#include "kv8.hpp"
+
+namespace infr {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16x __attribute__((ext_vector_type(16)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNoMax = -3.4028234e38f;  // running maximum before the first token: finite, so that -inf - it is -inf
+
+// Two codes (bytes 2 * word, 2 * word + 1 of c) as f16.
+template <bool F8>
+__device__ __forceinline__ h2 code_pair(uint32_t c, int word) {
+    if constexpr (F8) {
+        return word ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.0f, false);
+    } else {
+        // 0x6400 | u is 1024 + u; with u = code + 128 the difference to 1152 is the code, exactly
+        const uint32_t u = __builtin_amdgcn_perm(0x64646464u, c ^ 0x80808080u, word ? 0x04030402u : 0x04010400u);
+        return __builtin_bit_cast(h2, u) - (h2)(_Float16)1152.0f;
+    }
+}
+template <bool F8>
+__device__ __forceinline__ h8 code_oct(uint32_t a, uint32_t b) {
+    const h2 p = code_pair<F8>(a, 0), q = code_pair<F8>(a, 1), r = code_pair<F8>(b, 0), s = code_pair<F8>(b, 1);
+    return h8{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
+}
+
+// a, b = hi + lo, both rounded towards zero (one instruction for two numbers): 22 bits of each remain.
+__device__ __forceinline__ void split_pair(float a, float b, h2* hi, h2* lo) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    const auto l = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], -1.0f, a), __builtin_fmaf((float)h[1], -1.0f, b));
+    *hi = __builtin_bit_cast(h2, h);
+    *lo = __builtin_bit_cast(h2, l);
+}
+
+// Maximum / sum over lanes l, l ^ 16, l ^ 32, l ^ 48.
+template <typename F>
+__device__ __forceinline__ float across_quads(float x, F f) {
+    // (the elements are copied before they are reinterpreted: a bit cast of a vector's element reads its first one)
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t a = r[0], b = r[1];
+    const uint32_t w = __builtin_bit_cast(uint32_t, f(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+    const auto q = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+    const uint32_t c = q[0], d = q[1];
+    return f(__builtin_bit_cast(float, c), __builtin_bit_cast(float, d));
+}
+__device__ __forceinline__ float quads_max(float x) {
+    return across_quads(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float quads_sum(float x) {
+    return across_quads(x, [](float a, float b) { return a + b; });
+}
+
+// Power of two that brings a query row with this largest |value| to 2^14; rows of zeros and of values too small
+// or too large for it get the nearest that keeps every factor a normal number.
+__device__ __forceinline__ int row_exponent(uint32_t amax_bits) {
+    const int e = (int)(amax_bits >> 23) - 127 - 14;
+    return min(max(e, -100), 114);
+}
+__device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
+
+// c * tanh(s / c), to the last bits of s: an odd polynomial (the series of tanh) where tanh is nearly its
+// argument, 1 - 2 / (e^2y + 1) beyond, where the difference cancels no more than two bits.
+__device__ __forceinline__ float cap_score(float s, float c, float inv_c) {
+    const float y = s * inv_c, z = y * y;
+    float p = -1382.0f / 155925.0f;
+    p = __builtin_fmaf(p, z, 62.0f / 2835.0f);
+    p = __builtin_fmaf(p, z, -17.0f / 315.0f);
+    p = __builtin_fmaf(p, z, 2.0f / 15.0f);
+    p = __builtin_fmaf(p, z, -1.0f / 3.0f);
+    const float near = __builtin_fmaf(s * z, p, s);
+    const float a = fabsf(y);
+    if (__all(a < 0.35f)) return near;
+    const float e = __builtin_amdgcn_exp2f(a * (2.0f * kLog2e));
+    const float far = __builtin_copysignf(c * (1.0f - 2.0f / (e + 1.0f)), s);
+    return a < 0.35f ? near : a >= 0.35f ? far : s;  // NaN stays
+}
+
+// What one query row sees, and its bias.
+struct Kv8Row {
+    int slot, pos, first, prefix, window;  // slot: last token by causality; prefix: positions below it are seen always
+    float slope;                           // times log2 e; 0: none
+    __device__ __forceinline__ bool sees(int token, int kpos) const {
+        return (token <= slot || kpos < prefix) && pos - kpos < window && kpos >= first;
+    }
+};
+// Row i of sequence s, head `head`. Positions are taken to lie in [0, 2^30].
+__device__ __forceinline__ Kv8Row kv8_row(const Kv8Batch& b, const Kv8Attn& a, const Kv8Seq& q, int s, int i, int head) {
+    Kv8Row r;
+    r.slot = a.causal ? q.len - q.n + i : 0x7FFFFFFF;
+    r.pos = b.pos[q.r0 + i];
+    r.first = a.first ? a.first[q.r0 + i] : -0x7FFFFFFF - 1;
+    r.prefix = a.prefix ? a.prefix[s] : -0x7FFFFFFF - 1;
+    r.window = a.window > 0 ? a.window : 0x7FFFFFFF;
+    r.slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+    return r;
+}
+
+}  // namespace infr

@@ -1,0 +1,425 @@
+// AttentionKv8 for few rows per sequence: decode steps and drafts. Bound by reading the cache once.
+//
+// Up to 16 query rows of one (sequence, KV head) - its rows times the heads of the group - are one column tile of
+// the 16x16x32 f16 MFMA. A wave takes one page at a time: 64 tokens as four row tiles chosen so that lane group g
+// holds tokens 16 g .. 16 g + 15 of its query row, which is what P.V wants side by side from V^T's 16-byte pieces.
+// Key and value codes go from HBM to registers in 16-byte loads (whole lines per instruction), become f16 there and
+// feed the MFMA; the next page's keys are requested before the current page's softmax, its values before its scores.
+//
+// The pages of all sequences are cut into pieces of one size, found on the device from the lengths: long sequences
+// get many workgroups, short ones one, and no piece is empty. A sequence in one piece writes its result; the pieces
+// of others are joined by a second kernel, in their order.
+#include "kv8_attn.hpp"
+#include "kv8_device.hpp"
+
+namespace infr {
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kRows = 16;
+constexpr int kBias = 10;    // softmax weights are 2^kBias at the running maximum ..
+constexpr float kLag = 4.0f; // .. which may lag behind the true one by this many powers of two
+
+// How the batch's pages are cut.
+struct Cut {
+    int s, h, rt, part;    // sequence, KV head, row tile, piece
+    int parts, item;       // pieces of this (sequence, head, row tile); number of the first one in the scratch
+    int p0, p1;            // pages of the piece
+};
+
+struct SeqWork {
+    int tiles, p_lo, pages;  // row tiles, first page any row sees, pages from there
+};
+__device__ __forceinline__ SeqWork seq_work(const Kv8Batch& b, const Kv8Attn& a, int s) {
+    const Kv8Seq q = kv8_seq(b, s);
+    SeqWork w;
+    w.tiles = (q.n * a.group + kRows - 1) / kRows;
+    if (!q.ok) {  // one item per tile writes the rows' NaN
+        w.p_lo = 0;
+        w.pages = 1;
+        return w;
+    }
+    // positions ascend with the tokens, so a token `window` or more tokens back is outside the window
+    const int lo = a.window > 0 ? max(q.len - q.n - a.window + 1, 0) : 0;
+    w.p_lo = lo / kPage;
+    w.pages = max((q.len + kPage - 1) / kPage - w.p_lo, 1);
+    return w;
+}
+// Pages per piece: about `target` pieces in all, at least one page for each wave of a workgroup.
+__device__ __forceinline__ int piece_pages(const Kv8Batch& b, const Kv8Attn& a, int n_kv, int target) {
+    const int lane = threadIdx.x & 63;
+    float total = 0.0f;
+    for (int s = lane; s < b.n_seq; s += 64) {
+        const SeqWork w = seq_work(b, a, s);
+        total += (float)w.tiles * (float)w.pages;
+    }
+    for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
+    return max((int)__builtin_ceilf(total * (float)n_kv / (float)target), kWaves);
+}
+
+// O, maximum and sum of a piece: f32 [rows][DP], then [rows] maxima and [rows] sums.
+template <int DP>
+constexpr int kPieceFloats = kRows * DP + 2 * kRows;
+
+template <int DP, bool F8, bool GEN>
+__global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void step_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a,
+                                                                             float* __restrict__ dst, float* __restrict__ lse,
+                                                                             float* __restrict__ scratch, int target) {
+    constexpr int kCols = DP / 64;   // 64-column groups of a key
+    constexpr int kOut = DP / 16;    // 16-column groups of a value
+    __shared__ float part_o[kWaves][kRows * (DP + 4)];
+    __shared__ float part_m[kWaves][kRows], part_l[kWaves][kRows];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+    const int cp = piece_pages(b, a, c.n_kv, target);
+    int rest = 0;
+    const int s = find_seq(b.n_seq, (int)blockIdx.x, &rest, [&](int i) {
+        const SeqWork w = seq_work(b, a, i);
+        return c.n_kv * w.tiles * ((w.pages + cp - 1) / cp);
+    });
+    if (s < 0) return;
+    const Kv8Seq q = kv8_seq(b, s);
+    const SeqWork work = seq_work(b, a, s);
+    const int parts = (work.pages + cp - 1) / cp, part = rest % parts, rt = rest / parts % work.tiles, h = rest / parts / work.tiles;
+    const int per = (work.pages + parts - 1) / parts;
+    const int p0 = work.p_lo + part * per;
+    const int p1 = q.ok ? min(p0 + per, (q.len + kPage - 1) / kPage) : p0;
+    const int n_rows = q.n * a.group;
+    const int rr = rt * kRows + col;                   // this lane's query row
+    const bool live = rr < n_rows;
+    const int i = live ? rr / a.group : q.n - 1, head = h * a.group + (live ? rr % a.group : 0);
+
+    // the query row, scaled by a power of two, as hi + lo
+    h8 qh[2 * kCols], ql[2 * kCols];
+    float row_factor;
+    {
+        const float* x = a.q + (size_t)(q.r0 + i) * a.q_stride + (size_t)head * c.dim;
+        float v[16 * kCols];
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < kCols; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int d = j * 64 + g * 16 + e;
+                v[j * 16 + e] = live && d < c.dim ? x[d] : 0.0f;
+                top = max(top, abs_bits(v[j * 16 + e]));
+            }
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+        const int e = row_exponent(top);
+        const float down = pow2(-e);
+        row_factor = a.scale * pow2(e);
+#pragma unroll
+        for (int k = 0; k < 2 * kCols; ++k)
+#pragma unroll
+            for (int o = 0; o < 4; ++o) {
+                h2 hi, lo;
+                split_pair(v[k * 8 + 2 * o] * down, v[k * 8 + 2 * o + 1] * down, &hi, &lo);
+                qh[k][2 * o] = hi[0], qh[k][2 * o + 1] = hi[1];
+                ql[k][2 * o] = lo[0], ql[k][2 * o + 1] = lo[1];
+            }
+    }
+    const Kv8Row row = kv8_row(b, a, q, s, i, head);
+    const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+    const bool use_pos = GEN && (a.window > 0 || a.slopes || a.first || a.prefix);
+    // tokens below this one are seen by every row of the tile (without masks by position)
+    const int all_see = a.causal ? q.len - q.n + rt * kRows / a.group + 1 : q.len;
+
+    f4 o[kOut];
+#pragma unroll
+    for (int k = 0; k < kOut; ++k) o[k] = f4{0, 0, 0, 0};
+    float top = kNoMax, sum = 0.0f;
+    int v_exp = -200;       // values are scaled by 2^-v_exp
+    bool bad = !q.ok;
+
+    const int32_t* table = b.pages + (size_t)s * b.max_pages;
+    const int subs = kPage / c.block;
+    const uint32_t kv_stride = (uint32_t)DP * kPage;
+    uint4 kf[4][kCols], vf[kOut];
+    float ks = 0.0f, vs = 0.0f;
+    int page = 0, ids = 0;
+    // lane n holds the wave's n-th next page
+    auto load_ids = [&](int p) {
+        const int at = p + lane * kWaves;
+        ids = at < p1 ? table[at] : 0;
+        if (ids < 0 || ids >= c.n_pages) ids = -1;
+        if (__any(ids < 0)) bad = true;
+    };
+    auto load_keys = [&](int n) {
+        page = max(__builtin_amdgcn_readlane(ids, n), 0);
+        const uint8_t* kp = c.k + ((size_t)page * c.n_kv + h) * kv_stride + (16 * (col >> 2) + (col & 3)) * 64 + 16 * g;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < kCols; ++j) kf[t][j] = *reinterpret_cast<const uint4*>(kp + j * kPage * 64 + t * 4 * 64);
+        const size_t sc = ((size_t)page * c.n_kv + h) * subs + g * 16 / c.block;
+        ks = c.ks[sc];
+        vs = c.vs[sc];
+    };
+    int p = p0 + wave, n = 0;
+    if (p < p1) {
+        load_ids(p);
+        load_keys(0);
+    }
+    while (p < p1) {
+        const uint8_t* vp = c.v + ((size_t)page * c.n_kv + h) * kv_stride + col * kPage + 16 * g;
+#pragma unroll
+        for (int k = 0; k < kOut; ++k) vf[k] = *reinterpret_cast<const uint4*>(vp + k * 16 * kPage);
+        int kpos[16];
+        if (use_pos) {
+            const int4* pp = reinterpret_cast<const int4*>(c.pos + ((size_t)page * c.n_kv + h) * kPage + 16 * g);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int4 x = pp[t];
+                kpos[4 * t] = x.x, kpos[4 * t + 1] = x.y, kpos[4 * t + 2] = x.z, kpos[4 * t + 3] = x.w;
+            }
+        }
+        // scores: sc[t][i] is token 16 g + 4 t + i of the page
+        f4 sc[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            sc[t] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < kCols; ++j) {
+                const h8 lo = code_oct<F8>(kf[t][j].x, kf[t][j].y), hi = code_oct<F8>(kf[t][j].z, kf[t][j].w);
+                sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, qh[2 * j], sc[t], 0, 0, 0);
+                sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qh[2 * j + 1], sc[t], 0, 0, 0);
+                sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, ql[2 * j], sc[t], 0, 0, 0);
+                sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ql[2 * j + 1], sc[t], 0, 0, 0);
+            }
+        }
+        const int tok0 = p * kPage + 16 * g;
+        const float factor = row_factor * ks;
+        const float vs_now = vs;
+        const bool tail = (p + 1) * kPage > q.len;
+        // the next page's keys are on their way from here
+        const int np = p + kWaves;
+        if (np < p1) {
+            if (++n == 64) {
+                load_ids(np);
+                n = 0;
+            }
+            load_keys(n);
+        }
+        const bool masked = use_pos || (p + 1) * kPage > all_see || tail;
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            float v = sc[e / 4][e % 4] * factor;
+            if (GEN && a.softcap > 0.0f) v = cap_score(v, a.softcap, inv_cap);
+            v *= kLog2e;
+            if (GEN && a.slopes) v -= row.slope * fabsf((float)(row.pos - kpos[e]));
+            x[e] = v;
+        }
+        uint32_t see = 0xFFFFu;
+        if (masked) {
+            see = 0;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int tok = tok0 + e;
+                const bool yes = tok < q.len && (use_pos ? row.sees(tok, kpos[e]) : tok <= row.slot);
+                see |= (yes ? 1u : 0u) << e;
+                x[e] = yes ? x[e] : -__builtin_inff();
+            }
+        }
+        float high = x[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) high = fmaxf(high, x[e]);
+        // the scale of this lane's values, as a power of two times 1 .. 2
+        const int e_now = (vs_now < __builtin_inff() && see) ? (int)((__builtin_bit_cast(uint32_t, vs_now) >> 23) & 255u) - 127 : -200;
+        if (__any(high > top + kLag || e_now > v_exp)) {
+            const float new_top = fmaxf(top, quads_max(high));
+            const int new_exp = max(v_exp, (int)quads_max((float)e_now));
+            const float keep = __builtin_amdgcn_exp2f(top - new_top);
+            const float keep_o = v_exp == -200 ? 0.0f : keep * __builtin_amdgcn_exp2f((float)(v_exp - new_exp));
+            sum *= keep;
+#pragma unroll
+            for (int k = 0; k < kOut; ++k) o[k] *= keep_o;
+            top = new_top;
+            v_exp = new_exp;
+        }
+        const float ratio = vs_now * __builtin_amdgcn_exp2f(-(float)max(v_exp, -126));
+        const float base = (float)kBias - top;
+        float w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float pe = __builtin_amdgcn_exp2f(x[e] + base);
+            sum += pe;
+            w[e] = pe * ratio;
+        }
+        if (masked)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[e] = (see >> e) & 1u ? w[e] : 0.0f;
+        h8 wh[2], wl[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                h2 hi, lo;
+                split_pair(w[8 * k + 2 * e], w[8 * k + 2 * e + 1], &hi, &lo);
+                wh[k][2 * e] = hi[0], wh[k][2 * e + 1] = hi[1];
+                wl[k][2 * e] = lo[0], wl[k][2 * e + 1] = lo[1];
+            }
+        if (F8 && tail) {  // what stands behind the last token may be NaN as a code
+            const int left = min(max(q.len - tok0, 0), 16);
+#pragma unroll
+            for (int k = 0; k < kOut; ++k) {
+                uint32_t* u = reinterpret_cast<uint32_t*>(&vf[k]);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const int m = min(max(left - 4 * t, 0), 4);
+                    u[t] = m == 4 ? u[t] : u[t] & ((1u << (8 * m)) - 1u);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kOut; ++k) {
+            const h8 lo = code_oct<F8>(vf[k].x, vf[k].y), hi = code_oct<F8>(vf[k].z, vf[k].w);
+            o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wh[0], o[k], 0, 0, 0);
+            o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wh[1], o[k], 0, 0, 0);
+            o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wl[0], o[k], 0, 0, 0);
+            o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wl[1], o[k], 0, 0, 0);
+        }
+        p = np;
+    }
+    // the waves' results as one: largest maximum, everything scaled to it
+    sum = quads_sum(sum);
+    if (g == 0) {
+        part_m[wave][col] = top;
+        part_l[wave][col] = sum;
+    }
+    const bool any_bad = __syncthreads_or(bad) != 0;
+    float all_top = kNoMax;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) all_top = fmaxf(all_top, part_m[k][col]);
+    // (a wave that has seen nothing has sum 0 and O 0; exp2 of its maximum's distance is 0)
+    const float mine = __builtin_amdgcn_exp2f(top - all_top) * (v_exp == -200 ? 0.0f : __builtin_amdgcn_exp2f((float)v_exp));
+#pragma unroll
+    for (int k = 0; k < kOut; ++k) *reinterpret_cast<f4*>(&part_o[wave][col * (DP + 4) + k * 16 + 4 * g]) = o[k] * mine;
+    __syncthreads();
+    const bool whole = parts == 1;
+    float* piece = whole ? nullptr : scratch + (size_t)blockIdx.x * kPieceFloats<DP>;
+    const float nan = __builtin_nanf("");
+    for (int at = threadIdx.x; at < kRows * DP; at += 64 * kWaves) {
+        const int r = at / DP, d = at % DP, r_all = rt * kRows + r;
+        if (r_all >= n_rows) continue;
+        float x = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) x += part_o[k][r * (DP + 4) + d];
+        if (!whole) {
+            piece[at] = any_bad ? nan : x;
+            continue;
+        }
+        if (d >= c.dim) continue;
+        float m = kNoMax, l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) m = fmaxf(m, part_m[k][r]);
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) l += part_l[k][r] * __builtin_amdgcn_exp2f(part_m[k][r] - m);
+        dst[((size_t)(q.r0 + r_all / a.group) * a.n_head + h * a.group + r_all % a.group) * c.dim + d] =
+            any_bad ? nan : l == 0.0f ? 0.0f : x / l;
+    }
+    if (threadIdx.x < kRows && rt * kRows + (int)threadIdx.x < n_rows) {
+        const int r = threadIdx.x, r_all = rt * kRows + r;
+        float m = kNoMax, l = 0.0f;
+        for (int k = 0; k < kWaves; ++k) m = fmaxf(m, part_m[k][r]);
+        for (int k = 0; k < kWaves; ++k) l += part_l[k][r] * __builtin_amdgcn_exp2f(part_m[k][r] - m);
+        if (!whole) {
+            piece[kRows * DP + r] = m;
+            piece[kRows * DP + kRows + r] = any_bad ? nan : l;
+        } else if (lse) {
+            lse[(size_t)(q.r0 + r_all / a.group) * a.n_head + h * a.group + r_all % a.group] =
+                any_bad ? nan : l == 0.0f ? -__builtin_inff() : (__builtin_amdgcn_logf(l) + m - (float)kBias) * kLn2;
+        }
+    }
+}
+
+// Joins the pieces of one query row: blockIdx.x counts (sequence, head, row tile), blockIdx.y the row in the tile.
+template <int DP>
+__global__ __launch_bounds__(256) void join_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a, float* __restrict__ dst,
+                                                   float* __restrict__ lse, const float* __restrict__ scratch, int target,
+                                                   int max_tiles) {
+    __shared__ float part[256];
+    const int lane = threadIdx.x & 63;
+    const int rt = blockIdx.x % max_tiles, h = blockIdx.x / max_tiles % c.n_kv, s = blockIdx.x / max_tiles / c.n_kv;
+    const int r = blockIdx.y, r_all = rt * kRows + r;
+    const Kv8Seq q = kv8_seq(b, s);
+    if (r_all >= q.n * a.group) return;
+    const int cp = piece_pages(b, a, c.n_kv, target);
+    const SeqWork work = seq_work(b, a, s);
+    const int parts = (work.pages + cp - 1) / cp;
+    if (parts == 1) return;
+    int before = 0;
+    for (int k = lane; k < s; k += 64) {
+        const SeqWork w = seq_work(b, a, k);
+        before += c.n_kv * w.tiles * ((w.pages + cp - 1) / cp);
+    }
+    for (int o = 1; o < 64; o <<= 1) before += __shfl_xor(before, o);
+    const float* first = scratch + (size_t)(before + (h * work.tiles + rt) * parts) * kPieceFloats<DP>;
+    auto max_of = [&](int k) { return first[(size_t)k * kPieceFloats<DP> + kRows * DP + r]; };
+    auto sum_of = [&](int k) { return first[(size_t)k * kPieceFloats<DP> + kRows * DP + kRows + r]; };
+    float m = kNoMax;
+    for (int k = lane; k < parts; k += 64) m = fmaxf(m, max_of(k));
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    float l = 0.0f;
+    for (int k = lane; k < parts; k += 64) l += sum_of(k) * __builtin_amdgcn_exp2f(max_of(k) - m);
+    for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
+    const size_t out = (size_t)(q.r0 + r_all / a.group) * a.n_head + h * a.group + r_all % a.group;
+    if (lse && threadIdx.x == 0)
+        lse[out] = l == 0.0f ? -__builtin_inff() : (__builtin_amdgcn_logf(l) + m - (float)kBias) * kLn2;
+    constexpr int kGroups = 256 / DP;  // threads that share a column, each every kGroups-th piece
+    const int d = threadIdx.x % DP, first_k = threadIdx.x / DP;
+    float x = 0.0f;
+    if (first_k < kGroups)
+        for (int k = first_k; k < parts; k += kGroups)
+            x += first[(size_t)k * kPieceFloats<DP> + r * DP + d] * __builtin_amdgcn_exp2f(max_of(k) - m);
+    part[threadIdx.x] = x;
+    __syncthreads();
+    if ((int)threadIdx.x >= DP || d >= c.dim) return;
+    x = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) x += part[k * DP + d];
+    dst[out * c.dim + d] = l == 0.0f ? 0.0f : x / l;
+}
+
+int max_tiles_of(int group, int max_q) { return (int)(((int64_t)max_q * group + kRows - 1) / kRows); }
+
+template <int DP>
+void launch_step_dp(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch, int cus,
+                    hipStream_t stream) {
+    const int target = step_target(cus), tiles = max_tiles_of(a.group, b.max_q);
+    const bool gen = a.softcap > 0.0f || a.window > 0 || a.slopes || a.first || a.prefix;
+    const unsigned items = (unsigned)step_items(cus, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);
+    auto kernel = c.f8 ? (gen ? step_kernel<DP, true, true> : step_kernel<DP, true, false>)
+                       : (gen ? step_kernel<DP, false, true> : step_kernel<DP, false, false>);
+    hipLaunchKernelGGL(kernel, dim3(items), dim3(64 * kWaves), 0, stream, c, b, a, dst, lse, scratch, target);
+    if (b.max_pages <= kWaves) return;  // no sequence has two pieces
+    hipLaunchKernelGGL(join_kernel<DP>, dim3((unsigned)(b.n_seq * c.n_kv * tiles), (unsigned)std::min(kRows, b.max_q * a.group)),
+                       dim3(256), 0, stream, c, b, a, dst, lse, scratch, target, tiles);
+}
+
+}  // namespace
+
+// Pieces aimed at: two workgroups for each compute unit.
+int step_target(int cus) { return 2 * cus; }
+// Upper bound of the pieces: the total is cut into `target`, and each (sequence, head, row tile) rounds up once.
+size_t step_items(int cus, int n_kv, int group, int n_seq, int max_q, int max_pages) {
+    const size_t tiles = (size_t)n_seq * n_kv * max_tiles_of(group, max_q);
+    return std::min((size_t)step_target(cus) + tiles, tiles * (size_t)((max_pages + kWaves - 1) / kWaves));
+}
+size_t step_scratch(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages) {
+    if (max_pages <= kWaves) return 0;
+    const size_t dp = (size_t)(dim + 63) / 64 * 64;
+    return step_items(cus, n_kv, group, n_seq, max_q, max_pages) * (kRows * dp + 2 * kRows) * sizeof(float);
+}
+void launch_attention_step(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch,
+                           int cus, hipStream_t stream) {
+    switch (c.dp) {
+    case 64: launch_step_dp<64>(c, b, a, dst, lse, scratch, cus, stream); break;
+    case 128: launch_step_dp<128>(c, b, a, dst, lse, scratch, cus, stream); break;
+    case 192: launch_step_dp<192>(c, b, a, dst, lse, scratch, cus, stream); break;
+    default: launch_step_dp<256>(c, b, a, dst, lse, scratch, cus, stream); break;
+    }
+}
+
+}  // namespace infr
