@@ -50,14 +50,25 @@ __device__ __forceinline__ void split_pair(float a, float b, h2* hi, h2* lo) {
     *lo = __builtin_bit_cast(h2, l);
 }
 
-// Maximum / sum over lanes l, l ^ 16, l ^ 32, l ^ 48.
+// f over lanes l and l ^ 32.
 template <typename F>
-__device__ __forceinline__ float across_quads(float x, F f) {
+__device__ __forceinline__ float across_halves(float x, F f) {
     // (the elements are copied before they are reinterpreted: a bit cast of a vector's element reads its first one)
     const uint32_t u = __builtin_bit_cast(uint32_t, x);
     const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
     const uint32_t a = r[0], b = r[1];
-    const uint32_t w = __builtin_bit_cast(uint32_t, f(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+    return f(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+__device__ __forceinline__ float halves_max(float x) {
+    return across_halves(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float halves_sum(float x) {
+    return across_halves(x, [](float a, float b) { return a + b; });
+}
+// Maximum / sum over lanes l, l ^ 16, l ^ 32, l ^ 48.
+template <typename F>
+__device__ __forceinline__ float across_quads(float x, F f) {
+    const uint32_t w = __builtin_bit_cast(uint32_t, across_halves(x, f));
     const auto q = __builtin_amdgcn_permlane16_swap(w, w, false, false);
     const uint32_t c = q[0], d = q[1];
     return f(__builtin_bit_cast(float, c), __builtin_bit_cast(float, d));

@@ -1,0 +1,405 @@
+// AttentionKv8 for many rows per sequence: prompts and their chunks. Bound by the matrix cores: 4 head_dim flops for
+// each pair of row and key that see each other, twice that in f16 products (hi + lo).
+//
+// A workgroup takes 128 query rows of one (sequence, KV head) - tokens times the heads of the group, so that a page
+// of keys serves the whole group - and walks over the pages; each of its four waves owns 32 rows, the columns of the
+// 32x32x16 f16 MFMA. The page's codes become f16 once per workgroup on their way into LDS (two buffers: the next
+// page's codes are requested before the current page is multiplied and written behind it, one barrier a page); a
+// wave's scores, softmax and output stay in its registers. Tokens are dealt to the MFMA's rows so that a lane holds
+// 16 neighbours: one block's scale, and P.V's operand as it stands.
+// Pages no row of the workgroup sees are not visited; pages all rows of a wave see take no mask.
+#include "kv8_attn.hpp"
+#include "kv8_device.hpp"
+
+namespace infr {
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kCols = 32;                // query rows of a wave
+constexpr int kRows = kCols * kWaves;    // and of a workgroup
+constexpr int kBias = 10;
+constexpr float kLag = 4.0f;
+
+template <int DP>
+constexpr int kPieceFloats = kRows * DP + 2 * kRows;
+
+// A page in LDS. Rows are padded by 16 bytes: neighbours then start four banks apart.
+template <int DP>
+struct Stage {
+    _Float16 k[kPage][DP + 8];
+    _Float16 v[DP][kPage + 8];
+    float ks[4], vs[4];    // scales of the four runs of 16 tokens
+    int32_t pos[kPage];
+};
+
+template <int DP, bool F8, bool GEN>
+__global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a,
+                                                                            float* __restrict__ dst, float* __restrict__ lse,
+                                                                            float* __restrict__ scratch, int tiles, int parts) {
+    constexpr int kSteps = DP / 16;  // of the scores' sum
+    constexpr int kOut = DP / 32;    // output tiles
+    constexpr int kLoads = DP / 64;  // 16-byte pieces of K, and of V, that a thread brings in
+    extern __shared__ __align__(16) unsigned char smem[];
+    Stage<DP>* stage = reinterpret_cast<Stage<DP>*>(smem);
+    __shared__ int first_page[kWaves], last_page[kWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, hf = lane >> 5;
+    const int h = blockIdx.x / parts, part = blockIdx.x % parts, s = blockIdx.z;
+    const int rt = tiles - 1 - (int)blockIdx.y;  // causal rows get longer: the long ones start first
+    const Kv8Seq q = kv8_seq(b, s);
+    const int n_rows = q.n * a.group;
+    if (rt * kRows >= n_rows) return;
+    const int rr = rt * kRows + wave * kCols + col;
+    const bool live = rr < n_rows;
+    const int i = live ? rr / a.group : q.n - 1, head = h * a.group + (live ? rr % a.group : 0);
+    const Kv8Row row = kv8_row(b, a, q, s, i, head);
+
+    // Tokens the row can see at all lie in [lo, hi): positions ascend strictly and are not negative, so a token is at
+    // least as far from the row in positions as in tokens, and none with a position below `prefix` lies behind it.
+    int lo = 0x7FFFFFFF, hi = 0;
+    if (live && q.ok) {
+        const int slot = q.len - q.n + i;
+        lo = 0;
+        if (a.window > 0) lo = max(lo, slot - a.window + 1);
+        if (a.first) lo = row.pos >= row.first ? max(lo, slot - (row.pos - row.first)) : 0x7FFFFFFF;
+        hi = a.causal ? max(slot + 1, min(a.prefix ? row.prefix : 0, q.len)) : q.len;
+    }
+    int full_hi = live ? (a.causal ? q.len - q.n + i + 1 : q.len) : 0x7FFFFFFF;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        lo = min(lo, __shfl_xor(lo, o));
+        hi = max(hi, __shfl_xor(hi, o));
+        full_hi = min(full_hi, __shfl_xor(full_hi, o));
+    }
+    // this wave's pages; none when lo >= hi
+    const int w0 = lo < hi ? lo / kPage : 0x7FFFFFFF, w1 = lo < hi ? (hi + kPage - 1) / kPage : 0;
+    if (lane == 0) {
+        first_page[wave] = w0;
+        last_page[wave] = w1;
+    }
+    __syncthreads();
+    int g0 = 0x7FFFFFFF, g1 = 0;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+        g0 = min(g0, first_page[k]);
+        g1 = max(g1, last_page[k]);
+    }
+    int p0 = min(g0, g1), p1 = g1;
+    if (parts > 1) {
+        const int per = (p1 - p0 + parts - 1) / parts;
+        p0 = min(p0 + part * per, p1);
+        p1 = min(p0 + per, p1);
+    }
+
+    h8 qh[kSteps], ql[kSteps];
+    float row_factor;
+    {
+        const float* x = a.q + (size_t)(q.r0 + i) * a.q_stride + (size_t)head * c.dim;
+        uint32_t top = 0;
+        for (int d = hf * 8; d < c.dim; d += 16)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (live && d + e < c.dim) top = max(top, abs_bits(x[d + e]));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+        const int e2 = row_exponent(top);
+        const float down = pow2(-e2);
+        row_factor = a.scale * pow2(e2);
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int d = k * 16 + hf * 8 + e;
+                v[e] = live && d < c.dim ? x[d] * down : 0.0f;
+            }
+#pragma unroll
+            for (int o = 0; o < 4; ++o) {
+                h2 u, w;
+                split_pair(v[2 * o], v[2 * o + 1], &u, &w);
+                qh[k][2 * o] = u[0], qh[k][2 * o + 1] = u[1];
+                ql[k][2 * o] = w[0], ql[k][2 * o + 1] = w[1];
+            }
+        }
+    }
+    const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+    const bool use_pos = GEN && (a.window > 0 || a.slopes || a.first || a.prefix);
+
+    f16x o[kOut];
+#pragma unroll
+    for (int k = 0; k < kOut; ++k) o[k] = (f16x)(0.0f);
+    float top = kNoMax, sum = 0.0f;
+    int v_exp = -200;
+    bool bad = !q.ok;
+
+    const int32_t* table = b.pages + (size_t)s * b.max_pages;
+    const int subs = kPage / c.block;
+    // codes of one page on their way: thread -> token / column tid / 4, 16 bytes tid % 4 of each 64
+    uint4 kr[kLoads], vr[kLoads];
+    float sr = 0.0f;
+    int pr = 0;
+    auto fetch = [&](int p) {
+        int page = table[p];
+        if (page < 0 || page >= c.n_pages) {
+            bad = true;
+            page = 0;
+        }
+        const size_t at = (size_t)page * c.n_kv + h;
+        const uint8_t* kp = c.k + at * (DP * kPage) + tid * 16;
+        const uint8_t* vp = c.v + at * (DP * kPage) + tid * 16;
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            kr[j] = *reinterpret_cast<const uint4*>(kp + j * kThreads * 16);
+            vr[j] = *reinterpret_cast<const uint4*>(vp + j * kThreads * 16);
+        }
+        if (tid < 8) sr = (tid < 4 ? c.ks : c.vs)[at * subs + (tid & 3) * 16 / c.block];
+        if (use_pos && tid < kPage) pr = c.pos[at * kPage + tid];
+        if (F8 && (p + 1) * kPage > q.len) {  // what stands behind the last token may be NaN as a code
+            const int left = min(max(q.len - p * kPage - (tid & 3) * 16, 0), 16);
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+                uint32_t* u = reinterpret_cast<uint32_t*>(&vr[j]);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const int m = min(max(left - 4 * t, 0), 4);
+                    u[t] = m == 4 ? u[t] : u[t] & ((1u << (8 * m)) - 1u);
+                }
+            }
+        }
+    };
+    auto store = [&](Stage<DP>& st) {
+        const int t = tid >> 2, e = (tid & 3) * 16;
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            *reinterpret_cast<h8*>(&st.k[t][j * 64 + e]) = code_oct<F8>(kr[j].x, kr[j].y);
+            *reinterpret_cast<h8*>(&st.k[t][j * 64 + e + 8]) = code_oct<F8>(kr[j].z, kr[j].w);
+            *reinterpret_cast<h8*>(&st.v[j * 64 + t][e]) = code_oct<F8>(vr[j].x, vr[j].y);
+            *reinterpret_cast<h8*>(&st.v[j * 64 + t][e + 8]) = code_oct<F8>(vr[j].z, vr[j].w);
+        }
+        if (tid < 4) st.ks[tid] = sr;
+        else if (tid < 8) st.vs[tid - 4] = sr;
+        if (use_pos && tid < kPage) st.pos[tid] = pr;
+    };
+
+    if (p0 < p1) {
+        fetch(p0);
+        store(stage[0]);
+    }
+    __syncthreads();
+    const int my_tok = (col & 3) + ((col >> 3) << 2) + (((col >> 2) & 1) << 4);  // token of MFMA row `col`
+    for (int p = p0; p < p1; ++p) {
+        const Stage<DP>& st = stage[(p - p0) & 1];
+        const bool more = p + 1 < p1;
+        if (more) fetch(p + 1);
+        if (p >= w0 && p < w1) {
+            // x[t][e]: token 32 t + 16 hf + e of the page
+            f16x x[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                x[t] = (f16x)(0.0f);
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    const h8 key = *reinterpret_cast<const h8*>(&st.k[t * 32 + my_tok][k * 16 + hf * 8]);
+                    x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, qh[k], x[t], 0, 0, 0);
+                    x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, ql[k], x[t], 0, 0, 0);
+                }
+            }
+            const bool masked = use_pos || (p + 1) * kPage > min(full_hi, q.len);
+            uint32_t see = 0xFFFFFFFFu;
+            if (masked) see = 0;
+            float high = -__builtin_inff();
+            int e_now = -200;
+            float vs[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const float factor = row_factor * st.ks[2 * t + hf];
+                vs[t] = st.vs[2 * t + hf];
+                const int tok0 = p * kPage + t * 32 + hf * 16;
+                int kpos[16];
+                if (use_pos)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const int4 y = *reinterpret_cast<const int4*>(&st.pos[t * 32 + hf * 16 + e]);
+                        kpos[e] = y.x, kpos[e + 1] = y.y, kpos[e + 2] = y.z, kpos[e + 3] = y.w;
+                    }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float v = x[t][e] * factor;
+                    if (GEN && a.softcap > 0.0f) v = cap_score(v, a.softcap, inv_cap);
+                    v *= kLog2e;
+                    if (GEN && a.slopes) v -= row.slope * fabsf((float)(row.pos - kpos[e]));
+                    x[t][e] = v;
+                }
+                if (masked)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int tok = tok0 + e;
+                        const bool yes = tok < q.len && (use_pos ? row.sees(tok, kpos[e]) : tok <= row.slot);
+                        see |= (yes ? 1u : 0u) << (16 * t + e);
+                        x[t][e] = yes ? x[t][e] : -__builtin_inff();
+                    }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) high = fmaxf(high, x[t][e]);
+                if (vs[t] < __builtin_inff() && (see >> (16 * t)) & 0xFFFFu)
+                    e_now = max(e_now, (int)((__builtin_bit_cast(uint32_t, vs[t]) >> 23) & 255u) - 127);
+            }
+            if (__any(high > top + kLag || e_now > v_exp)) {
+                const float new_top = fmaxf(top, halves_max(high));
+                const int new_exp = max(v_exp, (int)halves_max((float)e_now));
+                const float keep = __builtin_amdgcn_exp2f(top - new_top);
+                const float keep_o = v_exp == -200 ? 0.0f : keep * __builtin_amdgcn_exp2f((float)(v_exp - new_exp));
+                sum *= keep;
+#pragma unroll
+                for (int k = 0; k < kOut; ++k) o[k] *= keep_o;
+                top = new_top;
+                v_exp = new_exp;
+            }
+            const float unit = __builtin_amdgcn_exp2f(-(float)max(v_exp, -126)), base = (float)kBias - top;
+            h8 wh[4], wl[4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const float ratio = vs[t] * unit;
+                float w[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float pe = __builtin_amdgcn_exp2f(x[t][e] + base);
+                    sum += pe;
+                    w[e] = pe * ratio;
+                }
+                if (masked)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) w[e] = (see >> (16 * t + e)) & 1u ? w[e] : 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    h2 u, v;
+                    split_pair(w[2 * e], w[2 * e + 1], &u, &v);
+                    wh[2 * t + e / 4][2 * e % 8] = u[0], wh[2 * t + e / 4][2 * e % 8 + 1] = u[1];
+                    wl[2 * t + e / 4][2 * e % 8] = v[0], wl[2 * t + e / 4][2 * e % 8 + 1] = v[1];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kOut; ++k)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {  // tokens 32 (t / 2) + 16 hf + 8 (t % 2) ..
+                    const h8 val = *reinterpret_cast<const h8*>(&st.v[k * 32 + col][(t / 2) * 32 + hf * 16 + (t % 2) * 8]);
+                    o[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(val, wh[t], o[k], 0, 0, 0);
+                    o[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(val, wl[t], o[k], 0, 0, 0);
+                }
+        }
+        if (more) store(stage[(p + 1 - p0) & 1]);
+        __syncthreads();
+    }
+    bad = __syncthreads_or(bad) != 0;
+    sum = halves_sum(sum);
+    if (!live) return;
+    const float nan = __builtin_nanf(""), up = v_exp == -200 ? 0.0f : __builtin_amdgcn_exp2f((float)v_exp);
+    if (parts > 1) {
+        float* piece = scratch + ((((size_t)s * c.n_kv + h) * tiles + rt) * parts + part) * kPieceFloats<DP>;
+        const int r = wave * kCols + col;
+#pragma unroll
+        for (int k = 0; k < kOut; ++k)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<f4*>(&piece[r * DP + k * 32 + 2 * e + 4 * hf]) = f4{o[k][e], o[k][e + 1], o[k][e + 2], o[k][e + 3]} * up;
+        if (hf == 0) {
+            piece[kRows * DP + r] = top;
+            piece[kRows * DP + kRows + r] = bad ? nan : sum;
+        }
+        return;
+    }
+    const size_t at = (size_t)(q.r0 + i) * a.n_head + head;
+    const float scale = bad ? nan : sum == 0.0f ? 0.0f : up / sum;
+    float* out = dst + at * c.dim;
+    const bool vec = c.dim % 4 == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+#pragma unroll
+    for (int k = 0; k < kOut; ++k)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int d = k * 32 + 2 * e + 4 * hf;
+            const f4 y = f4{o[k][e], o[k][e + 1], o[k][e + 2], o[k][e + 3]} * scale;
+            if (vec) {
+                if (d < c.dim) *reinterpret_cast<f4*>(out + d) = y;
+            } else {
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                    if (d + n < c.dim) out[d + n] = y[n];
+            }
+        }
+    if (lse && hf == 0)
+        lse[at] = bad ? nan : sum == 0.0f ? -__builtin_inff() : (__builtin_amdgcn_logf(sum) + top - (float)kBias) * kLn2;
+}
+
+// Joins the pieces of the rows of one (sequence, head, row tile), a wave at a time per row.
+template <int DP>
+__global__ __launch_bounds__(kThreads) void join_rows_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a, float* __restrict__ dst,
+                                                             float* __restrict__ lse, const float* __restrict__ scratch,
+                                                             int tiles, int parts) {
+    const int lane = threadIdx.x & 63;
+    const int rt = blockIdx.x % tiles, h = blockIdx.x / tiles % c.n_kv, s = blockIdx.x / tiles / c.n_kv;
+    const int r = (int)blockIdx.y * kWaves + ((int)threadIdx.x >> 6), r_all = rt * kRows + r;
+    const Kv8Seq q = kv8_seq(b, s);
+    if (r_all >= q.n * a.group) return;
+    const float* first = scratch + (((size_t)s * c.n_kv + h) * tiles + rt) * parts * kPieceFloats<DP>;
+    float m = kNoMax, l = 0.0f;
+    for (int k = 0; k < parts; ++k) m = fmaxf(m, first[(size_t)k * kPieceFloats<DP> + kRows * DP + r]);
+    float x[DP / 64] = {};
+    for (int k = 0; k < parts; ++k) {
+        const float* piece = first + (size_t)k * kPieceFloats<DP>;
+        const float f = __builtin_amdgcn_exp2f(piece[kRows * DP + r] - m);
+        l += piece[kRows * DP + kRows + r] * f;
+#pragma unroll
+        for (int j = 0; j < DP / 64; ++j) x[j] += piece[r * DP + j * 64 + lane] * f;
+    }
+    const size_t at = (size_t)(q.r0 + r_all / a.group) * a.n_head + h * a.group + r_all % a.group;
+#pragma unroll
+    for (int j = 0; j < DP / 64; ++j)
+        if (j * 64 + lane < c.dim) dst[at * c.dim + j * 64 + lane] = l == 0.0f ? 0.0f : l != l ? l : x[j] / l;
+    if (lse && lane == 0) lse[at] = l == 0.0f ? -__builtin_inff() : (__builtin_amdgcn_logf(l) + m - (float)kBias) * kLn2;
+}
+
+int tiles_of(int group, int max_q) { return (int)(((int64_t)max_q * group + kRows - 1) / kRows); }
+
+// Pieces each row tile's pages are cut into: enough for two workgroups on each compute unit, of at least eight pages.
+int parts_of(int cus, int n_kv, int group, int n_seq, int max_q, int max_pages) {
+    const int64_t wgs = (int64_t)n_seq * n_kv * tiles_of(group, max_q);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus / wgs, max_pages / 8));
+}
+
+template <int DP>
+void launch_prompt_dp(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch, int cus,
+                      hipStream_t stream) {
+    const bool gen = a.softcap > 0.0f || a.window > 0 || a.slopes || a.first || a.prefix;
+    const int tiles = tiles_of(a.group, b.max_q), parts = parts_of(cus, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);
+    auto kernel = c.f8 ? (gen ? prompt_kernel<DP, true, true> : prompt_kernel<DP, true, false>)
+                       : (gen ? prompt_kernel<DP, false, true> : prompt_kernel<DP, false, false>);
+    const size_t lds = 2 * sizeof(Stage<DP>);
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    // heads side by side: workgroups go round the XCDs in this order, so a head's pages stay in one L2
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(c.n_kv * parts), (unsigned)tiles, (unsigned)b.n_seq), dim3(kThreads), lds, stream,
+                       c, b, a, dst, lse, scratch, tiles, parts);
+    if (parts > 1)
+        hipLaunchKernelGGL(join_rows_kernel<DP>, dim3((unsigned)(b.n_seq * c.n_kv * tiles), kRows / kWaves), dim3(kThreads), 0,
+                           stream, c, b, a, dst, lse, scratch, tiles, parts);
+}
+
+}  // namespace
+
+bool prompt_takes(int max_q, int group) {
+    return (int64_t)max_q * group > 32 && tiles_of(group, max_q) <= 65535;
+}
+size_t prompt_scratch(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages) {
+    const int parts = parts_of(cus, n_kv, group, n_seq, max_q, max_pages);
+    const size_t dp = (size_t)(dim + 63) / 64 * 64;
+    return parts == 1 ? 0 : (size_t)n_seq * n_kv * tiles_of(group, max_q) * parts * (kRows * dp + 2 * kRows) * sizeof(float);
+}
+void launch_attention_prompt(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch,
+                             int cus, hipStream_t stream) {
+    switch (c.dp) {
+    case 64: launch_prompt_dp<64>(c, b, a, dst, lse, scratch, cus, stream); break;
+    case 128: launch_prompt_dp<128>(c, b, a, dst, lse, scratch, cus, stream); break;
+    case 192: launch_prompt_dp<192>(c, b, a, dst, lse, scratch, cus, stream); break;
+    default: launch_prompt_dp<256>(c, b, a, dst, lse, scratch, cus, stream); break;
+    }
+}
+
+}  // namespace infr
