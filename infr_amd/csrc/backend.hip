@@ -89,7 +89,7 @@ struct infr_hip {
     // MoE scratch
     void* moe_ws = nullptr;
     size_t moe_ws_bytes = 0;
-    // AttentionKv8's partial results
+    // partial results of AttentionKv8 and ScoreKv8
     void* kv8_ws = nullptr;
     size_t kv8_ws_bytes = 0;
     // Counts reallocations of the scratch above. A recorded launch sequence carries the scratch
@@ -688,9 +688,10 @@ static uint32_t kv8_max_tensor(const infr_hip_op_t& op) {
 
 // Scratch an op of this shape needs.
 static size_t kv8_scratch(const infr_hip_t* be, int kind, const infr_hip_kv8_params_t& p) {
-    return kind == INFR_OP_ATTENTION_KV8
-               ? infr::attention_kv8_scratch(be->props.multiProcessorCount, (int)p.head_dim, (int)p.n_kv, (int)(p.n_head / p.n_kv), (int)p.n_seq, (int)p.max_q, (int)p.max_pages)
-               : 0;
+    if (kind != INFR_OP_ATTENTION_KV8 && kind != INFR_OP_SCORE_KV8) return 0;
+    const int cus = be->props.multiProcessorCount, group = (int)(p.n_head / p.n_kv), n_kv = (int)p.n_kv, n_seq = (int)p.n_seq;
+    return kind == INFR_OP_SCORE_KV8 ? infr::score_kv8_scratch(cus, n_kv, group, n_seq, (int)p.max_q, (int)p.max_pages)
+                                     : infr::attention_kv8_scratch(cus, (int)p.head_dim, n_kv, group, n_seq, (int)p.max_q, (int)p.max_pages);
 }
 
 static int ensure_kv8_ws(infr_hip_t* be, size_t bytes) {
@@ -707,18 +708,18 @@ static int ensure_kv8_ws(infr_hip_t* be, size_t bytes) {
     (void)hipSetDevice(current);
     if (e != hipSuccess) {
         be->kv8_ws = nullptr;
-        return fail(be, INFR_HIP_ERR_BACKEND, "attention_kv8: hipMalloc(" + std::to_string(bytes) + "): " + hipGetErrorString(e));
+        return fail(be, INFR_HIP_ERR_BACKEND, "kv8: hipMalloc(" + std::to_string(bytes) + "): " + hipGetErrorString(e));
     }
     be->kv8_ws_bytes = bytes;
     return INFR_HIP_OK;
 }
 
 static int enqueue_kv8(infr_hip_t* be, int kind, const infr_hip_kv8_params_t& p, const Kv8Args& k) {
-    if (kv8_scratch(be, kind, p) > be->kv8_ws_bytes) return fail(be, INFR_HIP_ERR_OTHER, "attention_kv8: scratch was not sized");
+    if (kv8_scratch(be, kind, p) > be->kv8_ws_bytes) return fail(be, INFR_HIP_ERR_OTHER, "kv8: scratch was not sized");
     switch (kind) {
     case INFR_OP_WRITE_KV8: infr::launch_write_kv8(k.c, k.b, k.slots, k.x, k.x_stride, k.v, k.v_stride, be->stream); break;
     case INFR_OP_ATTENTION_KV8: infr::launch_attention_kv8(k.c, k.b, k.a, k.dst, k.lse, be->kv8_ws, be->props.multiProcessorCount, be->stream); break;
-    case INFR_OP_SCORE_KV8: infr::launch_score_kv8(k.c, k.b, k.a, k.lse, p.decay, be->stream); break;
+    case INFR_OP_SCORE_KV8: infr::launch_score_kv8(k.c, k.b, k.a, k.lse, p.decay, be->kv8_ws, be->props.multiProcessorCount, be->stream); break;
     default: infr::launch_evict_kv8(k.c, k.e, be->stream); break;
     }
     HIP_TRY(be, hipGetLastError());

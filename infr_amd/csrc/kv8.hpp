@@ -69,8 +69,9 @@ void launch_write_kv8(const Kv8Cache& c, const Kv8Batch& b, const int32_t* slots
 size_t attention_kv8_scratch(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages);
 void launch_attention_kv8(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, void* scratch,
                           int cus, hipStream_t stream);
-void launch_score_kv8(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, const float* lse, float decay,
-                      hipStream_t stream);
+size_t score_kv8_scratch(int cus, int n_kv, int group, int n_seq, int max_q, int max_pages);
+void launch_score_kv8(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, const float* lse, float decay, void* scratch,
+                      int cus, hipStream_t stream);
 void launch_evict_kv8(const Kv8Cache& c, const Kv8Evict& e, hipStream_t stream);
 
 #ifdef __HIPCC__

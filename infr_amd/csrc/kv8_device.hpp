@@ -125,4 +125,40 @@ __device__ __forceinline__ Kv8Row kv8_row(const Kv8Batch& b, const Kv8Attn& a, c
     return r;
 }
 
+// ---- how the kernels for few rows cut a batch's pages: pieces of one size, found from the lengths ----
+
+constexpr int kStepWaves = 4;   // waves of a workgroup, each a page at a time
+constexpr int kStepRows = 16;   // query rows of a workgroup
+
+struct SeqWork {
+    int tiles, p_lo, pages;  // row tiles, first page any row sees, pages from there
+};
+// `all`: every cached page is gone over by one tile, whether rows see it or not (ScoreKv8 lets sums decay).
+__device__ __forceinline__ SeqWork seq_work(const Kv8Batch& b, const Kv8Attn& a, int s, bool all = false) {
+    const Kv8Seq q = kv8_seq(b, s);
+    SeqWork w;
+    w.tiles = all ? 1 : (q.n * a.group + kStepRows - 1) / kStepRows;
+    if (!q.ok) {  // one item per tile writes the rows' NaN
+        w.p_lo = 0;
+        w.pages = 1;
+        return w;
+    }
+    // positions ascend with the tokens, so a token `window` or more tokens back is outside the window
+    const int lo = a.window > 0 && !all ? max(q.len - q.n - a.window + 1, 0) : 0;
+    w.p_lo = lo / kPage;
+    w.pages = max((q.len + kPage - 1) / kPage - w.p_lo, 1);
+    return w;
+}
+// Pages per piece: about `target` pieces in all, at least one page for each wave of a workgroup.
+__device__ __forceinline__ int piece_pages(const Kv8Batch& b, const Kv8Attn& a, int n_kv, int target, bool all = false) {
+    const int lane = threadIdx.x & 63;
+    float total = 0.0f;
+    for (int s = lane; s < b.n_seq; s += 64) {
+        const SeqWork w = seq_work(b, a, s, all);
+        total += (float)w.tiles * (float)w.pages;
+    }
+    for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
+    return max((int)__builtin_ceilf(total * (float)n_kv / (float)target), kStepWaves);
+}
+
 }  // namespace infr

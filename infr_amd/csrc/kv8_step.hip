@@ -16,47 +16,10 @@ namespace infr {
 
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kRows = 16;
+constexpr int kWaves = kStepWaves;
+constexpr int kRows = kStepRows;
 constexpr int kBias = 10;    // softmax weights are 2^kBias at the running maximum ..
 constexpr float kLag = 4.0f; // .. which may lag behind the true one by this many powers of two
-
-// How the batch's pages are cut.
-struct Cut {
-    int s, h, rt, part;    // sequence, KV head, row tile, piece
-    int parts, item;       // pieces of this (sequence, head, row tile); number of the first one in the scratch
-    int p0, p1;            // pages of the piece
-};
-
-struct SeqWork {
-    int tiles, p_lo, pages;  // row tiles, first page any row sees, pages from there
-};
-__device__ __forceinline__ SeqWork seq_work(const Kv8Batch& b, const Kv8Attn& a, int s) {
-    const Kv8Seq q = kv8_seq(b, s);
-    SeqWork w;
-    w.tiles = (q.n * a.group + kRows - 1) / kRows;
-    if (!q.ok) {  // one item per tile writes the rows' NaN
-        w.p_lo = 0;
-        w.pages = 1;
-        return w;
-    }
-    // positions ascend with the tokens, so a token `window` or more tokens back is outside the window
-    const int lo = a.window > 0 ? max(q.len - q.n - a.window + 1, 0) : 0;
-    w.p_lo = lo / kPage;
-    w.pages = max((q.len + kPage - 1) / kPage - w.p_lo, 1);
-    return w;
-}
-// Pages per piece: about `target` pieces in all, at least one page for each wave of a workgroup.
-__device__ __forceinline__ int piece_pages(const Kv8Batch& b, const Kv8Attn& a, int n_kv, int target) {
-    const int lane = threadIdx.x & 63;
-    float total = 0.0f;
-    for (int s = lane; s < b.n_seq; s += 64) {
-        const SeqWork w = seq_work(b, a, s);
-        total += (float)w.tiles * (float)w.pages;
-    }
-    for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
-    return max((int)__builtin_ceilf(total * (float)n_kv / (float)target), kWaves);
-}
 
 // O, maximum and sum of a piece: f32 [rows][DP], then [rows] maxima and [rows] sums.
 template <int DP>
