@@ -813,9 +813,7 @@ class HipBackend:
 
     def execute(self, plan: Plan, bindings: Bindings) -> None:
         n = len(bindings.slots)
-        arr = (_vp * max(1, n))()
-        for i, b in enumerate(bindings.slots):
-            arr[i] = b._h if b is not None else None
+        arr = (_vp * max(1, n))(*[b._h if b is not None else None for b in bindings.slots])
         self._check(self._lib.infr_hip_execute(self._h, plan._h, arr, n))
 
     # -- the ops, directly --
