@@ -101,16 +101,34 @@ __device__ __forceinline__ float kv8_scale(uint32_t amax_bits, bool f8) {
     if (amax_bits >= 0x7F800000u) return __builtin_nanf("");
     return fmaxf(__builtin_bit_cast(float, amax_bits) / (f8 ? 448.0f : 127.0f), kMinScale);
 }
-// Nearest code of x / scale, ties to even. |x / scale| stays below the largest code's rounding border: the
-// scale is amax / code_max rounded once and the quotient is rounded once more.
-__device__ __forceinline__ uint32_t kv8_code(float x, float scale, bool f8) {
-    if (!(scale < __builtin_inff())) return 0;  // a NaN scale
-    const float y = x / scale;
-    if (f8) return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false) & 0xFFu;
-    return (uint32_t)(int)fminf(fmaxf(rintf(y), -127.0f), 127.0f) & 0xFFu;
+// 1 / scale for kv8_code, to an ulp; 0 for a NaN scale, whose codes are 0.
+__device__ __forceinline__ float kv8_inverse(float scale) {
+    return scale < __builtin_inff() ? __builtin_amdgcn_rcpf(scale) : 0.0f;
 }
-__device__ __forceinline__ float kv8_value(uint32_t code, bool f8) {
-    return f8 ? __builtin_amdgcn_cvt_f32_fp8((int)code, 0) : (float)(int)(int8_t)code;
+// Nearest code of x / scale (the correctly rounded quotient), ties to even. x * inverse is off by less than 2^-21 of
+// it; only where that leaves the code in doubt is the quotient itself formed, a few in 10^4. |x / scale| stays below
+// the largest code's rounding border: the scale is amax / code_max rounded once and the quotient once more.
+template <bool F8>
+__device__ __forceinline__ uint32_t kv8_code(float x, float scale, float inverse) {
+    if (inverse == 0.0f) return 0;
+    float y = x * inverse;
+    if constexpr (F8) {
+        uint32_t two = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y * (1.0f - 0x1p-20f), y * (1.0f + 0x1p-20f), 0, false);
+        if ((two & 0xFFu) != ((two >> 8) & 0xFFu)) {
+            y = x / scale;
+            two = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
+        }
+        return two & 0xFFu;
+    } else {
+        float n = rintf(y);
+        if (fabsf(fabsf(y - n) - 0.5f) < 0x1p-13f) n = rintf(x / scale);
+        return (uint32_t)(int)fminf(fmaxf(n, -127.0f), 127.0f) & 0xFFu;
+    }
+}
+template <bool F8>
+__device__ __forceinline__ float kv8_value(uint32_t code) {
+    if constexpr (F8) return __builtin_amdgcn_cvt_f32_fp8((int)code, 0);
+    else return (float)(int)(int8_t)code;
 }
 
 // Byte offset of key code d of token t of (page, head) / of value code d.

@@ -2,13 +2,16 @@
 //
 // Kept are the first `sink` tokens, the last `recent` and, of those between, the ones with the largest sums of
 // attention weight (equal sums: the lower slot), in their order. Two launches:
-//   select  one workgroup per (sequence, head): the rank of the smallest kept sum by a radix search, 8 bits a
-//           pass over the candidates (LDS counters: integer sums, so the same counts in any order), then the kept
-//           slots in ascending order by a running prefix count. Reads 4 bytes a token a pass, from L2 after the
-//           first; bound by the passes' latency.
-//   move    one workgroup per (new page, head): gathers the kept tokens' codes. A block whose tokens come whole
-//           and in place from one block keeps its codes and scale; the others are quantized again from
-//           code * scale. Bound by the gather: single bytes of V^T rows and 64-byte pieces of K rows.
+//   select  one workgroup per (sequence, head), each thread with a run of neighbouring tokens whose sums stay in its
+//           registers: the smallest kept sum is found by counting in 2048 bins over the range of the sums, then over
+//           the bin it lies in, 11 bits a pass (integer counts in LDS: the same in any order); two prefix sums then
+//           give every kept token its place. Bound by the passes' latency.
+//   move    one workgroup per (new page, head, K or V): gathers the kept tokens' codes, 16-byte pieces of K rows and
+//           single bytes of V^T rows, a lane to a token, so that a wave's bytes lie in as few lines as the tokens'
+//           pages allow. A block whose tokens come whole and in place from one block keeps its codes and scale; the
+//           others are quantized again from code * scale. Bound by the lines of V that hold any kept token.
+#include <type_traits>
+
 #include "kv8.hpp"
 
 namespace infr {
@@ -17,6 +20,7 @@ namespace {
 
 constexpr int kSelect = 1024;
 constexpr int kMove = 256;
+constexpr int kBinBits = 11, kBins = 1 << kBinBits;
 
 struct EvictSeq {
     int len, n_out;
@@ -68,10 +72,13 @@ __device__ __forceinline__ int block_scan(int x, int* part, int* total) {
     return before + sum - x;
 }
 
-__global__ __launch_bounds__(kSelect) void evict_select_kernel(Kv8Cache c, Kv8Evict e) {
-    __shared__ int hist[256];
+// EACH neighbouring tokens of a thread at a time; sequences of more than EACH * 1024 tokens go over them in rounds,
+// reading the sums again for each pass.
+template <int EACH>
+__global__ __launch_bounds__(kSelect, 4) void evict_select_kernel(Kv8Cache c, Kv8Evict e) {
     __shared__ int part[kSelect / 64];
-    __shared__ uint32_t found[2];
+    __shared__ int hist[kBins];
+    __shared__ uint32_t found[2], ends[2];
     const int s = blockIdx.y, h = blockIdx.x, tid = threadIdx.x;
     const EvictSeq q = evict_seq(c, e, s, tid, kSelect);
     int32_t* kept = e.kept + ((size_t)s * c.n_kv + h) * e.keep;
@@ -83,114 +90,221 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(Kv8Cache c, Kv8Ev
         return;
     }
     const int32_t* pages = e.pages + (size_t)s * e.max_pages;
-    auto key_at = [&](int j) { return sum_key(c.sums[((size_t)pages[j / kPage] * c.n_kv + h) * kPage + j % kPage]); };
     const int lo = e.sink, hi = q.len - e.recent;  // candidates: more than `need` of them, as len > keep
-    int need = e.keep - e.sink - e.recent;
-    uint32_t prefix = 0;
-    // the need-th largest key, from its top byte down; `need` becomes its rank among the equal ones
-    for (int shift = 24; need > 0 && shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += kSelect) hist[i] = 0;
+    const int need = e.keep - e.sink - e.recent;
+    const int span = EACH * kSelect, rounds = (q.len + span - 1) / span;
+    // key of each of the thread's tokens, 0 for those that are no candidates: below every number's key
+    uint32_t key[EACH];
+    auto load = [&](int round) {
+        const int j0 = round * span + tid * EACH;
+#pragma unroll
+        for (int n = 0; n < EACH; n += 4) {
+            const int j = j0 + n;  // (four tokens lie in one page)
+            float4 x = make_float4(0, 0, 0, 0);
+            if (j < q.len) x = *reinterpret_cast<const float4*>(c.sums + ((size_t)pages[j / kPage] * c.n_kv + h) * kPage + j % kPage);
+            key[n] = j >= lo && j < hi ? sum_key(x.x) : 0;
+            key[n + 1] = j + 1 >= lo && j + 1 < hi ? sum_key(x.y) : 0;
+            key[n + 2] = j + 2 >= lo && j + 2 < hi ? sum_key(x.z) : 0;
+            key[n + 3] = j + 3 >= lo && j + 3 < hi ? sum_key(x.w) : 0;
+        }
+    };
+    load(0);
+    // the need-th largest key: `limit`, and how many of those equal to it stay: `ties`
+    uint32_t limit = 0;
+    int ties = need;
+    if (need > 0) {
+        uint32_t low = 0xFFFFFFFFu, high = 0;
+        for (int r = 0; r < rounds; ++r) {
+            if (rounds > 1) load(r);
+#pragma unroll
+            for (int n = 0; n < EACH; ++n) {
+                low = key[n] ? min(low, key[n]) : low;
+                high = max(high, key[n]);
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            low = min(low, (uint32_t)__shfl_xor((int)low, o));
+            high = max(high, (uint32_t)__shfl_xor((int)high, o));
+        }
+        if (tid < 2) ends[tid] = tid ? 0 : 0xFFFFFFFFu;
         __syncthreads();
-        for (int j = lo + tid; j < hi; j += kSelect) {
-            const uint32_t k = key_at(j);
-            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255u], 1);
+        if ((tid & 63) == 0) {
+            atomicMin(&ends[0], low);
+            atomicMax(&ends[1], high);
         }
         __syncthreads();
-        if (tid < 64) {  // lane l: bins 255 - 4 l downwards
-            int mine = 0;
-            for (int i = 0; i < 4; ++i) mine += hist[255 - 4 * tid - i];
-            const int sum = wave_scan(mine);
-            int above = sum - mine;
-            if (above < need && need <= sum)
-                for (int i = 0; i < 4; ++i) {
-                    const int n = hist[255 - 4 * tid - i];
-                    if (above < need && need <= above + n) {
-                        found[0] = (uint32_t)(255 - 4 * tid - i);
-                        found[1] = (uint32_t)(need - above);
+        limit = ends[0];
+        uint32_t width = ends[1] - ends[0];  // keys in question: limit .. limit + width
+        while (width > 0) {
+            const int shift = max(32 - __builtin_clz(width) - kBinBits, 0);
+            for (int i = tid; i < kBins; i += kSelect) hist[i] = 0;
+            __syncthreads();
+            for (int r = 0; r < rounds; ++r) {
+                if (rounds > 1) load(r);
+#pragma unroll
+                for (int n = 0; n < EACH; ++n)
+                    if (key[n] && key[n] - limit <= width) atomicAdd(&hist[(key[n] - limit) >> shift], 1);
+            }
+            __syncthreads();
+            // thread i: bins from the top, kBins / kSelect of them
+            constexpr int kMine = kBins / kSelect;
+            const int top = kBins - 1 - tid * kMine;
+            int mine = 0, total = 0;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) mine += hist[top - i];
+            int above = block_scan(mine, part, &total);
+            if (above < ties && ties <= above + mine)
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) {
+                    const int n = hist[top - i];
+                    if (above < ties && ties <= above + n) {
+                        found[0] = (uint32_t)(top - i);
+                        found[1] = (uint32_t)(ties - above);
                     }
                     above += n;
                 }
+            __syncthreads();
+            const uint32_t base = found[0] << shift, size = (1u << shift) - 1u;
+            width = min(size, width - base);
+            limit += base;
+            ties = (int)found[1];
+            __syncthreads();
         }
-        __syncthreads();
-        prefix |= found[0] << shift;
-        need = (int)found[1];
-        __syncthreads();
     }
-    const bool any = e.keep > e.sink + e.recent;
+    int total = 0;
     int equal_before = 0, out_before = 0;
-    for (int base = 0; base < q.len; base += kSelect) {
-        const int j = base + tid;
-        const bool in = j < q.len, must = in && (j < lo || j >= hi);
-        const uint32_t k = in && !must && any ? key_at(j) : 0;
-        const bool equal = in && !must && any && k == prefix;
-        int total = 0;
-        const int rank = equal_before + block_scan(equal ? 1 : 0, part, &total);
+    for (int r = 0; r < rounds; ++r) {
+        if (rounds > 1) load(r);
+        const int j0 = r * span + tid * EACH;
+        int equal = 0;
+#pragma unroll
+        for (int n = 0; n < EACH; ++n) equal += need > 0 && key[n] == limit && key[n] ? 1 : 0;
+        int rank = equal_before + block_scan(equal, part, &total);
         equal_before += total;
-        const bool take = must || (in && any && !must && (k > prefix || (equal && rank < need)));
-        const int at = out_before + block_scan(take ? 1 : 0, part, &total);
+        uint32_t take = 0;
+#pragma unroll
+        for (int n = 0; n < EACH; ++n) {
+            const int j = j0 + n;
+            bool yes = j < q.len && (j < lo || j >= hi);
+            if (need > 0 && key[n]) {
+                if (key[n] > limit) yes = true;
+                else if (key[n] == limit) yes = rank++ < ties;
+            }
+            take |= (uint32_t)yes << n;
+        }
+        int at = out_before + block_scan(__builtin_popcount(take), part, &total);
         out_before += total;
-        if (take) kept[at] = j;
+#pragma unroll
+        for (int n = 0; n < EACH; ++n)
+            if ((take >> n) & 1) kept[at++] = j0 + n;
     }
 }
 
+template <int DP, bool F8>
 __global__ __launch_bounds__(kMove) void evict_move_kernel(Kv8Cache c, Kv8Evict e) {
-    __shared__ uint32_t amax[2][kPage];
-    __shared__ uint8_t whole[kPage];
-    __shared__ int from[kPage], slot[kPage];
-    const int s = blockIdx.z, h = blockIdx.y, po = blockIdx.x, tid = threadIdx.x;
+    constexpr int kPieces = DP / 64, kColumns = DP / 4;
+    __shared__ uint32_t amax[kPage];
+    const int s = blockIdx.z, h = (int)blockIdx.y >> 1, po = blockIdx.x, tid = threadIdx.x;
+    const bool is_v = blockIdx.y & 1;
     const int n_out = e.lens_out[s];
     if (n_out <= po * kPage) return;  // also -1: a sequence that was left as it is
     const int cnt = min(kPage, n_out - po * kPage);
     const int to = e.pages_out[(size_t)s * e.out_pages + po];
     const int subs = kPage / c.block;
-    const bool f8 = c.f8 != 0;
-    const int32_t* kept = e.kept + ((size_t)s * c.n_kv + h) * e.keep + po * kPage;
-    if (tid < kPage) {
-        const int j = tid < cnt ? kept[tid] : 0;
-        from[tid] = e.pages[(size_t)s * e.max_pages + j / kPage];
-        slot[tid] = j % kPage;
-        const int lead = __shfl(j, tid / c.block * c.block);
-        const bool fits = tid >= cnt || (j == lead + tid % c.block && lead % c.block == 0);
-        whole[tid] = fits;
-        amax[0][tid] = amax[1][tid] = 0;
-    }
-    __syncthreads();
-    const int t = tid >> 2, sub = t / c.block;
-    bool copy = true;  // this thread's block comes whole from one block
-    for (int o = 0; o < c.block; ++o) copy = copy && whole[sub * c.block + o];
+    // K: four lanes to a token, 16 columns of each 64; V: a lane to a token, a quarter of the columns to a wave
+    const int t = is_v ? tid & 63 : tid >> 2, part = is_v ? tid >> 6 : tid & 3;
     const bool live = t < cnt;
-    const int pg = from[t], sl = slot[t];
-    const size_t old_at = ((size_t)pg * c.n_kv + h) * subs + sl / c.block;
-    for (int part = 0; part < 2; ++part) {
-        const uint8_t* codes = part ? c.v : c.k;
-        const float old = (part ? c.vs : c.ks)[old_at];
-        auto code_at = [&](int d) { return (uint32_t)codes[part ? v_at(c, pg, h, sl, d) : k_at(c, pg, h, sl, d)]; };
-        uint32_t top = 0;
-        if (live && !copy)
-            for (int d = tid & 3; d < c.dim; d += 4) top = max(top, abs_bits(kv8_value(code_at(d), f8) * old));
-        if (top) atomicMax(&amax[part][sub * c.block], top);
-        __syncthreads();
-        const float scale = copy ? old : kv8_scale(amax[part][sub * c.block], f8);
-        if (live && t % c.block == 0 && (tid & 3) == 0) (part ? c.vs : c.ks)[((size_t)to * c.n_kv + h) * subs + sub] = scale;
-        for (int d = tid & 3; d < c.dp; d += 4) {
-            uint32_t code = 0;
-            if (live && d < c.dim) code = copy ? code_at(d) : kv8_code(kv8_value(code_at(d), f8) * old, scale, f8);
-            if (live) (part ? c.v : c.k)[part ? v_at(c, to, h, t, d) : k_at(c, to, h, t, d)] = (uint8_t)code;
+    const int32_t* kept = e.kept + ((size_t)s * c.n_kv + h) * e.keep + po * kPage;
+    const int j = live ? kept[t] : -1, j0 = kept[t / c.block * c.block < cnt ? t / c.block * c.block : 0];
+    if (tid < kPage) amax[tid] = 0;
+    // amax's top bit marks a block that has to be quantized again
+    const bool in_place = !live || (j == j0 + t % c.block && j0 % c.block == 0);
+    __syncthreads();
+    if (!in_place && part == 0) atomicOr(&amax[t / c.block], 0x80000000u);
+    // (a lane without a token reads the first token of page 0 and writes nothing)
+    const int page = live ? e.pages[(size_t)s * e.max_pages + j / kPage] : 0, slot = live ? j % kPage : 0;
+    const size_t from = (size_t)page * c.n_kv + h, dst = (size_t)to * c.n_kv + h;
+    float* scales = is_v ? c.vs : c.ks;
+    const float old = scales[from * subs + slot / c.block];
+    uint4 kw[kPieces];
+    uint32_t vw[kColumns / 4];
+    if (!is_v) {
+        const uint8_t* src = c.k + from * (DP * kPage) + slot * 64 + part * 16;
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) kw[p] = *reinterpret_cast<const uint4*>(src + p * kPage * 64);
+    } else {
+        const uint8_t* src = c.v + (from * DP + part * kColumns) * kPage + slot;
+#pragma unroll
+        for (int d = 0; d < kColumns / 4; ++d) {
+            vw[d] = 0;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) vw[d] |= (uint32_t)src[(4 * d + n) * kPage] << (8 * n);
         }
     }
-    if (live && (tid & 3) == 0) {
-        const size_t a = ((size_t)pg * c.n_kv + h) * kPage + sl, z = ((size_t)to * c.n_kv + h) * kPage + t;
-        c.pos[z] = c.pos[a];
-        c.sums[z] = c.sums[a];
+    __syncthreads();
+    const bool again = amax[t / c.block] >> 31;
+    __syncthreads();
+    if (again) {
+        uint32_t top = 0;
+        auto look = [&](uint32_t w) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) top = max(top, abs_bits(kv8_value<F8>((w >> (8 * n)) & 255u) * old));
+        };
+        if (live && !is_v)
+#pragma unroll
+            for (int p = 0; p < kPieces; ++p) look(kw[p].x), look(kw[p].y), look(kw[p].z), look(kw[p].w);
+        if (live && is_v)
+#pragma unroll
+            for (int d = 0; d < kColumns / 4; ++d) look(vw[d]);
+        atomicMax(&amax[t / c.block], top | 0x80000000u);
+    }
+    __syncthreads();
+    const float scale = again ? kv8_scale(amax[t / c.block] & 0x7FFFFFFFu, F8) : old, inverse = kv8_inverse(scale);
+    auto code = [&](uint32_t w) {
+        uint32_t r = 0;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) r |= kv8_code<F8>(kv8_value<F8>((w >> (8 * n)) & 255u) * old, scale, inverse) << (8 * n);
+        return r;
+    };
+    if (!live) return;
+    if (t % c.block == 0 && part == 0) scales[dst * subs + t / c.block] = scale;
+    if (!is_v) {
+        uint8_t* out = c.k + dst * (DP * kPage) + t * 64 + part * 16;
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+            if (again) kw[p] = make_uint4(code(kw[p].x), code(kw[p].y), code(kw[p].z), code(kw[p].w));
+            *reinterpret_cast<uint4*>(out + p * kPage * 64) = kw[p];
+        }
+        if (part == 0) {
+            c.pos[dst * kPage + t] = c.pos[from * kPage + slot];
+            c.sums[dst * kPage + t] = c.sums[from * kPage + slot];
+        }
+    } else {
+        uint8_t* out = c.v + (dst * DP + part * kColumns) * kPage + t;
+#pragma unroll
+        for (int d = 0; d < kColumns / 4; ++d) {
+            const uint32_t w = again ? code(vw[d]) : vw[d];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) out[(4 * d + n) * kPage] = (uint8_t)(w >> (8 * n));
+        }
     }
 }
 
 }  // namespace
 
 void launch_evict_kv8(const Kv8Cache& c, const Kv8Evict& e, hipStream_t stream) {
-    hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)c.n_kv, (unsigned)e.n_seq), dim3(kSelect), 0, stream, c, e);
-    hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)e.out_pages, (unsigned)c.n_kv, (unsigned)e.n_seq), dim3(kMove), 0,
-                       stream, c, e);
+    const dim3 grid((unsigned)c.n_kv, (unsigned)e.n_seq);
+    const int64_t most = (int64_t)e.max_pages * kPage;
+    auto select = most <= 4 * kSelect ? evict_select_kernel<4> : evict_select_kernel<32>;
+    hipLaunchKernelGGL(select, grid, dim3(kSelect), 0, stream, c, e);
+    auto pick = [&](auto f8) {
+        constexpr bool F8 = decltype(f8)::value;
+        return c.dp == 64 ? evict_move_kernel<64, F8> : c.dp == 128 ? evict_move_kernel<128, F8>
+             : c.dp == 192 ? evict_move_kernel<192, F8> : evict_move_kernel<256, F8>;
+    };
+    auto move = c.f8 ? pick(std::true_type{}) : pick(std::false_type{});
+    hipLaunchKernelGGL(move, dim3((unsigned)e.out_pages, (unsigned)(2 * c.n_kv), (unsigned)e.n_seq), dim3(kMove), 0, stream, c, e);
 }
 
 }  // namespace infr

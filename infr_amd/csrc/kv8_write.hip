@@ -11,6 +11,7 @@
 // segment; value codes turn in LDS. Bound by HBM on 8 bytes read and 2 written per column of a token; a single
 // token per sequence is bound by the launch.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv8.hpp"
 
@@ -27,9 +28,11 @@ __device__ __forceinline__ int pages_written(const Kv8Batch& b, int s) {
     return q.ok && q.n > 0 ? (q.len - 1) / kPage - (q.len - q.n) / kPage + 1 : 0;
 }
 
+template <int DP, bool F8>
 __global__ __launch_bounds__(kThreads) void write_kv8_kernel(Kv8Cache c, Kv8Batch b, const int32_t* __restrict__ slots,
                                                              const float* __restrict__ kx, size_t k_stride,
                                                              const float* __restrict__ vx, size_t v_stride) {
+    constexpr int kGroups = DP / 64;
     __shared__ uint32_t amax[kPage];
     __shared__ __align__(16) uint8_t turn[64 * kTurn];
     int rest = 0;
@@ -44,7 +47,6 @@ __global__ __launch_bounds__(kThreads) void write_kv8_kernel(Kv8Cache c, Kv8Batc
     const int tail_slot = slots[s];
     const bool page_ok = page >= 0 && page < c.n_pages;
     const bool tail_ok = tail_slot >= 0 && tail_slot < c.n_slots;
-    const bool f8 = c.f8 != 0;
     const int tid = threadIdx.x, t = tid >> 2, col = (tid & 3) * 16;
     const int subs = kPage / c.block, sub = t / c.block;
     const int tok = pi * kPage + t;                      // token of this thread
@@ -61,45 +63,58 @@ __global__ __launch_bounds__(kThreads) void write_kv8_kernel(Kv8Cache c, Kv8Batc
     const bool is_new = tok >= slot0 && tok < q.len, is_old = touched && tok < slot0;
     const float old_scale = is_old && !raw && page_ok ? scales[scale_at] : 0.0f;
 
-    // value of column d of this thread's token: zero behind the sequence's end and the row's
-    auto value = [&](int d) -> float {
-        if (d >= c.dim) return 0.0f;
-        if (is_new) return x[(size_t)(q.r0 + tok - slot0) * stride + (size_t)h * c.dim + d];
-        if (!is_old) return 0.0f;
-        if (raw) return c.tail[tail_at + (size_t)(tok - open) * c.dim + d];
-        const size_t at = is_v ? v_at(c, page, h, t, d) : k_at(c, page, h, t, d);
-        return kv8_value((is_v ? c.v : c.k)[at], f8) * old_scale;
-    };
-
-    float r[4][16];  // this thread's columns: 16 of each 64
-    uint32_t top = 0;
-    if (page_ok)
+    // this thread's columns, 16 of each 64: zero behind the sequence's end and the row's
+    float r[kGroups][16];
+    const float* src = nullptr;
+    if (is_new) src = x + (size_t)(q.r0 + tok - slot0) * stride + (size_t)h * c.dim;
+    else if (is_old && raw) src = c.tail + tail_at + (size_t)(tok - open) * c.dim;
+    const bool vec = c.dim % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j * 64 < c.dp)
+    for (int j = 0; j < kGroups; ++j) {
+        const int d0 = j * 64 + col;
+        if (src && vec && d0 + 16 <= c.dim) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    r[j][e] = value(j * 64 + col + e);
-                    top = max(top, abs_bits(r[j][e]));
+            for (int e = 0; e < 16; e += 4) {
+                const float4 y = *reinterpret_cast<const float4*>(src + d0 + e);
+                r[j][e] = y.x, r[j][e + 1] = y.y, r[j][e + 2] = y.z, r[j][e + 3] = y.w;
+            }
+        } else if (src) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) r[j][e] = d0 + e < c.dim ? src[d0 + e] : 0.0f;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                r[j][e] = 0.0f;
+                if (is_old && page_ok && d0 + e < c.dim) {
+                    const size_t at = is_v ? v_at(c, page, h, t, d0 + e) : k_at(c, page, h, t, d0 + e);
+                    r[j][e] = kv8_value<F8>((is_v ? c.v : c.k)[at]) * old_scale;
                 }
+            }
+        }
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = max(top, abs_bits(r[j][e]));
     top = max(top, (uint32_t)__shfl_xor((int)top, 1));
     top = max(top, (uint32_t)__shfl_xor((int)top, 2));
     if ((tid & 3) == 0) amax[t] = top;
     __syncthreads();
     for (int o = 0; o < c.block; ++o) top = max(top, amax[sub * c.block + o]);
-    const float scale = kv8_scale(top, f8);
+    const float scale = kv8_scale(top, F8), inverse = kv8_inverse(scale);
     if (page_ok && touched && t % c.block == 0 && (tid & 3) == 0) scales[scale_at] = scale;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (j * 64 >= c.dp || !page_ok) continue;
+    for (int j = 0; j < kGroups; ++j) {
+        if (!page_ok) continue;
         uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int e = 0; e < 16; ++e) w[e / 4] |= kv8_code(r[j][e], scale, f8) << (8 * (e % 4));
+        for (int e = 0; e < 16; ++e) w[e / 4] |= kv8_code<F8>(r[j][e], scale, inverse) << (8 * (e % 4));
         if (!is_v) {
             if (touched) *reinterpret_cast<uint4*>(c.k + k_at(c, page, h, t, j * 64 + col)) = make_uint4(w[0], w[1], w[2], w[3]);
             continue;
         }
-        __syncthreads();  // (page_ok and dp are the workgroup's)
+        __syncthreads();  // (page_ok is the workgroup's)
 #pragma unroll
         for (int e = 0; e < 16; ++e) turn[(col + e) * kTurn + t] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
         __syncthreads();
@@ -124,7 +139,7 @@ __global__ __launch_bounds__(kThreads) void write_kv8_kernel(Kv8Cache c, Kv8Batc
     const bool lpage_ok = lpage >= 0 && lpage < c.n_pages;
     if (last == open && is_old && !raw && page_ok)       // rows only the cache had, at their values there
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < kGroups; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 if (j * 64 + col + e < c.dim) c.tail[tail_at + (size_t)(tok - open) * c.dim + j * 64 + col + e] = r[j][e];
@@ -145,8 +160,13 @@ void launch_write_kv8(const Kv8Cache& c, const Kv8Batch& b, const int32_t* slots
                       const float* v, size_t v_stride, hipStream_t stream) {
     // a run of n rows touches at most n and at most n / 64 + 2 pages
     const unsigned pages = (unsigned)std::min<size_t>((size_t)b.rows, (size_t)b.rows / kPage + 2 * (size_t)b.n_seq);
-    hipLaunchKernelGGL(write_kv8_kernel, dim3(pages, (unsigned)c.n_kv, 2), dim3(kThreads), 0, stream, c, b, slots, k,
-                       k_stride, v, v_stride);
+    auto pick = [&](auto f8) {
+        constexpr bool F8 = decltype(f8)::value;
+        return c.dp == 64 ? write_kv8_kernel<64, F8> : c.dp == 128 ? write_kv8_kernel<128, F8>
+             : c.dp == 192 ? write_kv8_kernel<192, F8> : write_kv8_kernel<256, F8>;
+    };
+    auto kernel = c.f8 ? pick(std::true_type{}) : pick(std::false_type{});
+    hipLaunchKernelGGL(kernel, dim3(pages, (unsigned)c.n_kv, 2), dim3(kThreads), 0, stream, c, b, slots, k, k_stride, v, v_stride);
 }
 
 }  // namespace infr

@@ -643,6 +643,25 @@ def test_evict_ties_zeros_and_odd_sums(be):
 
 
 @gpu
+@pytest.mark.parametrize("n_len", [4096, 4097, 32768, 32769, 70001])
+@pytest.mark.parametrize("sums", ["spread", "steps", "one"])
+def test_evict_of_long_sequences(be, n_len, sums):
+    """Lengths either side of what a workgroup holds at once; sums of many sizes, of few values and all equal."""
+    rng = np.random.default_rng(n_len)
+    n_pages = -(-n_len // 64) + 3
+    c = orc.Cache(n_pages, 1, 2, 1, "i8", 16)
+    order = rng.permutation(n_pages)
+    c.k[...], c.v[...] = rng.integers(0, 256, c.k.shape), rng.integers(0, 256, c.v.shape)
+    c.k[..., 2:] = 0
+    c.v[:, :, 2:] = 0
+    c.k_scale[...], c.v_scale[...] = rng.random(c.k_scale.shape) + 0.5, rng.random(c.v_scale.shape) + 0.5
+    c.pos[order[:-3]] = np.arange((n_pages - 3) * 64, dtype=np.int32).reshape(-1, 1, 64)
+    shape = c.sums.shape
+    c.sums[...] = {"spread": np.exp(10 * rng.standard_normal(shape)), "steps": rng.integers(0, 5, shape) * 0.125, "one": np.full(shape, 0.5)}[sums]
+    check_evict(be, c, [order[:-3].tolist()], [n_len], [order[-3:].tolist()], 190, 3, 60)
+
+
+@gpu
 def test_evict_leaves_alone_sequences_with_wrong_tables(be):
     rng = np.random.default_rng(24)
     c, pages, free = filled(rng, "i8", 16, 2, 32, (200, 200, 200, 200), spare=8)
