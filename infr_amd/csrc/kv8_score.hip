@@ -37,23 +37,46 @@ __global__ __launch_bounds__(64 * kStepWaves, DP <= 128 ? 2 : 1) void score_step
                                                                                        float decay, int target) {
     constexpr int kCols = DP / 64;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    const int cp = piece_pages(b, a, c.n_kv, target, true);
-    int rest = 0;
-    const int s = find_seq(b.n_seq, (int)blockIdx.x, &rest, [&](int i) {
-        const SeqWork w = seq_work(b, a, i, true);
-        return c.n_kv * w.tiles * ((w.pages + cp - 1) / cp);
-    });
-    if (s < 0) return;
-    const Kv8Seq q = kv8_seq(b, s);
-    if (!q.ok) return;
-    const SeqWork work = seq_work(b, a, s, true);
-    const int parts = (work.pages + cp - 1) / cp, part = rest % parts, h = rest / parts;
+    const SeqCut cut = find_cut(b, a, c.n_kv, target, true, -1, (int)blockIdx.x);
+    if (cut.s < 0 || !cut.q.ok) return;
+    const int s = cut.s, parts = cut.parts, rest = (int)blockIdx.x - cut.first;
+    const Kv8Seq q = cut.q;
+    const SeqWork work = cut.work;
+    const int part = rest % parts, h = rest / parts;
     const int per = (work.pages + parts - 1) / parts;
     const int p0 = part * per, p1 = min(p0 + per, (q.len + kPage - 1) / kPage);
     const bool live = col < q.n * a.group;
     const int i = live ? col / a.group : max(q.n - 1, 0), head = h * a.group + (live ? col % a.group : 0);
     const bool any_row = q.n > 0;
 
+    const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+    const bool use_pos = GEN && (a.window > 0 || a.slopes || a.first || a.prefix);
+    const int all_see = a.causal ? q.len - q.n + 1 : q.len;
+    const int32_t* table = b.pages + (size_t)s * b.max_pages;
+    const int subs = kPage / c.block;
+    uint4 kf[4][kCols];
+    float ks = 0.0f;
+    int page = 0, ids = 0;
+    auto load_ids = [&](int p) {
+        const int at = p + lane * kStepWaves;
+        ids = at < p1 ? table[at] : 0;
+        if (ids < 0 || ids >= c.n_pages) ids = -1;
+    };
+    auto load_keys = [&](int n) {
+        page = __builtin_amdgcn_readlane(ids, n);
+        const size_t at = (size_t)max(page, 0) * c.n_kv + h;
+        const uint8_t* kp = c.k + at * (DP * kPage) + (16 * (col >> 2) + (col & 3)) * 64 + 16 * g;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < kCols; ++j) kf[t][j] = load_stream(kp + j * kPage * 64 + t * 4 * 64);
+        ks = c.ks[at * subs + g * 16 / c.block];
+    };
+    int p = p0 + wave, n = 0;
+    if (p < p1) {
+        load_ids(p);
+        load_keys(0);
+    }
     h8 qh[2 * kCols], ql[2 * kCols];
     float row_factor, row_lse = 0.0f;
     Kv8Row row{};
@@ -87,34 +110,6 @@ __global__ __launch_bounds__(64 * kStepWaves, DP <= 128 ? 2 : 1) void score_step
             row = kv8_row(b, a, q, s, i, head);
             row_lse = lse[(size_t)(q.r0 + i) * a.n_head + head] * kLog2e;
         }
-    }
-    const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
-    const bool use_pos = GEN && (a.window > 0 || a.slopes || a.first || a.prefix);
-    const int all_see = a.causal ? q.len - q.n + 1 : q.len;
-    const int32_t* table = b.pages + (size_t)s * b.max_pages;
-    const int subs = kPage / c.block;
-    uint4 kf[4][kCols];
-    float ks = 0.0f;
-    int page = 0, ids = 0;
-    auto load_ids = [&](int p) {
-        const int at = p + lane * kStepWaves;
-        ids = at < p1 ? table[at] : 0;
-        if (ids < 0 || ids >= c.n_pages) ids = -1;
-    };
-    auto load_keys = [&](int n) {
-        page = __builtin_amdgcn_readlane(ids, n);
-        const size_t at = (size_t)max(page, 0) * c.n_kv + h;
-        const uint8_t* kp = c.k + at * (DP * kPage) + (16 * (col >> 2) + (col & 3)) * 64 + 16 * g;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int j = 0; j < kCols; ++j) kf[t][j] = *reinterpret_cast<const uint4*>(kp + j * kPage * 64 + t * 4 * 64);
-        ks = c.ks[at * subs + g * 16 / c.block];
-    };
-    int p = p0 + wave, n = 0;
-    if (p < p1) {
-        load_ids(p);
-        load_keys(0);
     }
     while (p < p1) {
         const int now = page;

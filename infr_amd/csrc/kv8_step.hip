@@ -9,6 +9,7 @@
 // The pages of all sequences are cut into pieces of one size, found on the device from the lengths: long sequences
 // get many workgroups, short ones one, and no piece is empty. A sequence in one piece writes its result; the pieces
 // of others are joined by a second kernel, in their order.
+#include <cstdlib>
 #include "kv8_attn.hpp"
 #include "kv8_device.hpp"
 
@@ -34,16 +35,12 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void step_kernel(Kv
     __shared__ float part_o[kWaves][kRows * (DP + 4)];
     __shared__ float part_m[kWaves][kRows], part_l[kWaves][kRows];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    const int cp = piece_pages(b, a, c.n_kv, target);
-    int rest = 0;
-    const int s = find_seq(b.n_seq, (int)blockIdx.x, &rest, [&](int i) {
-        const SeqWork w = seq_work(b, a, i);
-        return c.n_kv * w.tiles * ((w.pages + cp - 1) / cp);
-    });
-    if (s < 0) return;
-    const Kv8Seq q = kv8_seq(b, s);
-    const SeqWork work = seq_work(b, a, s);
-    const int parts = (work.pages + cp - 1) / cp, part = rest % parts, rt = rest / parts % work.tiles, h = rest / parts / work.tiles;
+    const SeqCut cut = find_cut(b, a, c.n_kv, target, false, -1, (int)blockIdx.x);
+    if (cut.s < 0) return;
+    const int s = cut.s, parts = cut.parts, rest = (int)blockIdx.x - cut.first;
+    const Kv8Seq q = cut.q;
+    const SeqWork work = cut.work;
+    const int part = rest % parts, rt = rest / parts % work.tiles, h = rest / parts / work.tiles;
     const int per = (work.pages + parts - 1) / parts;
     const int p0 = work.p_lo + part * per;
     const int p1 = q.ok ? min(p0 + per, (q.len + kPage - 1) / kPage) : p0;
@@ -52,36 +49,6 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void step_kernel(Kv
     const bool live = rr < n_rows;
     const int i = live ? rr / a.group : q.n - 1, head = h * a.group + (live ? rr % a.group : 0);
 
-    // the query row, scaled by a power of two, as hi + lo
-    h8 qh[2 * kCols], ql[2 * kCols];
-    float row_factor;
-    {
-        const float* x = a.q + (size_t)(q.r0 + i) * a.q_stride + (size_t)head * c.dim;
-        float v[16 * kCols];
-        uint32_t top = 0;
-#pragma unroll
-        for (int j = 0; j < kCols; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int d = j * 64 + g * 16 + e;
-                v[j * 16 + e] = live && d < c.dim ? x[d] : 0.0f;
-                top = max(top, abs_bits(v[j * 16 + e]));
-            }
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-        const int e = row_exponent(top);
-        const float down = pow2(-e);
-        row_factor = a.scale * pow2(e);
-#pragma unroll
-        for (int k = 0; k < 2 * kCols; ++k)
-#pragma unroll
-            for (int o = 0; o < 4; ++o) {
-                h2 hi, lo;
-                split_pair(v[k * 8 + 2 * o] * down, v[k * 8 + 2 * o + 1] * down, &hi, &lo);
-                qh[k][2 * o] = hi[0], qh[k][2 * o + 1] = hi[1];
-                ql[k][2 * o] = lo[0], ql[k][2 * o + 1] = lo[1];
-            }
-    }
     const Kv8Row row = kv8_row(b, a, q, s, i, head);
     const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
     const bool use_pos = GEN && (a.window > 0 || a.slopes || a.first || a.prefix);
@@ -114,7 +81,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void step_kernel(Kv
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int j = 0; j < kCols; ++j) kf[t][j] = *reinterpret_cast<const uint4*>(kp + j * kPage * 64 + t * 4 * 64);
+            for (int j = 0; j < kCols; ++j) kf[t][j] = load_stream(kp + j * kPage * 64 + t * 4 * 64);
         const size_t sc = ((size_t)page * c.n_kv + h) * subs + g * 16 / c.block;
         ks = c.ks[sc];
         vs = c.vs[sc];
@@ -124,10 +91,40 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void step_kernel(Kv
         load_ids(p);
         load_keys(0);
     }
+    // the query row, scaled by a power of two, as hi + lo
+    h8 qh[2 * kCols], ql[2 * kCols];
+    float row_factor;
+    {
+        const float* x = a.q + (size_t)(q.r0 + i) * a.q_stride + (size_t)head * c.dim;
+        float v[16 * kCols];
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < kCols; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int d = j * 64 + g * 16 + e;
+                v[j * 16 + e] = live && d < c.dim ? x[d] : 0.0f;
+                top = max(top, abs_bits(v[j * 16 + e]));
+            }
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+        const int e = row_exponent(top);
+        const float down = pow2(-e);
+        row_factor = a.scale * pow2(e);
+#pragma unroll
+        for (int k = 0; k < 2 * kCols; ++k)
+#pragma unroll
+            for (int o = 0; o < 4; ++o) {
+                h2 hi, lo;
+                split_pair(v[k * 8 + 2 * o] * down, v[k * 8 + 2 * o + 1] * down, &hi, &lo);
+                qh[k][2 * o] = hi[0], qh[k][2 * o + 1] = hi[1];
+                ql[k][2 * o] = lo[0], ql[k][2 * o + 1] = lo[1];
+            }
+    }
     while (p < p1) {
         const uint8_t* vp = c.v + ((size_t)page * c.n_kv + h) * kv_stride + col * kPage + 16 * g;
 #pragma unroll
-        for (int k = 0; k < kOut; ++k) vf[k] = *reinterpret_cast<const uint4*>(vp + k * 16 * kPage);
+        for (int k = 0; k < kOut; ++k) vf[k] = load_stream(vp + k * 16 * kPage);
         int kpos[16];
         if (use_pos) {
             const int4* pp = reinterpret_cast<const int4*>(c.pos + ((size_t)page * c.n_kv + h) * kPage + 16 * g);
@@ -302,23 +299,15 @@ template <int DP>
 __global__ __launch_bounds__(256) void join_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a, float* __restrict__ dst,
                                                    float* __restrict__ lse, const float* __restrict__ scratch, int target,
                                                    int max_tiles) {
-    __shared__ float part[256];
+    __shared__ __align__(16) float part[1024 / DP][DP];
     const int lane = threadIdx.x & 63;
     const int rt = blockIdx.x % max_tiles, h = blockIdx.x / max_tiles % c.n_kv, s = blockIdx.x / max_tiles / c.n_kv;
     const int r = blockIdx.y, r_all = rt * kRows + r;
-    const Kv8Seq q = kv8_seq(b, s);
-    if (r_all >= q.n * a.group) return;
-    const int cp = piece_pages(b, a, c.n_kv, target);
-    const SeqWork work = seq_work(b, a, s);
-    const int parts = (work.pages + cp - 1) / cp;
-    if (parts == 1) return;
-    int before = 0;
-    for (int k = lane; k < s; k += 64) {
-        const SeqWork w = seq_work(b, a, k);
-        before += c.n_kv * w.tiles * ((w.pages + cp - 1) / cp);
-    }
-    for (int o = 1; o < 64; o <<= 1) before += __shfl_xor(before, o);
-    const float* first = scratch + (size_t)(before + (h * work.tiles + rt) * parts) * kPieceFloats<DP>;
+    const SeqCut cut = find_cut(b, a, c.n_kv, target, false, s, 0);
+    const Kv8Seq q = cut.q;
+    const int parts = cut.parts;
+    if (r_all >= q.n * a.group || parts == 1) return;
+    const float* first = scratch + (size_t)(cut.first + (h * cut.work.tiles + rt) * parts) * kPieceFloats<DP>;
     auto max_of = [&](int k) { return first[(size_t)k * kPieceFloats<DP> + kRows * DP + r]; };
     auto sum_of = [&](int k) { return first[(size_t)k * kPieceFloats<DP> + kRows * DP + kRows + r]; };
     float m = kNoMax;
@@ -330,19 +319,23 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8Cache c, Kv8Batch b, Kv8At
     const size_t out = (size_t)(q.r0 + r_all / a.group) * a.n_head + h * a.group + r_all % a.group;
     if (lse && threadIdx.x == 0)
         lse[out] = l == 0.0f ? -__builtin_inff() : (__builtin_amdgcn_logf(l) + m - (float)kBias) * kLn2;
-    constexpr int kGroups = 256 / DP;  // threads that share a column, each every kGroups-th piece
-    const int d = threadIdx.x % DP, first_k = threadIdx.x / DP;
-    float x = 0.0f;
-    if (first_k < kGroups)
-        for (int k = first_k; k < parts; k += kGroups)
-            x += first[(size_t)k * kPieceFloats<DP> + r * DP + d] * __builtin_amdgcn_exp2f(max_of(k) - m);
-    part[threadIdx.x] = x;
+    // four columns to a thread; the threads that share them take every kGroups-th piece
+    constexpr int kFours = DP / 4, kGroups = 256 / kFours;
+    const int d4 = threadIdx.x % kFours, group = threadIdx.x / kFours;
+    f4 x = f4{0, 0, 0, 0};
+    if (group < kGroups) {
+#pragma unroll 4
+        for (int k = group; k < parts; k += kGroups)
+            x += *reinterpret_cast<const f4*>(first + (size_t)k * kPieceFloats<DP> + r * DP + 4 * d4) * __builtin_amdgcn_exp2f(max_of(k) - m);
+        *reinterpret_cast<f4*>(&part[group][4 * d4]) = x;
+    }
     __syncthreads();
-    if ((int)threadIdx.x >= DP || d >= c.dim) return;
-    x = 0.0f;
+    const int d = threadIdx.x;
+    if (d >= c.dim) return;
+    float y = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kGroups; ++k) x += part[k * DP + d];
-    dst[out * c.dim + d] = l == 0.0f ? 0.0f : x / l;
+    for (int k = 0; k < kGroups; ++k) y += part[k][d];
+    dst[out * c.dim + d] = l == 0.0f ? 0.0f : y / l;
 }
 
 int max_tiles_of(int group, int max_q) { return (int)(((int64_t)max_q * group + kRows - 1) / kRows); }
@@ -364,7 +357,7 @@ void launch_step_dp(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, floa
 }  // namespace
 
 // Pieces aimed at: two workgroups for each compute unit.
-int step_target(int cus) { return 2 * cus; }
+int step_target(int cus) { static const int f = getenv("KV8_T") ? atoi(getenv("KV8_T")) : 2; return f * cus; }
 // Upper bound of the pieces: the total is cut into `target`, and each (sequence, head, row tile) rounds up once.
 size_t step_items(int cus, int n_kv, int group, int n_seq, int max_q, int max_pages) {
     const size_t tiles = (size_t)n_seq * n_kv * max_tiles_of(group, max_q);
