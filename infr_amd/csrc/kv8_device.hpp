@@ -96,6 +96,27 @@ __device__ __forceinline__ int row_exponent(uint32_t amax_bits) {
 }
 __device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
 
+// N floats of a row of `dim` from column d0 on, zeros behind its end; N is a multiple of 4 and so is d0. `vec`: the
+// row's length is a multiple of 4 and it is aligned to 16 bytes.
+template <int N>
+__device__ __forceinline__ void load_row(const float* x, int d0, int dim, bool live, bool vec, float* v) {
+#pragma unroll
+    for (int e = 0; e < N; e += 4) {
+        const int d = d0 + e;
+        f4 y = f4{0, 0, 0, 0};
+        if (live && d < dim) {
+            if (vec) y = *reinterpret_cast<const f4*>(x + d);
+            else
+#pragma unroll
+                for (int k = 0; k < 4; ++k) y[k] = d + k < dim ? x[d + k] : 0.0f;
+        }
+        v[e] = y[0], v[e + 1] = y[1], v[e + 2] = y[2], v[e + 3] = y[3];
+    }
+}
+__device__ __forceinline__ bool rows_vec(const Kv8Cache& c, const Kv8Attn& a) {
+    return c.dim % 4 == 0 && a.q_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0;
+}
+
 // c * tanh(s / c), to the last bits of s: an odd polynomial (the series of tanh) where tanh is nearly its
 // argument, 1 - 2 / (e^2y + 1) beyond, where the difference cancels no more than two bits.
 __device__ __forceinline__ float cap_score(float s, float c, float inv_c) {
@@ -136,16 +157,17 @@ __device__ __forceinline__ Kv8Row kv8_row(const Kv8Batch& b, const Kv8Attn& a, c
 // ---- how the kernels for few rows cut a batch's pages: pieces of one size, found from the lengths ----
 
 constexpr int kStepWaves = 4;   // waves of a workgroup, each a page at a time
-constexpr int kStepRows = 16;   // query rows of a workgroup
+constexpr int kStepRows = 16;   // query rows of a workgroup, or half of them: see step_rows
+constexpr int kWholePages = 12; // sequences of up to so many pages are one piece: four pages a wave cost less than a join
 
 // Row tiles, first page any row sees, pages from there. `all`: every cached page is gone over by one tile, whether
 // rows see it or not (ScoreKv8 lets sums decay).
 struct SeqWork {
     int tiles, p_lo, pages;
 };
-__device__ __forceinline__ SeqWork seq_work(const Kv8Seq& q, const Kv8Attn& a, bool all) {
+__device__ __forceinline__ SeqWork seq_work(const Kv8Seq& q, const Kv8Attn& a, int rows, bool all) {
     SeqWork w;
-    w.tiles = all ? 1 : (q.n * a.group + kStepRows - 1) / kStepRows;
+    w.tiles = all ? 1 : (q.n * a.group + rows - 1) / rows;
     w.p_lo = 0;
     w.pages = 1;  // of a sequence whose tables are wrong one item per tile writes the rows' NaN
     if (q.ok) {
@@ -155,6 +177,54 @@ __device__ __forceinline__ SeqWork seq_work(const Kv8Seq& q, const Kv8Attn& a, b
         w.pages = max((q.len + kPage - 1) / kPage - w.p_lo, 1);
     }
     return w;
+}
+
+// Value of lane l ^ 8 (within rows of 16 lanes, which a rotation by 8 swaps the halves of).
+__device__ __forceinline__ float from_other_eight(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xF, 0xF, true));
+}
+
+// The query rows of a workgroup in LDS as f16, scaled by their powers of two: low parts behind the high ones (with
+// ROWS = 8 the two are the 16 columns of one MFMA). Rows are padded by 16 bytes.
+template <int DP, int ROWS>
+struct StepQ {
+    _Float16 x[2 * ROWS][DP + 8];
+    float factor[ROWS];
+};
+// 256 threads bring in rows 0 .. ROWS - 1 of `tile`, row by row side by side.
+template <int DP, int ROWS>
+__device__ __forceinline__ void stage_rows(StepQ<DP, ROWS>& st, const Kv8Cache& c, const Kv8Attn& a, const Kv8Seq& q, int h, int row0) {
+    constexpr int kEach = ROWS, kSide = 256 / ROWS;  // threads of a row; each four columns at a time
+    constexpr int kFours = (DP / 4 + kSide - 1) / kSide;
+    static_assert(kEach * kSide == 256, "a workgroup of 256");
+    const int r = (int)threadIdx.x / kSide, t = (int)threadIdx.x % kSide, rr = row0 + r;
+    const bool live = rr < q.n * a.group, vec = rows_vec(c, a);
+    const float* x = a.q;
+    if (live) x += (size_t)(q.r0 + rr / a.group) * a.q_stride + (size_t)(h * a.group + rr % a.group) * c.dim;
+    float v[4 * kFours];
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < kFours; ++k) {
+        load_row<4>(x, (k * kSide + t) * 4, c.dim, live, vec, v + 4 * k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max(top, abs_bits(v[4 * k + e]));
+    }
+#pragma unroll
+    for (int o = 1; o < kSide; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+    const int e2 = row_exponent(top);
+    const float down = pow2(-e2);
+#pragma unroll
+    for (int k = 0; k < kFours; ++k) {
+        const int d = (k * kSide + t) * 4;
+        h2 h0, h1, l0, l1;
+        split_pair(v[4 * k] * down, v[4 * k + 1] * down, &h0, &l0);
+        split_pair(v[4 * k + 2] * down, v[4 * k + 3] * down, &h1, &l1);
+        if (d < DP) {
+            *reinterpret_cast<h4*>(&st.x[r][d]) = h4{h0[0], h0[1], h1[0], h1[1]};
+            *reinterpret_cast<h4*>(&st.x[ROWS + r][d]) = h4{l0[0], l0[1], l1[0], l1[1]};
+        }
+    }
+    if (t == 0) st.factor[r] = a.scale * pow2(e2);
 }
 
 // A sequence's share of the pieces: `parts` of each (head, row tile), the first of them number `first`.
@@ -167,14 +237,15 @@ struct SeqCut {
 // The share of sequence `want`, or, with want < 0, of the sequence that holds piece `item`. About `target` pieces are
 // aimed at, of at least one page for each wave of a workgroup. Up to 64 sequences take one round of loads, and the
 // sequence found is passed between the lanes; more of them take a loop over the tables and another over the counts.
-__device__ __forceinline__ SeqCut find_cut(const Kv8Batch& b, const Kv8Attn& a, int n_kv, int target, bool all, int want, int item) {
+__device__ __forceinline__ SeqCut find_cut(const Kv8Batch& b, const Kv8Attn& a, int n_kv, int rows, int target, bool all, int want,
+                                           int item) {
     const int lane = (int)(threadIdx.x & 63);
     Kv8Seq q{};
     SeqWork w{};
     float total = 0.0f;
     for (int s = lane; s < b.n_seq; s += 64) {
         q = kv8_seq(b, s);
-        w = seq_work(q, a, all);
+        w = seq_work(q, a, rows, all);
         total += (float)w.tiles * (float)w.pages;
     }
 #pragma unroll
@@ -188,10 +259,10 @@ __device__ __forceinline__ SeqCut find_cut(const Kv8Batch& b, const Kv8Attn& a, 
         if (b.n_seq > 64) {
             if (s < b.n_seq) {
                 q = kv8_seq(b, s);
-                w = seq_work(q, a, all);
+                w = seq_work(q, a, rows, all);
             }
         }
-        const int parts = s < b.n_seq ? (w.pages + size - 1) / size : 0, n = n_kv * w.tiles * parts;
+        const int parts = s < b.n_seq ? (w.pages <= kWholePages ? 1 : (w.pages + size - 1) / size) : 0, n = n_kv * w.tiles * parts;
         const int sum = wave_scan(s < b.n_seq ? n : 0);
         const unsigned long long hit = __ballot(want >= 0 ? s == want : item - before < sum);
         if (hit) {

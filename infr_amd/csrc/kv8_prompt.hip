@@ -96,27 +96,25 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
     float row_factor;
     {
         const float* x = a.q + (size_t)(q.r0 + i) * a.q_stride + (size_t)head * c.dim;
+        const bool vec = rows_vec(c, a);
+        float v[kSteps][8];
         uint32_t top = 0;
-        for (int d = hf * 8; d < c.dim; d += 16)
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (live && d + e < c.dim) top = max(top, abs_bits(x[d + e]));
+        for (int k = 0; k < kSteps; ++k) {
+            load_row<8>(x, k * 16 + hf * 8, c.dim, live, vec, v[k]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max(top, abs_bits(v[k][e]));
+        }
         top = max(top, (uint32_t)__shfl_xor((int)top, 32));
         const int e2 = row_exponent(top);
         const float down = pow2(-e2);
         row_factor = a.scale * pow2(e2);
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int d = k * 16 + hf * 8 + e;
-                v[e] = live && d < c.dim ? x[d] * down : 0.0f;
-            }
 #pragma unroll
             for (int o = 0; o < 4; ++o) {
                 h2 u, w;
-                split_pair(v[2 * o], v[2 * o + 1], &u, &w);
+                split_pair(v[k][2 * o] * down, v[k][2 * o + 1] * down, &u, &w);
                 qh[k][2 * o] = u[0], qh[k][2 * o + 1] = u[1];
                 ql[k][2 * o] = w[0], ql[k][2 * o + 1] = w[1];
             }

@@ -37,7 +37,7 @@ __global__ __launch_bounds__(64 * kStepWaves, DP <= 128 ? 2 : 1) void score_step
                                                                                        float decay, int target) {
     constexpr int kCols = DP / 64;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    const SeqCut cut = find_cut(b, a, c.n_kv, target, true, -1, (int)blockIdx.x);
+    const SeqCut cut = find_cut(b, a, c.n_kv, kStepRows, target, true, -1, (int)blockIdx.x);
     if (cut.s < 0 || !cut.q.ok) return;
     const int s = cut.s, parts = cut.parts, rest = (int)blockIdx.x - cut.first;
     const Kv8Seq q = cut.q;
@@ -47,7 +47,6 @@ __global__ __launch_bounds__(64 * kStepWaves, DP <= 128 ? 2 : 1) void score_step
     const int p0 = part * per, p1 = min(p0 + per, (q.len + kPage - 1) / kPage);
     const bool live = col < q.n * a.group;
     const int i = live ? col / a.group : max(q.n - 1, 0), head = h * a.group + (live ? col % a.group : 0);
-    const bool any_row = q.n > 0;
 
     const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
     const bool use_pos = GEN && (a.window > 0 || a.slopes || a.first || a.prefix);
@@ -77,39 +76,22 @@ __global__ __launch_bounds__(64 * kStepWaves, DP <= 128 ? 2 : 1) void score_step
         load_ids(p);
         load_keys(0);
     }
+    __shared__ StepQ<DP, kStepRows> rows_q;
+    stage_rows<DP, kStepRows>(rows_q, c, a, q, h, 0);
+    __syncthreads();
     h8 qh[2 * kCols], ql[2 * kCols];
-    float row_factor, row_lse = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2 * kCols; ++k) {
+        const int d = (k / 2) * 64 + g * 16 + (k % 2) * 8;
+        qh[k] = *reinterpret_cast<const h8*>(&rows_q.x[col][d]);
+        ql[k] = *reinterpret_cast<const h8*>(&rows_q.x[16 + col][d]);
+    }
+    const float row_factor = rows_q.factor[col];
     Kv8Row row{};
-    {
-        const float* x = a.q + (size_t)(any_row ? q.r0 + i : 0) * a.q_stride + (size_t)head * c.dim;
-        float v[16 * kCols];
-        uint32_t top = 0;
-#pragma unroll
-        for (int j = 0; j < kCols; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int d = j * 64 + g * 16 + e;
-                v[j * 16 + e] = live && d < c.dim ? x[d] : 0.0f;
-                top = max(top, abs_bits(v[j * 16 + e]));
-            }
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-        const int e = row_exponent(top);
-        const float down = pow2(-e);
-        row_factor = a.scale * pow2(e);
-#pragma unroll
-        for (int k = 0; k < 2 * kCols; ++k)
-#pragma unroll
-            for (int o = 0; o < 4; ++o) {
-                h2 hi, lo;
-                split_pair(v[k * 8 + 2 * o] * down, v[k * 8 + 2 * o + 1] * down, &hi, &lo);
-                qh[k][2 * o] = hi[0], qh[k][2 * o + 1] = hi[1];
-                ql[k][2 * o] = lo[0], ql[k][2 * o + 1] = lo[1];
-            }
-        if (live) {
-            row = kv8_row(b, a, q, s, i, head);
-            row_lse = lse[(size_t)(q.r0 + i) * a.n_head + head] * kLog2e;
-        }
+    float row_lse = 0.0f;
+    if (live) {
+        row = kv8_row(b, a, q, s, i, head);
+        row_lse = lse[(size_t)(q.r0 + i) * a.n_head + head] * kLog2e;
     }
     while (p < p1) {
         const int now = page;
@@ -237,13 +219,13 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void score_prompt_kern
     float in_lse = 0.0f;
     bool in_live = false;
     const int my_row = tid >> 3, my_col = (tid & 7) * kEach;
+    const bool vec = rows_vec(c, a);
     auto fetch = [&](int rt) {
         const int rr = rt * kTile + my_row;
         in_live = rr < q.n * a.group;
         const int i = in_live ? rr / a.group : q.n - 1, head = h * a.group + (in_live ? rr % a.group : 0);
         const float* x = a.q + (size_t)(q.r0 + i) * a.q_stride + (size_t)head * c.dim;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) v[e] = in_live && my_col + e < c.dim ? x[my_col + e] : 0.0f;
+        load_row<kEach>(x, my_col, c.dim, in_live, vec, v);
         if ((tid & 7) == 0) {
             in = kv8_row(b, a, q, s, i, head);
             in_lse = lse[(size_t)(q.r0 + i) * a.n_head + head] * kLog2e;
@@ -389,7 +371,8 @@ void launch_score_dp(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, con
         auto kernel = c.f8 ? (gen ? score_step_kernel<DP, true, true> : score_step_kernel<DP, true, false>)
                            : (gen ? score_step_kernel<DP, false, true> : score_step_kernel<DP, false, false>);
         const unsigned items = (unsigned)step_items(cus, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);
-        hipLaunchKernelGGL(kernel, dim3(items), dim3(64 * kStepWaves), 0, stream, c, b, a, lse, decay, step_target(cus));
+        hipLaunchKernelGGL(kernel, dim3(items), dim3(64 * kStepWaves), 0, stream, c, b, a, lse, decay,
+                           step_target(cus, (int64_t)b.n_seq * c.n_kv));
         return;
     }
     const int parts = parts_of(cus, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);

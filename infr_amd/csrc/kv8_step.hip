@@ -1,15 +1,16 @@
 // AttentionKv8 for few rows per sequence: decode steps and drafts. Bound by reading the cache once.
 //
 // Up to 16 query rows of one (sequence, KV head) - its rows times the heads of the group - are one column tile of
-// the 16x16x32 f16 MFMA. A wave takes one page at a time: 64 tokens as four row tiles chosen so that lane group g
+// the 16x16x32 f16 MFMA; up to 8 of them take its other 8 columns for their low parts, and half the products. A wave takes one page at a time: 64 tokens as four row tiles chosen so that lane group g
 // holds tokens 16 g .. 16 g + 15 of its query row, which is what P.V wants side by side from V^T's 16-byte pieces.
 // Key and value codes go from HBM to registers in 16-byte loads (whole lines per instruction), become f16 there and
 // feed the MFMA; the next page's keys are requested before the current page's softmax, its values before its scores.
 //
 // The pages of all sequences are cut into pieces of one size, found on the device from the lengths: long sequences
 // get many workgroups, short ones one, and no piece is empty. A sequence in one piece writes its result; the pieces
-// of others are joined by a second kernel, in their order.
-#include <cstdlib>
+// of others are joined by a second kernel, in their order. (A join by the workgroup that comes last to its row tile
+// saves that launch but costs its own round trips past the L2, which the XCDs do not share: 53 us against 49 for two
+// sequences of 115000 tokens, 48 against 44 for drafts of four tokens.)
 #include "kv8_attn.hpp"
 #include "kv8_device.hpp"
 
@@ -18,24 +19,27 @@ namespace infr {
 namespace {
 
 constexpr int kWaves = kStepWaves;
-constexpr int kRows = kStepRows;
 constexpr int kBias = 10;    // softmax weights are 2^kBias at the running maximum ..
 constexpr float kLag = 4.0f; // .. which may lag behind the true one by this many powers of two
 
-// O, maximum and sum of a piece: f32 [rows][DP], then [rows] maxima and [rows] sums.
-template <int DP>
-constexpr int kPieceFloats = kRows * DP + 2 * kRows;
+// O, maxima and sums of a piece: f32 [rows][DP], then [rows] pairs of a maximum and a sum.
+template <int DP, int ROWS>
+constexpr int kPieceFloats = ROWS * DP + 2 * ROWS;
 
-template <int DP, bool F8, bool GEN>
-__global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void step_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a,
+template <int DP, int ROWS, bool F8, bool GEN>
+__global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192 && ROWS == 8) ? 2 : 1) void step_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a,
                                                                              float* __restrict__ dst, float* __restrict__ lse,
                                                                              float* __restrict__ scratch, int target) {
     constexpr int kCols = DP / 64;   // 64-column groups of a key
     constexpr int kOut = DP / 16;    // 16-column groups of a value
-    __shared__ float part_o[kWaves][kRows * (DP + 4)];
-    __shared__ float part_m[kWaves][kRows], part_l[kWaves][kRows];
+    constexpr int kFours = DP / 4, kThreads = 64 * kWaves;
+    constexpr int kPart = 16 * (DP + 4);
+    constexpr bool PACK = ROWS == 8;   // columns 8..15 are the low parts of columns 0..7
+    __shared__ __align__(16) float part_o[kWaves * kPart];  // the waves' outputs; before, the query rows
+    static_assert(sizeof(StepQ<DP, ROWS>) <= sizeof(part_o), "the rows fit");
+    __shared__ float part_m[kWaves][16], part_l[kWaves][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    const SeqCut cut = find_cut(b, a, c.n_kv, target, false, -1, (int)blockIdx.x);
+    const SeqCut cut = find_cut(b, a, c.n_kv, ROWS, target, false, -1, (int)blockIdx.x);
     if (cut.s < 0) return;
     const int s = cut.s, parts = cut.parts, rest = (int)blockIdx.x - cut.first;
     const Kv8Seq q = cut.q;
@@ -45,7 +49,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void step_kernel(Kv
     const int p0 = work.p_lo + part * per;
     const int p1 = q.ok ? min(p0 + per, (q.len + kPage - 1) / kPage) : p0;
     const int n_rows = q.n * a.group;
-    const int rr = rt * kRows + col;                   // this lane's query row
+    const int rr = rt * ROWS + col % ROWS;                   // this lane's query row
     const bool live = rr < n_rows;
     const int i = live ? rr / a.group : q.n - 1, head = h * a.group + (live ? rr % a.group : 0);
 
@@ -53,7 +57,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void step_kernel(Kv
     const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
     const bool use_pos = GEN && (a.window > 0 || a.slopes || a.first || a.prefix);
     // tokens below this one are seen by every row of the tile (without masks by position)
-    const int all_see = a.causal ? q.len - q.n + rt * kRows / a.group + 1 : q.len;
+    const int all_see = a.causal ? q.len - q.n + rt * ROWS / a.group + 1 : q.len;
 
     f4 o[kOut];
 #pragma unroll
@@ -91,36 +95,18 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void step_kernel(Kv
         load_ids(p);
         load_keys(0);
     }
-    // the query row, scaled by a power of two, as hi + lo
-    h8 qh[2 * kCols], ql[2 * kCols];
-    float row_factor;
-    {
-        const float* x = a.q + (size_t)(q.r0 + i) * a.q_stride + (size_t)head * c.dim;
-        float v[16 * kCols];
-        uint32_t top = 0;
+    // the query rows as hi + lo
+    StepQ<DP, ROWS>& rows_q = *reinterpret_cast<StepQ<DP, ROWS>*>(part_o);
+    stage_rows<DP, ROWS>(rows_q, c, a, q, h, rt * ROWS);
+    __syncthreads();
+    h8 qh[2 * kCols], ql[PACK ? 1 : 2 * kCols];
 #pragma unroll
-        for (int j = 0; j < kCols; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int d = j * 64 + g * 16 + e;
-                v[j * 16 + e] = live && d < c.dim ? x[d] : 0.0f;
-                top = max(top, abs_bits(v[j * 16 + e]));
-            }
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-        const int e = row_exponent(top);
-        const float down = pow2(-e);
-        row_factor = a.scale * pow2(e);
-#pragma unroll
-        for (int k = 0; k < 2 * kCols; ++k)
-#pragma unroll
-            for (int o = 0; o < 4; ++o) {
-                h2 hi, lo;
-                split_pair(v[k * 8 + 2 * o] * down, v[k * 8 + 2 * o + 1] * down, &hi, &lo);
-                qh[k][2 * o] = hi[0], qh[k][2 * o + 1] = hi[1];
-                ql[k][2 * o] = lo[0], ql[k][2 * o + 1] = lo[1];
-            }
+    for (int k = 0; k < 2 * kCols; ++k) {
+        const int d = (k / 2) * 64 + g * 16 + (k % 2) * 8;
+        qh[k] = *reinterpret_cast<const h8*>(&rows_q.x[col][d]);
+        if constexpr (!PACK) ql[k] = *reinterpret_cast<const h8*>(&rows_q.x[16 + col][d]);
     }
+    const float row_factor = rows_q.factor[col % ROWS];
     while (p < p1) {
         const uint8_t* vp = c.v + ((size_t)page * c.n_kv + h) * kv_stride + col * kPage + 16 * g;
 #pragma unroll
@@ -144,8 +130,10 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void step_kernel(Kv
                 const h8 lo = code_oct<F8>(kf[t][j].x, kf[t][j].y), hi = code_oct<F8>(kf[t][j].z, kf[t][j].w);
                 sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, qh[2 * j], sc[t], 0, 0, 0);
                 sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qh[2 * j + 1], sc[t], 0, 0, 0);
-                sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, ql[2 * j], sc[t], 0, 0, 0);
-                sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ql[2 * j + 1], sc[t], 0, 0, 0);
+                if constexpr (!PACK) {
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, ql[2 * j], sc[t], 0, 0, 0);
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ql[2 * j + 1], sc[t], 0, 0, 0);
+                }
             }
         }
         const int tok0 = p * kPage + 16 * g;
@@ -165,7 +153,9 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void step_kernel(Kv
         float x[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            float v = sc[e / 4][e % 4] * factor;
+            float v = sc[e / 4][e % 4];
+            if (PACK) v += from_other_eight(v);
+            v *= factor;
             if (GEN && a.softcap > 0.0f) v = cap_score(v, a.softcap, inv_cap);
             v *= kLog2e;
             if (GEN && a.slopes) v -= row.slope * fabsf((float)(row.pos - kpos[e]));
@@ -210,15 +200,16 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void step_kernel(Kv
         if (masked)
 #pragma unroll
             for (int e = 0; e < 16; ++e) w[e] = (see >> e) & 1u ? w[e] : 0.0f;
-        h8 wh[2], wl[2];
+        h8 wh[2], wl[PACK ? 1 : 2];
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 h2 hi, lo;
                 split_pair(w[8 * k + 2 * e], w[8 * k + 2 * e + 1], &hi, &lo);
+                if (PACK) hi = col < 8 ? hi : lo;
                 wh[k][2 * e] = hi[0], wh[k][2 * e + 1] = hi[1];
-                wl[k][2 * e] = lo[0], wl[k][2 * e + 1] = lo[1];
+                if (!PACK) wl[k][2 * e] = lo[0], wl[k][2 * e + 1] = lo[1];
             }
         if (F8 && tail) {  // what stands behind the last token may be NaN as a code
             const int left = min(max(q.len - tok0, 0), 16);
@@ -237,8 +228,10 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void step_kernel(Kv
             const h8 lo = code_oct<F8>(vf[k].x, vf[k].y), hi = code_oct<F8>(vf[k].z, vf[k].w);
             o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wh[0], o[k], 0, 0, 0);
             o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wh[1], o[k], 0, 0, 0);
-            o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wl[0], o[k], 0, 0, 0);
-            o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wl[1], o[k], 0, 0, 0);
+            if constexpr (!PACK) {
+                o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wl[0], o[k], 0, 0, 0);
+                o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wl[1], o[k], 0, 0, 0);
+            }
         }
         p = np;
     }
@@ -255,61 +248,70 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void step_kernel(Kv
     // (a wave that has seen nothing has sum 0 and O 0; exp2 of its maximum's distance is 0)
     const float mine = __builtin_amdgcn_exp2f(top - all_top) * (v_exp == -200 ? 0.0f : __builtin_amdgcn_exp2f((float)v_exp));
 #pragma unroll
-    for (int k = 0; k < kOut; ++k) *reinterpret_cast<f4*>(&part_o[wave][col * (DP + 4) + k * 16 + 4 * g]) = o[k] * mine;
+    for (int k = 0; k < kOut; ++k) *reinterpret_cast<f4*>(&part_o[wave * kPart + col * (DP + 4) + k * 16 + 4 * g]) = o[k] * mine;
     __syncthreads();
     const bool whole = parts == 1;
-    float* piece = whole ? nullptr : scratch + (size_t)blockIdx.x * kPieceFloats<DP>;
+    const int rows = min(ROWS, n_rows - rt * ROWS), tid = threadIdx.x;
     const float nan = __builtin_nanf("");
-    for (int at = threadIdx.x; at < kRows * DP; at += 64 * kWaves) {
-        const int r = at / DP, d = at % DP, r_all = rt * kRows + r;
-        if (r_all >= n_rows) continue;
-        float x = 0.0f;
+    const bool vec = c.dim % 4 == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+    auto out_row = [&](int r) {
+        const int r_all = rt * ROWS + r;
+        return (size_t)(q.r0 + r_all / a.group) * a.n_head + h * a.group + r_all % a.group;
+    };
+    auto store_out = [&](int r, int d, f4 x) {
+        float* y = dst + out_row(r) * c.dim + d;
+        if (vec) {
+            if (d < c.dim) *reinterpret_cast<f4*>(y) = x;
+        } else {
 #pragma unroll
-        for (int k = 0; k < kWaves; ++k) x += part_o[k][r * (DP + 4) + d];
+            for (int e = 0; e < 4; ++e)
+                if (d + e < c.dim) y[e] = x[e];
+        }
+    };
+    auto lse_of = [&](float l, float m) {
+        return l == 0.0f ? -__builtin_inff() : (__builtin_amdgcn_logf(l) + m - (float)kBias) * kLn2;
+    };
+    float* piece = whole ? nullptr : scratch + (size_t)blockIdx.x * kPieceFloats<DP, ROWS>;
+    for (int at = tid; at < rows * kFours; at += kThreads) {
+        const int r = at / kFours, d = at % kFours * 4;
+        f4 x = f4{0, 0, 0, 0};
+        float m = kNoMax, l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) {
+            x += *reinterpret_cast<const f4*>(&part_o[k * kPart + r * (DP + 4) + d]);
+            if (PACK) x += *reinterpret_cast<const f4*>(&part_o[k * kPart + (r + 8) * (DP + 4) + d]);
+            m = fmaxf(m, part_m[k][r]);
+        }
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) l += part_l[k][r] * __builtin_amdgcn_exp2f(part_m[k][r] - m);
+        if (any_bad) x = f4{nan, nan, nan, nan}, l = nan;
         if (!whole) {
-            piece[at] = any_bad ? nan : x;
+            *reinterpret_cast<f4*>(piece + r * DP + d) = x;
+            if (d == 0) *reinterpret_cast<float2*>(piece + ROWS * DP + 2 * r) = make_float2(m, l);
             continue;
         }
-        if (d >= c.dim) continue;
-        float m = kNoMax, l = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kWaves; ++k) m = fmaxf(m, part_m[k][r]);
-#pragma unroll
-        for (int k = 0; k < kWaves; ++k) l += part_l[k][r] * __builtin_amdgcn_exp2f(part_m[k][r] - m);
-        dst[((size_t)(q.r0 + r_all / a.group) * a.n_head + h * a.group + r_all % a.group) * c.dim + d] =
-            any_bad ? nan : l == 0.0f ? 0.0f : x / l;
-    }
-    if (threadIdx.x < kRows && rt * kRows + (int)threadIdx.x < n_rows) {
-        const int r = threadIdx.x, r_all = rt * kRows + r;
-        float m = kNoMax, l = 0.0f;
-        for (int k = 0; k < kWaves; ++k) m = fmaxf(m, part_m[k][r]);
-        for (int k = 0; k < kWaves; ++k) l += part_l[k][r] * __builtin_amdgcn_exp2f(part_m[k][r] - m);
-        if (!whole) {
-            piece[kRows * DP + r] = m;
-            piece[kRows * DP + kRows + r] = any_bad ? nan : l;
-        } else if (lse) {
-            lse[(size_t)(q.r0 + r_all / a.group) * a.n_head + h * a.group + r_all % a.group] =
-                any_bad ? nan : l == 0.0f ? -__builtin_inff() : (__builtin_amdgcn_logf(l) + m - (float)kBias) * kLn2;
-        }
+        const float scale = l == 0.0f ? 0.0f : 1.0f / l;
+        store_out(r, d, x * scale);
+        if (lse && d == 0) lse[out_row(r)] = lse_of(l, m);
     }
 }
 
 // Joins the pieces of one query row: blockIdx.x counts (sequence, head, row tile), blockIdx.y the row in the tile.
-template <int DP>
+template <int DP, int ROWS>
 __global__ __launch_bounds__(256) void join_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a, float* __restrict__ dst,
                                                    float* __restrict__ lse, const float* __restrict__ scratch, int target,
                                                    int max_tiles) {
     __shared__ __align__(16) float part[1024 / DP][DP];
     const int lane = threadIdx.x & 63;
     const int rt = blockIdx.x % max_tiles, h = blockIdx.x / max_tiles % c.n_kv, s = blockIdx.x / max_tiles / c.n_kv;
-    const int r = blockIdx.y, r_all = rt * kRows + r;
-    const SeqCut cut = find_cut(b, a, c.n_kv, target, false, s, 0);
+    const int r = blockIdx.y, r_all = rt * ROWS + r;
+    const SeqCut cut = find_cut(b, a, c.n_kv, ROWS, target, false, s, 0);
     const Kv8Seq q = cut.q;
     const int parts = cut.parts;
     if (r_all >= q.n * a.group || parts == 1) return;
-    const float* first = scratch + (size_t)(cut.first + (h * cut.work.tiles + rt) * parts) * kPieceFloats<DP>;
-    auto max_of = [&](int k) { return first[(size_t)k * kPieceFloats<DP> + kRows * DP + r]; };
-    auto sum_of = [&](int k) { return first[(size_t)k * kPieceFloats<DP> + kRows * DP + kRows + r]; };
+    const float* first = scratch + (size_t)(cut.first + (h * cut.work.tiles + rt) * parts) * kPieceFloats<DP, ROWS>;
+    auto max_of = [&](int k) { return first[(size_t)k * kPieceFloats<DP, ROWS> + ROWS * DP + 2 * r]; };
+    auto sum_of = [&](int k) { return first[(size_t)k * kPieceFloats<DP, ROWS> + ROWS * DP + 2 * r + 1]; };
     float m = kNoMax;
     for (int k = lane; k < parts; k += 64) m = fmaxf(m, max_of(k));
     for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
@@ -326,7 +328,7 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8Cache c, Kv8Batch b, Kv8At
     if (group < kGroups) {
 #pragma unroll 4
         for (int k = group; k < parts; k += kGroups)
-            x += *reinterpret_cast<const f4*>(first + (size_t)k * kPieceFloats<DP> + r * DP + 4 * d4) * __builtin_amdgcn_exp2f(max_of(k) - m);
+            x += *reinterpret_cast<const f4*>(first + (size_t)k * kPieceFloats<DP, ROWS> + r * DP + 4 * d4) * __builtin_amdgcn_exp2f(max_of(k) - m);
         *reinterpret_cast<f4*>(&part[group][4 * d4]) = x;
     }
     __syncthreads();
@@ -338,35 +340,48 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8Cache c, Kv8Batch b, Kv8At
     dst[out * c.dim + d] = l == 0.0f ? 0.0f : y / l;
 }
 
-int max_tiles_of(int group, int max_q) { return (int)(((int64_t)max_q * group + kRows - 1) / kRows); }
+int max_tiles_of(int group, int max_q) {
+    const int rows = step_rows(group, max_q);
+    return (int)(((int64_t)max_q * group + rows - 1) / rows);
+}
 
+template <int DP, int ROWS>
+void launch_step_rows(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch, int cus,
+                      hipStream_t stream) {
+    const int tiles = max_tiles_of(a.group, b.max_q), target = step_target(cus, (int64_t)b.n_seq * c.n_kv * tiles);
+    const bool gen = a.softcap > 0.0f || a.window > 0 || a.slopes || a.first || a.prefix;
+    const unsigned items = (unsigned)step_items(cus, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);
+    auto kernel = c.f8 ? (gen ? step_kernel<DP, ROWS, true, true> : step_kernel<DP, ROWS, true, false>)
+                       : (gen ? step_kernel<DP, ROWS, false, true> : step_kernel<DP, ROWS, false, false>);
+    hipLaunchKernelGGL(kernel, dim3(items), dim3(64 * kWaves), 0, stream, c, b, a, dst, lse, scratch, target);
+    if (b.max_pages <= kWholePages) return;  // no sequence has two pieces
+    hipLaunchKernelGGL((join_kernel<DP, ROWS>), dim3((unsigned)(b.n_seq * c.n_kv * tiles), (unsigned)std::min(ROWS, b.max_q * a.group)),
+                       dim3(256), 0, stream, c, b, a, dst, lse, scratch, target, tiles);
+}
 template <int DP>
 void launch_step_dp(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch, int cus,
                     hipStream_t stream) {
-    const int target = step_target(cus), tiles = max_tiles_of(a.group, b.max_q);
-    const bool gen = a.softcap > 0.0f || a.window > 0 || a.slopes || a.first || a.prefix;
-    const unsigned items = (unsigned)step_items(cus, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);
-    auto kernel = c.f8 ? (gen ? step_kernel<DP, true, true> : step_kernel<DP, true, false>)
-                       : (gen ? step_kernel<DP, false, true> : step_kernel<DP, false, false>);
-    hipLaunchKernelGGL(kernel, dim3(items), dim3(64 * kWaves), 0, stream, c, b, a, dst, lse, scratch, target);
-    if (b.max_pages <= kWaves) return;  // no sequence has two pieces
-    hipLaunchKernelGGL(join_kernel<DP>, dim3((unsigned)(b.n_seq * c.n_kv * tiles), (unsigned)std::min(kRows, b.max_q * a.group)),
-                       dim3(256), 0, stream, c, b, a, dst, lse, scratch, target, tiles);
+    if (step_rows(a.group, b.max_q) == 8) launch_step_rows<DP, 8>(c, b, a, dst, lse, scratch, cus, stream);
+    else launch_step_rows<DP, 16>(c, b, a, dst, lse, scratch, cus, stream);
 }
 
 }  // namespace
 
-// Pieces aimed at: two workgroups for each compute unit.
-int step_target(int cus) { static const int f = getenv("KV8_T") ? atoi(getenv("KV8_T")) : 2; return f * cus; }
+// Query rows of a workgroup: 8 where no sequence has more.
+int step_rows(int group, int max_q) { return (int64_t)max_q * group <= 8 ? 8 : kStepRows; }
+// Pieces aimed at: two for each compute unit, which is what runs at a time (two sequences of 115000 tokens: 46 us, with
+// three 50); three where the batch has more (sequence, head, row tile)s than compute units, whose pieces differ in size
+// (64 sequences of 500 to 8000 tokens, 8 heads: 72 us, with two 74).
+int step_target(int cus, int64_t tiles) { return (tiles > cus ? 3 : 2) * cus; }
 // Upper bound of the pieces: the total is cut into `target`, and each (sequence, head, row tile) rounds up once.
 size_t step_items(int cus, int n_kv, int group, int n_seq, int max_q, int max_pages) {
     const size_t tiles = (size_t)n_seq * n_kv * max_tiles_of(group, max_q);
-    return std::min((size_t)step_target(cus) + tiles, tiles * (size_t)((max_pages + kWaves - 1) / kWaves));
+    return std::min((size_t)step_target(cus, (int64_t)tiles) + tiles, tiles * (size_t)((max_pages + kWaves - 1) / kWaves));
 }
 size_t step_scratch(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages) {
-    if (max_pages <= kWaves) return 0;
+    if (max_pages <= kWholePages) return 0;
     const size_t dp = (size_t)(dim + 63) / 64 * 64;
-    return step_items(cus, n_kv, group, n_seq, max_q, max_pages) * (kRows * dp + 2 * kRows) * sizeof(float);
+    return step_items(cus, n_kv, group, n_seq, max_q, max_pages) * (kStepRows * dp + 2 * kStepRows) * sizeof(float);
 }
 void launch_attention_step(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch,
                            int cus, hipStream_t stream) {
