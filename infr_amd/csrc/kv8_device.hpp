@@ -33,6 +33,11 @@ __device__ __forceinline__ uint4 load_stream(const uint8_t* p) {
     return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
+// Exponents are formed as fma(product, factor, -maximum), with the maximum rounded and the product not: they miss by
+// half an ulp of the score, the same for all of a row. Above this size, where that could be more than 2^-8, the scores
+// are rounded first.
+constexpr float kLargeScore = 65536.0f;
+
 // Two codes (bytes 2 * word, 2 * word + 1 of c) as f16.
 template <bool F8>
 __device__ __forceinline__ h2 code_pair(uint32_t c, int word) {
@@ -117,7 +122,7 @@ __device__ __forceinline__ bool rows_vec(const Kv8Cache& c, const Kv8Attn& a) {
     return c.dim % 4 == 0 && a.q_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0;
 }
 
-// c * tanh(s / c), to the last bits of s: an odd polynomial (the series of tanh) where tanh is nearly its
+// c * tanh(s / c), to the last bits of s (with s and c both times log2 e it is the capped score times that): an odd polynomial (the series of tanh) where tanh is nearly its
 // argument, 1 - 2 / (e^2y + 1) beyond, where the difference cancels no more than two bits.
 __device__ __forceinline__ float cap_score(float s, float c, float inv_c) {
     const float y = s * inv_c, z = y * y;
@@ -132,6 +137,17 @@ __device__ __forceinline__ float cap_score(float s, float c, float inv_c) {
     const float e = __builtin_amdgcn_exp2f(a * (2.0f * kLog2e));
     const float far = __builtin_copysignf(c * (1.0f - 2.0f / (e + 1.0f)), s);
     return a < 0.35f ? near : a >= 0.35f ? far : s;  // NaN stays
+}
+
+// A block's value scale as the weights' exponent: log2 of scale / 2^v_exp. Blocks 2^60 below the largest scale count as
+// if they were that near: nothing of them reaches the result, and the weights keep clear of the smallest numbers.
+__device__ __forceinline__ float scale_log(float scale, int v_exp) {
+    const float l = __builtin_amdgcn_logf(scale * __builtin_amdgcn_exp2f(-(float)max(v_exp, -126)));
+    return l >= -60.0f ? l : l < -60.0f ? -60.0f : 0.0f;  // a NaN scale is the caller's
+}
+// The scale's exponent; -200 for a NaN scale and for blocks no token of which is seen.
+__device__ __forceinline__ int scale_exponent(float scale, bool any) {
+    return any && scale < __builtin_inff() ? (int)((__builtin_bit_cast(uint32_t, scale) >> 23) & 255u) - 127 : -200;
 }
 
 // What one query row sees, and its bias.
@@ -184,7 +200,8 @@ __device__ __forceinline__ float from_other_eight(float x) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xF, 0xF, true));
 }
 
-// The query rows of a workgroup in LDS as f16, scaled by their powers of two: low parts behind the high ones (with
+// The query rows of a workgroup in LDS as f16, scaled by their powers of two (factor: what a product of codes is to be
+// multiplied by, times log2 e): low parts behind the high ones (with
 // ROWS = 8 the two are the 16 columns of one MFMA). Rows are padded by 16 bytes.
 template <int DP, int ROWS>
 struct StepQ {
@@ -212,7 +229,7 @@ __device__ __forceinline__ void stage_rows(StepQ<DP, ROWS>& st, const Kv8Cache& 
 #pragma unroll
     for (int o = 1; o < kSide; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
     const int e2 = row_exponent(top);
-    const float down = pow2(-e2);
+    const float down = a.scale < 0.0f ? -pow2(-e2) : pow2(-e2);  // factors stay positive: a maximum may be taken before them
 #pragma unroll
     for (int k = 0; k < kFours; ++k) {
         const int d = (k * kSide + t) * 4;
@@ -224,7 +241,7 @@ __device__ __forceinline__ void stage_rows(StepQ<DP, ROWS>& st, const Kv8Cache& 
             *reinterpret_cast<h4*>(&st.x[ROWS + r][d]) = h4{l0[0], l0[1], l1[0], l1[1]};
         }
     }
-    if (t == 0) st.factor[r] = a.scale * pow2(e2);
+    if (t == 0) st.factor[r] = fabsf(a.scale) * kLog2e * pow2(e2);
 }
 
 // A sequence's share of the pieces: `parts` of each (head, row tile), the first of them number `first`.

@@ -32,6 +32,7 @@ struct Stage {
     _Float16 v[DP][kPage + 8];
     float ks[4], vs[4];    // scales of the four runs of 16 tokens
     int32_t pos[kPage];
+    float rel[kPage];      // positions from the workgroup's first row's on: exact as far as 2^24
 };
 
 template <int DP, bool F8, bool GEN>
@@ -65,12 +66,15 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
         if (a.first) lo = row.pos >= row.first ? max(lo, slot - (row.pos - row.first)) : 0x7FFFFFFF;
         hi = a.causal ? max(slot + 1, min(a.prefix ? row.prefix : 0, q.len)) : q.len;
     }
+    int last_pos = live ? row.pos : -0x7FFFFFFF - 1, last_first = live ? row.first : -0x7FFFFFFF - 1;
     int full_hi = live ? (a.causal ? q.len - q.n + i + 1 : q.len) : 0x7FFFFFFF;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         lo = min(lo, __shfl_xor(lo, o));
         hi = max(hi, __shfl_xor(hi, o));
         full_hi = min(full_hi, __shfl_xor(full_hi, o));
+        last_pos = max(last_pos, __shfl_xor(last_pos, o));
+        last_first = max(last_first, __shfl_xor(last_first, o));
     }
     // this wave's pages; none when lo >= hi
     const int w0 = lo < hi ? lo / kPage : 0x7FFFFFFF, w1 = lo < hi ? (hi + kPage - 1) / kPage : 0;
@@ -107,8 +111,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
         }
         top = max(top, (uint32_t)__shfl_xor((int)top, 32));
         const int e2 = row_exponent(top);
-        const float down = pow2(-e2);
-        row_factor = a.scale * pow2(e2);
+        const float down = a.scale < 0.0f ? -pow2(-e2) : pow2(-e2);  // factors stay positive: a maximum may be taken before them
+        row_factor = fabsf(a.scale) * kLog2e * pow2(e2);
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
 #pragma unroll
@@ -120,15 +124,18 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
             }
         }
     }
-    const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+    const float cap = a.softcap * kLog2e, inv_cap = GEN && cap > 0.0f ? 1.0f / cap : 0.0f;
     const bool use_pos = GEN && (a.window > 0 || a.slopes || a.first || a.prefix);
+
+    const int ref = use_pos ? b.pos[min(q.r0 + rt * kRows / a.group, b.rows - 1)] : 0;
+    const float my_rel = (float)(row.pos - ref);
 
     f16x o[kOut];
 #pragma unroll
     for (int k = 0; k < kOut; ++k) o[k] = (f16x)(0.0f);
     float top = kNoMax, sum = 0.0f;
     int v_exp = -200;
-    bool bad = !q.ok;
+    bool bad = !q.ok, v_bad = false;  // v_bad: the row sees a token whose value is NaN
 
     const int32_t* table = b.pages + (size_t)s * b.max_pages;
     const int subs = kPage / c.block;
@@ -176,7 +183,10 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
         }
         if (tid < 4) st.ks[tid] = sr;
         else if (tid < 8) st.vs[tid - 4] = sr;
-        if (use_pos && tid < kPage) st.pos[tid] = pr;
+        if (use_pos && tid < kPage) {
+            st.pos[tid] = pr;
+            st.rel[tid] = (float)(pr - ref);
+        }
     };
 
     if (p0 < p1) {
@@ -202,45 +212,63 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
                     x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, ql[k], x[t], 0, 0, 0);
                 }
             }
-            const bool masked = use_pos || (p + 1) * kPage > min(full_hi, q.len);
-            uint32_t see = 0xFFFFFFFFu;
-            if (masked) see = 0;
-            float high = -__builtin_inff();
+            // (positions ascend: what the last row's window and document allow at the page's first token, all rows allow)
+            const bool masked = (p + 1) * kPage > min(full_hi, q.len) ||
+                                (use_pos && (last_pos - st.pos[0] >= row.window || last_first > st.pos[0]));
+            const bool bent = GEN && (a.softcap > 0.0f || a.slopes);
+            float high = -__builtin_inff(), factor[2], vs[2];
+            bool any[2] = {true, true};
             int e_now = -200;
-            float vs[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const float factor = row_factor * st.ks[2 * t + hf];
+                factor[t] = row_factor * st.ks[2 * t + hf];
                 vs[t] = st.vs[2 * t + hf];
-                const int tok0 = p * kPage + t * 32 + hf * 16;
-                int kpos[16];
-                if (use_pos)
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        const int4 y = *reinterpret_cast<const int4*>(&st.pos[t * 32 + hf * 16 + e]);
-                        kpos[e] = y.x, kpos[e + 1] = y.y, kpos[e + 2] = y.z, kpos[e + 3] = y.w;
-                    }
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float v = x[t][e] * factor;
-                    if (GEN && a.softcap > 0.0f) v = cap_score(v, a.softcap, inv_cap);
-                    v *= kLog2e;
-                    if (GEN && a.slopes) v -= row.slope * fabsf((float)(row.pos - kpos[e]));
-                    x[t][e] = v;
-                }
-                if (masked)
+                if (masked || bent) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const int tok = tok0 + e;
-                        const bool yes = tok < q.len && (use_pos ? row.sees(tok, kpos[e]) : tok <= row.slot);
-                        see |= (yes ? 1u : 0u) << (16 * t + e);
-                        x[t][e] = yes ? x[t][e] : -__builtin_inff();
+                        float v = x[t][e] * factor[t];
+                        if (GEN && a.softcap > 0.0f) v = cap_score(v, cap, inv_cap);
+                        x[t][e] = v;
                     }
+                    factor[t] = 1.0f;
+                }
+                if (GEN && a.slopes)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) high = fmaxf(high, x[t][e]);
-                if (vs[t] < __builtin_inff() && (see >> (16 * t)) & 0xFFFFu)
-                    e_now = max(e_now, (int)((__builtin_bit_cast(uint32_t, vs[t]) >> 23) & 255u) - 127);
+                    for (int e = 0; e < 16; e += 4) {
+                        const f4 y = *reinterpret_cast<const f4*>(&st.rel[t * 32 + hf * 16 + e]);
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) x[t][e + n] = __builtin_fmaf(-row.slope, fabsf(my_rel - y[n]), x[t][e + n]);
+                    }
+                if (masked) {
+                    const int tok0 = p * kPage + t * 32 + hf * 16;
+                    any[t] = false;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        int4 y = make_int4(0, 0, 0, 0);
+                        if (use_pos) y = *reinterpret_cast<const int4*>(&st.pos[t * 32 + hf * 16 + e]);
+                        const int kpos[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            const int tok = tok0 + e + n;
+                            const bool yes = tok < q.len && (use_pos ? row.sees(tok, kpos[n]) : tok <= row.slot);
+                            any[t] = any[t] || yes;
+                            x[t][e + n] = yes ? x[t][e + n] : -__builtin_inff();
+                        }
+                    }
+                }
+                float most = x[t][0];
+#pragma unroll
+                for (int e = 1; e < 16; ++e) most = fmaxf(most, x[t][e]);
+                high = fmaxf(high, most * factor[t]);
+                e_now = max(e_now, scale_exponent(vs[t], any[t]));
             }
+            if (__any(fabsf(high) > kLargeScore))
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[t][e] *= factor[t];
+                    factor[t] = 1.0f;
+                }
             if (__any(high > top + kLag || e_now > v_exp)) {
                 const float new_top = fmaxf(top, halves_max(high));
                 const int new_exp = max(v_exp, (int)halves_max((float)e_now));
@@ -252,21 +280,19 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
                 top = new_top;
                 v_exp = new_exp;
             }
-            const float unit = __builtin_amdgcn_exp2f(-(float)max(v_exp, -126)), base = (float)kBias - top;
+            // weights times the values' scale in one exponential; their sum is divided by it
             h8 wh[4], wl[4];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const float ratio = vs[t] * unit;
-                float w[16];
+                v_bad = v_bad || (any[t] && vs[t] != vs[t]);
+                const float lift = any[t] ? scale_log(vs[t], v_exp) : 0.0f, base = (float)kBias - top + lift;
+                float run = 0.0f, w[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const float pe = __builtin_amdgcn_exp2f(x[t][e] + base);
-                    sum += pe;
-                    w[e] = pe * ratio;
+                    w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][e], factor[t], base));
+                    run += w[e];
                 }
-                if (masked)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) w[e] = (see >> (16 * t + e)) & 1u ? w[e] : 0.0f;
+                sum = __builtin_fmaf(run, __builtin_amdgcn_exp2f(-lift), sum);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     h2 u, v;
@@ -289,8 +315,11 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
     }
     bad = __syncthreads_or(bad) != 0;
     sum = halves_sum(sum);
+    if (halves_max(v_bad ? 1.0f : 0.0f) > 0.0f)
+#pragma unroll
+        for (int k = 0; k < kOut; ++k) o[k] = (f16x)(__builtin_nanf(""));
     if (!live) return;
-    const float nan = __builtin_nanf(""), up = v_exp == -200 ? 0.0f : __builtin_amdgcn_exp2f((float)v_exp);
+    const float nan = __builtin_nanf(""), up = __builtin_amdgcn_exp2f((float)max(v_exp, -126));
     if (parts > 1) {
         float* piece = scratch + ((((size_t)s * c.n_kv + h) * tiles + rt) * parts + part) * kPieceFloats<DP>;
         const int r = wave * kCols + col;

@@ -48,14 +48,14 @@ __global__ __launch_bounds__(64 * kStepWaves, DP <= 128 ? 2 : 1) void score_step
     const bool live = col < q.n * a.group;
     const int i = live ? col / a.group : max(q.n - 1, 0), head = h * a.group + (live ? col % a.group : 0);
 
-    const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+    const float cap = a.softcap * kLog2e, inv_cap = GEN && cap > 0.0f ? 1.0f / cap : 0.0f;
     const bool use_pos = GEN && (a.window > 0 || a.slopes || a.first || a.prefix);
     const int all_see = a.causal ? q.len - q.n + 1 : q.len;
     const int32_t* table = b.pages + (size_t)s * b.max_pages;
     const int subs = kPage / c.block;
     uint4 kf[4][kCols];
     float ks = 0.0f;
-    int page = 0, ids = 0;
+    int page = 0, ids = 0, pos0 = 0;
     auto load_ids = [&](int p) {
         const int at = p + lane * kStepWaves;
         ids = at < p1 ? table[at] : 0;
@@ -70,6 +70,7 @@ __global__ __launch_bounds__(64 * kStepWaves, DP <= 128 ? 2 : 1) void score_step
 #pragma unroll
             for (int j = 0; j < kCols; ++j) kf[t][j] = load_stream(kp + j * kPage * 64 + t * 4 * 64);
         ks = c.ks[at * subs + g * 16 / c.block];
+        if (use_pos) pos0 = c.pos[at * kPage];
     };
     int p = p0 + wave, n = 0;
     if (p < p1) {
@@ -88,16 +89,26 @@ __global__ __launch_bounds__(64 * kStepWaves, DP <= 128 ? 2 : 1) void score_step
     }
     const float row_factor = rows_q.factor[col];
     Kv8Row row{};
+    row.window = a.window > 0 ? a.window : 0x7FFFFFFF;
     float row_lse = 0.0f;
     if (live) {
         row = kv8_row(b, a, q, s, i, head);
         row_lse = lse[(size_t)(q.r0 + i) * a.n_head + head] * kLog2e;
     }
+    int last_pos = live ? row.pos : -0x7FFFFFFF - 1, last_first = live ? row.first : -0x7FFFFFFF - 1;
+    if (use_pos)
+#pragma unroll
+        for (int k = 1; k < 16; k <<= 1) {
+            last_pos = max(last_pos, __shfl_xor(last_pos, k));
+            last_first = max(last_first, __shfl_xor(last_first, k));
+        }
     while (p < p1) {
         const int now = page;
         const size_t at = ((size_t)max(now, 0) * c.n_kv + h) * kPage + 16 * g;
+        // (positions ascend: what the last row's window and document allow at the page's first token, all rows do)
+        const bool masked = (p + 1) * kPage > min(all_see, q.len) || (use_pos && (last_pos - pos0 >= row.window || last_first > pos0));
         int kpos[16];
-        if (use_pos) {
+        if (use_pos && (masked || a.slopes)) {
             const int4* pp = reinterpret_cast<const int4*>(c.pos + at);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -129,21 +140,24 @@ __global__ __launch_bounds__(64 * kStepWaves, DP <= 128 ? 2 : 1) void score_step
             }
             load_keys(n);
         }
-        const bool masked = use_pos || (p + 1) * kPage > min(all_see, q.len);
         float w[16];
+        const bool bent = GEN && (a.softcap > 0.0f || a.slopes);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            float v = sc[e / 4][e % 4] * factor;
-            if (GEN && a.softcap > 0.0f) v = cap_score(v, a.softcap, inv_cap);
-            v *= kLog2e;
-            if (GEN && a.slopes) v -= row.slope * fabsf((float)(row.pos - kpos[e]));
-            w[e] = live ? __builtin_amdgcn_exp2f(v - row_lse) : 0.0f;
+            float v = sc[e / 4][e % 4];
+            if (bent) {
+                v *= factor;
+                if (a.softcap > 0.0f) v = cap_score(v, cap, inv_cap);
+                if (a.slopes) v = __builtin_fmaf(-row.slope, fabsf((float)(row.pos - kpos[e])), v);
+            }
+            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(v, bent ? 1.0f : factor, -row_lse));
+            w[e] = live ? y : 0.0f;
         }
         if (masked)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int tok = tok0 + e;
-                w[e] = tok < q.len && (use_pos ? row.sees(tok, kpos[e]) : tok <= row.slot) && live ? w[e] : 0.0f;
+                w[e] = tok < q.len && (use_pos ? row.sees(tok, kpos[e]) : tok <= row.slot) ? w[e] : 0.0f;
             }
         fold<kMirror, 16>(w, col & 8);
         fold<kHalfMirror, 8>(w, col & 4);
@@ -164,6 +178,7 @@ struct Rows {
     _Float16 hi[kTile][DP + 8], lo[kTile][DP + 8];
     float factor[kTile], lse[kTile], slope[kTile];
     int slot[kTile], pos[kTile], first[kTile];
+    int last_first[kWaves];  // largest first[] of the rows each wave brought in
 };
 
 template <int DP, bool F8, bool GEN>
@@ -202,6 +217,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void score_prompt_kern
 #pragma unroll
             for (int e = 0; e < 16; ++e) kpos[t][e] = c.pos[at * kPage + 32 * t + 16 * hf + e];
     }
+    const int pos0 = use_pos ? c.pos[at * kPage] : 0;
     // rows that see any token of the workgroup's pages: by causality none before the first token's own, by the window
     // none from `window` behind the last one on (positions ascend strictly)
     const int t_first = group0 * kPage, t_last = min((group0 + kWaves) * kPage, q.len) - 1, begin = q.len - q.n;
@@ -212,7 +228,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void score_prompt_kern
     const int per = (r_hi - r_lo + parts - 1) / parts;
     const int r0 = min(r_lo + part * per, r_hi), r1 = min(r0 + per, r_hi);
 
-    const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+    const float cap = a.softcap * kLog2e, inv_cap = GEN && cap > 0.0f ? 1.0f / cap : 0.0f;
     const int prefix = a.prefix ? a.prefix[s] : -0x7FFFFFFF - 1, window = a.window > 0 ? a.window : 0x7FFFFFFF;
     float v[kEach];
     Kv8Row in{};
@@ -226,10 +242,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void score_prompt_kern
         const int i = in_live ? rr / a.group : q.n - 1, head = h * a.group + (in_live ? rr % a.group : 0);
         const float* x = a.q + (size_t)(q.r0 + i) * a.q_stride + (size_t)head * c.dim;
         load_row<kEach>(x, my_col, c.dim, in_live, vec, v);
-        if ((tid & 7) == 0) {
-            in = kv8_row(b, a, q, s, i, head);
-            in_lse = lse[(size_t)(q.r0 + i) * a.n_head + head] * kLog2e;
-        }
+        in = kv8_row(b, a, q, s, i, head);
+        in_lse = lse[(size_t)(q.r0 + i) * a.n_head + head] * kLog2e;
     };
     auto store = [&](Rows<DP>& r) {
         uint32_t top = 0;
@@ -238,7 +252,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void score_prompt_kern
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
         const int ex = row_exponent(top);
-        const float down = pow2(-ex);
+        const float down = a.scale < 0.0f ? -pow2(-ex) : pow2(-ex);
 #pragma unroll
         for (int e = 0; e < kEach; e += 8) {
             h8 u, w;
@@ -253,12 +267,18 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void score_prompt_kern
             *reinterpret_cast<h8*>(&r.lo[my_row][my_col + e]) = w;
         }
         if ((tid & 7) == 0) {
-            r.factor[my_row] = a.scale * pow2(ex);
+            r.factor[my_row] = fabsf(a.scale) * kLog2e * pow2(ex);
             r.lse[my_row] = in_lse;
             r.slope[my_row] = in.slope;
             r.slot[my_row] = in_live ? in.slot : -1;
             r.pos[my_row] = in.pos;
             r.first[my_row] = in_live ? in.first : 0x7FFFFFFF;
+        }
+        if (use_pos) {
+            int most = in_live ? in.first : -0x7FFFFFFF - 1;
+#pragma unroll
+            for (int o = 8; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
+            if (lane == 0) r.last_first[wave] = most;
         }
     };
     float acc[32];
@@ -292,23 +312,30 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void score_prompt_kern
             // tokens below this one are seen by all 32 rows (rows ascend, and so do their own tokens)
             const bool full = (rt + 1) * kTile <= q.n * a.group;
             const int all_see = a.causal ? begin + rt * kTile / a.group + 1 : q.len;
-            const bool masked = use_pos || !full || (p + 1) * kPage > min(all_see, q.len);
+            bool masked = !full || (p + 1) * kPage > min(all_see, q.len);
+            if (use_pos) {
+                const int last_first = max(max(r.last_first[0], r.last_first[1]), max(r.last_first[2], r.last_first[3]));
+                masked = masked || r.pos[kTile - 1] - pos0 >= window || last_first > pos0;
+            }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const float factor = r.factor[col] * ks[t];
-                const int tok0 = p * kPage + 32 * t + 16 * hf;
+                float factor = r.factor[col] * ks[t];
+                if (GEN && (a.softcap > 0.0f || a.slopes)) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float y = x[t][e] * factor;
-                    if (GEN && a.softcap > 0.0f) y = cap_score(y, a.softcap, inv_cap);
-                    y *= kLog2e;
-                    if (GEN && a.slopes) y -= row.slope * fabsf((float)(row.pos - kpos[t][e]));
-                    x[t][e] = __builtin_amdgcn_exp2f(y - row_lse);
+                    for (int e = 0; e < 16; ++e) {
+                        float y = x[t][e] * factor;
+                        if (a.softcap > 0.0f) y = cap_score(y, cap, inv_cap);
+                        if (a.slopes) y = __builtin_fmaf(-row.slope, fabsf((float)(row.pos - kpos[t][e])), y);
+                        x[t][e] = y;
+                    }
+                    factor = 1.0f;
                 }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][e], factor, -row_lse));
                 if (masked)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const int tok = tok0 + e;
+                        const int tok = p * kPage + 32 * t + 16 * hf + e;
                         const bool yes = tok < q.len && row.first != 0x7FFFFFFF && (use_pos ? row.sees(tok, kpos[t][e]) : tok <= row.slot);
                         x[t][e] = yes ? x[t][e] : 0.0f;
                     }

@@ -54,24 +54,32 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
     const int i = live ? rr / a.group : q.n - 1, head = h * a.group + (live ? rr % a.group : 0);
 
     const Kv8Row row = kv8_row(b, a, q, s, i, head);
-    const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+    const float cap = a.softcap * kLog2e, inv_cap = GEN && cap > 0.0f ? 1.0f / cap : 0.0f;
     const bool use_pos = GEN && (a.window > 0 || a.slopes || a.first || a.prefix);
     // tokens below this one are seen by every row of the tile (without masks by position)
     const int all_see = a.causal ? q.len - q.n + rt * ROWS / a.group + 1 : q.len;
+
+    int last_pos = live ? row.pos : -0x7FFFFFFF - 1, last_first = live ? row.first : -0x7FFFFFFF - 1;
+    if (use_pos)
+#pragma unroll
+        for (int k = 1; k < 16; k <<= 1) {
+            last_pos = max(last_pos, __shfl_xor(last_pos, k));
+            last_first = max(last_first, __shfl_xor(last_first, k));
+        }
 
     f4 o[kOut];
 #pragma unroll
     for (int k = 0; k < kOut; ++k) o[k] = f4{0, 0, 0, 0};
     float top = kNoMax, sum = 0.0f;
     int v_exp = -200;       // values are scaled by 2^-v_exp
-    bool bad = !q.ok;
+    bool bad = !q.ok, v_bad = false;  // v_bad: the row sees a token whose value is NaN
 
     const int32_t* table = b.pages + (size_t)s * b.max_pages;
     const int subs = kPage / c.block;
     const uint32_t kv_stride = (uint32_t)DP * kPage;
     uint4 kf[4][kCols], vf[kOut];
     float ks = 0.0f, vs = 0.0f;
-    int page = 0, ids = 0;
+    int page = 0, ids = 0, pos0 = 0;
     // lane n holds the wave's n-th next page
     auto load_ids = [&](int p) {
         const int at = p + lane * kWaves;
@@ -89,6 +97,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
         const size_t sc = ((size_t)page * c.n_kv + h) * subs + g * 16 / c.block;
         ks = c.ks[sc];
         vs = c.vs[sc];
+        if (use_pos) pos0 = c.pos[((size_t)page * c.n_kv + h) * kPage];
     };
     int p = p0 + wave, n = 0;
     if (p < p1) {
@@ -111,8 +120,10 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
         const uint8_t* vp = c.v + ((size_t)page * c.n_kv + h) * kv_stride + col * kPage + 16 * g;
 #pragma unroll
         for (int k = 0; k < kOut; ++k) vf[k] = load_stream(vp + k * 16 * kPage);
+        // (positions ascend: what the tile's last row's window and document allow at the page's first token, all rows do)
+        const bool masked = (p + 1) * kPage > min(all_see, q.len) || (use_pos && (last_pos - pos0 >= row.window || last_first > pos0));
         int kpos[16];
-        if (use_pos) {
+        if (use_pos && (masked || a.slopes)) {
             const int4* pp = reinterpret_cast<const int4*>(c.pos + ((size_t)page * c.n_kv + h) * kPage + 16 * g);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -149,34 +160,44 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
             }
             load_keys(n);
         }
-        const bool masked = use_pos || (p + 1) * kPage > all_see || tail;
-        float x[16];
+        float x[16], f = factor;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             float v = sc[e / 4][e % 4];
             if (PACK) v += from_other_eight(v);
-            v *= factor;
-            if (GEN && a.softcap > 0.0f) v = cap_score(v, a.softcap, inv_cap);
-            v *= kLog2e;
-            if (GEN && a.slopes) v -= row.slope * fabsf((float)(row.pos - kpos[e]));
             x[e] = v;
         }
-        uint32_t see = 0xFFFFu;
+        if (masked || (GEN && (a.softcap > 0.0f || a.slopes))) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                float v = x[e] * factor;
+                if (GEN && a.softcap > 0.0f) v = cap_score(v, cap, inv_cap);
+                if (GEN && a.slopes) v = __builtin_fmaf(-row.slope, fabsf((float)(row.pos - kpos[e])), v);
+                x[e] = v;
+            }
+            f = 1.0f;
+        }
+        bool any = true;
         if (masked) {
-            see = 0;
+            any = false;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int tok = tok0 + e;
                 const bool yes = tok < q.len && (use_pos ? row.sees(tok, kpos[e]) : tok <= row.slot);
-                see |= (yes ? 1u : 0u) << e;
+                any = any || yes;
                 x[e] = yes ? x[e] : -__builtin_inff();
             }
         }
         float high = x[0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) high = fmaxf(high, x[e]);
-        // the scale of this lane's values, as a power of two times 1 .. 2
-        const int e_now = (vs_now < __builtin_inff() && see) ? (int)((__builtin_bit_cast(uint32_t, vs_now) >> 23) & 255u) - 127 : -200;
+        high *= f;
+        if (__any(fabsf(high) > kLargeScore)) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] *= f;
+            f = 1.0f;
+        }
+        const int e_now = scale_exponent(vs_now, any);
         if (__any(high > top + kLag || e_now > v_exp)) {
             const float new_top = fmaxf(top, quads_max(high));
             const int new_exp = max(v_exp, (int)quads_max((float)e_now));
@@ -188,18 +209,16 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
             top = new_top;
             v_exp = new_exp;
         }
-        const float ratio = vs_now * __builtin_amdgcn_exp2f(-(float)max(v_exp, -126));
-        const float base = (float)kBias - top;
-        float w[16];
+        // weights times the values' scale in one exponential; their sum is divided by it
+        v_bad = v_bad || (any && vs_now != vs_now);
+        const float lift = any ? scale_log(vs_now, v_exp) : 0.0f, base = (float)kBias - top + lift;
+        float w[16], run = 0.0f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const float pe = __builtin_amdgcn_exp2f(x[e] + base);
-            sum += pe;
-            w[e] = pe * ratio;
+            w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], f, base));
+            run += w[e];
         }
-        if (masked)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) w[e] = (see >> e) & 1u ? w[e] : 0.0f;
+        sum = __builtin_fmaf(run, __builtin_amdgcn_exp2f(-lift), sum);
         h8 wh[2], wl[PACK ? 1 : 2];
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -237,6 +256,9 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
     }
     // the waves' results as one: largest maximum, everything scaled to it
     sum = quads_sum(sum);
+    if (quads_max(v_bad ? 1.0f : 0.0f) > 0.0f)
+#pragma unroll
+        for (int k = 0; k < kOut; ++k) o[k] = (f4)(__builtin_nanf(""));
     if (g == 0) {
         part_m[wave][col] = top;
         part_l[wave][col] = sum;
