@@ -25,29 +25,30 @@ constexpr float kLag = 4.0f;
 template <int DP>
 constexpr int kPieceFloats = kRows * DP + 2 * kRows;
 
-// A page in LDS. Rows are padded by 16 bytes: neighbours then start four banks apart.
-template <int DP>
+// A page's first DC columns in LDS. Rows are padded by 16 bytes: neighbours then start four banks apart.
+template <int DC>
 struct Stage {
-    _Float16 k[kPage][DP + 8];
-    _Float16 v[DP][kPage + 8];
+    _Float16 k[kPage][DC + 8];
+    _Float16 v[DC][kPage + 8];
     float ks[4], vs[4];    // scales of the four runs of 16 tokens
     int32_t pos[kPage];
     float rel[kPage];      // positions from the workgroup's first row's on: exact as far as 2^24
 };
 
-template <int DP, bool F8, bool GEN>
+// DC: the columns that are computed with, head_dim rounded up to 32.
+template <int DP, int DC, bool F8, bool GEN>
 __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a,
                                                                             float* __restrict__ dst, float* __restrict__ lse,
                                                                             float* __restrict__ scratch, int tiles, int parts) {
-    constexpr int kSteps = DP / 16;  // of the scores' sum
-    constexpr int kOut = DP / 32;    // output tiles
+    constexpr int kSteps = DC / 16;  // of the scores' sum
+    constexpr int kOut = DC / 32;    // output tiles
     constexpr int kLoads = DP / 64;  // 16-byte pieces of K, and of V, that a thread brings in
     extern __shared__ __align__(16) unsigned char smem[];
-    Stage<DP>* stage = reinterpret_cast<Stage<DP>*>(smem);
+    Stage<DC>* stage = reinterpret_cast<Stage<DC>*>(smem);
     __shared__ int first_page[kWaves], last_page[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, hf = lane >> 5;
-    const int h = blockIdx.x / parts, part = blockIdx.x % parts, s = blockIdx.z;
-    const int rt = tiles - 1 - (int)blockIdx.y;  // causal rows get longer: the long ones start first
+    const int h = blockIdx.x / parts, part = blockIdx.x % parts, s = blockIdx.y;
+    const int rt = tiles - 1 - (int)blockIdx.z;  // causal rows get longer: the long ones of all sequences start first
     const Kv8Seq q = kv8_seq(b, s);
     const int n_rows = q.n * a.group;
     if (rt * kRows >= n_rows) return;
@@ -154,8 +155,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
         const uint8_t* vp = c.v + at * (DP * kPage) + tid * 16;
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
-            kr[j] = *reinterpret_cast<const uint4*>(kp + j * kThreads * 16);
-            vr[j] = *reinterpret_cast<const uint4*>(vp + j * kThreads * 16);
+            if ((j + 1) * 64 <= DC || (tid & 3) < 2) kr[j] = *reinterpret_cast<const uint4*>(kp + j * kThreads * 16);
+            if ((j + 1) * 64 <= DC || tid < 128) vr[j] = *reinterpret_cast<const uint4*>(vp + j * kThreads * 16);
         }
         if (tid < 8) sr = (tid < 4 ? c.ks : c.vs)[at * subs + (tid & 3) * 16 / c.block];
         if (use_pos && tid < kPage) pr = c.pos[at * kPage + tid];
@@ -172,14 +173,18 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
             }
         }
     };
-    auto store = [&](Stage<DP>& st) {
+    auto store = [&](Stage<DC>& st) {
         const int t = tid >> 2, e = (tid & 3) * 16;
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
-            *reinterpret_cast<h8*>(&st.k[t][j * 64 + e]) = code_oct<F8>(kr[j].x, kr[j].y);
-            *reinterpret_cast<h8*>(&st.k[t][j * 64 + e + 8]) = code_oct<F8>(kr[j].z, kr[j].w);
-            *reinterpret_cast<h8*>(&st.v[j * 64 + t][e]) = code_oct<F8>(vr[j].x, vr[j].y);
-            *reinterpret_cast<h8*>(&st.v[j * 64 + t][e + 8]) = code_oct<F8>(vr[j].z, vr[j].w);
+            if ((j + 1) * 64 <= DC || e < 32) {
+                *reinterpret_cast<h8*>(&st.k[t][j * 64 + e]) = code_oct<F8>(kr[j].x, kr[j].y);
+                *reinterpret_cast<h8*>(&st.k[t][j * 64 + e + 8]) = code_oct<F8>(kr[j].z, kr[j].w);
+            }
+            if ((j + 1) * 64 <= DC || t < 32) {
+                *reinterpret_cast<h8*>(&st.v[j * 64 + t][e]) = code_oct<F8>(vr[j].x, vr[j].y);
+                *reinterpret_cast<h8*>(&st.v[j * 64 + t][e + 8]) = code_oct<F8>(vr[j].z, vr[j].w);
+            }
         }
         if (tid < 4) st.ks[tid] = sr;
         else if (tid < 8) st.vs[tid - 4] = sr;
@@ -196,22 +201,22 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
     __syncthreads();
     const int my_tok = (col & 3) + ((col >> 3) << 2) + (((col >> 2) & 1) << 4);  // token of MFMA row `col`
     for (int p = p0; p < p1; ++p) {
-        const Stage<DP>& st = stage[(p - p0) & 1];
+        const Stage<DC>& st = stage[(p - p0) & 1];
         const bool more = p + 1 < p1;
         if (more) fetch(p + 1);
         if (p >= w0 && p < w1) {
             // x[t][e]: token 32 t + 16 hf + e of the page
             f16x x[2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                x[t] = (f16x)(0.0f);
+            for (int t = 0; t < 2; ++t) x[t] = (f16x)(0.0f);
 #pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
                     const h8 key = *reinterpret_cast<const h8*>(&st.k[t * 32 + my_tok][k * 16 + hf * 8]);
                     x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, qh[k], x[t], 0, 0, 0);
                     x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, ql[k], x[t], 0, 0, 0);
                 }
-            }
             // (positions ascend: what the last row's window and document allow at the page's first token, all rows allow)
             const bool masked = (p + 1) * kPage > min(full_hi, q.len) ||
                                 (use_pos && (last_pos - st.pos[0] >= row.window || last_first > st.pos[0]));
@@ -369,7 +374,7 @@ __global__ __launch_bounds__(kThreads) void join_rows_kernel(Kv8Cache c, Kv8Batc
     const float* first = scratch + (((size_t)s * c.n_kv + h) * tiles + rt) * parts * kPieceFloats<DP>;
     float m = kNoMax, l = 0.0f;
     for (int k = 0; k < parts; ++k) m = fmaxf(m, first[(size_t)k * kPieceFloats<DP> + kRows * DP + r]);
-    float x[DP / 64] = {};
+    float x[DP / 64] = {};  // (columns behind head_dim are whatever the scratch held; they are not stored)
     for (int k = 0; k < parts; ++k) {
         const float* piece = first + (size_t)k * kPieceFloats<DP>;
         const float f = __builtin_amdgcn_exp2f(piece[kRows * DP + r] - m);
@@ -392,21 +397,27 @@ int parts_of(int cus, int n_kv, int group, int n_seq, int max_q, int max_pages) 
     return (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus / wgs, max_pages / 8));
 }
 
-template <int DP>
-void launch_prompt_dp(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch, int cus,
+template <int DP, int DC>
+void launch_prompt_dc(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch, int cus,
                       hipStream_t stream) {
     const bool gen = a.softcap > 0.0f || a.window > 0 || a.slopes || a.first || a.prefix;
     const int tiles = tiles_of(a.group, b.max_q), parts = parts_of(cus, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);
-    auto kernel = c.f8 ? (gen ? prompt_kernel<DP, true, true> : prompt_kernel<DP, true, false>)
-                       : (gen ? prompt_kernel<DP, false, true> : prompt_kernel<DP, false, false>);
-    const size_t lds = 2 * sizeof(Stage<DP>);
+    auto kernel = c.f8 ? (gen ? prompt_kernel<DP, DC, true, true> : prompt_kernel<DP, DC, true, false>)
+                       : (gen ? prompt_kernel<DP, DC, false, true> : prompt_kernel<DP, DC, false, false>);
+    const size_t lds = 2 * sizeof(Stage<DC>);
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     // heads side by side: workgroups go round the XCDs in this order, so a head's pages stay in one L2
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(c.n_kv * parts), (unsigned)tiles, (unsigned)b.n_seq), dim3(kThreads), lds, stream,
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(c.n_kv * parts), (unsigned)b.n_seq, (unsigned)tiles), dim3(kThreads), lds, stream,
                        c, b, a, dst, lse, scratch, tiles, parts);
     if (parts > 1)
         hipLaunchKernelGGL(join_rows_kernel<DP>, dim3((unsigned)(b.n_seq * c.n_kv * tiles), kRows / kWaves), dim3(kThreads), 0,
                            stream, c, b, a, dst, lse, scratch, tiles, parts);
+}
+template <int DP>
+void launch_prompt_dp(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch, int cus,
+                      hipStream_t stream) {
+    if (c.dim <= DP - 32) launch_prompt_dc<DP, DP - 32>(c, b, a, dst, lse, scratch, cus, stream);
+    else launch_prompt_dc<DP, DP>(c, b, a, dst, lse, scratch, cus, stream);
 }
 
 }  // namespace
