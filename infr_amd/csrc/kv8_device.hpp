@@ -122,21 +122,43 @@ __device__ __forceinline__ bool rows_vec(const Kv8Cache& c, const Kv8Attn& a) {
     return c.dim % 4 == 0 && a.q_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0;
 }
 
-// c * tanh(s / c), to the last bits of s (with s and c both times log2 e it is the capped score times that): an odd polynomial (the series of tanh) where tanh is nearly its
-// argument, 1 - 2 / (e^2y + 1) beyond, where the difference cancels no more than two bits.
-__device__ __forceinline__ float cap_score(float s, float c, float inv_c) {
-    const float y = s * inv_c, z = y * y;
-    float p = -1382.0f / 155925.0f;
-    p = __builtin_fmaf(p, z, 62.0f / 2835.0f);
-    p = __builtin_fmaf(p, z, -17.0f / 315.0f);
-    p = __builtin_fmaf(p, z, 2.0f / 15.0f);
-    p = __builtin_fmaf(p, z, -1.0f / 3.0f);
-    const float near = __builtin_fmaf(s * z, p, s);
-    const float a = fabsf(y);
-    if (__all(a < 0.35f)) return near;
-    const float e = __builtin_amdgcn_exp2f(a * (2.0f * kLog2e));
-    const float far = __builtin_copysignf(c * (1.0f - 2.0f / (e + 1.0f)), s);
-    return a < 0.35f ? near : a >= 0.35f ? far : s;  // NaN stays
+// x[i] = c * tanh(x[i] / c), to the last bits of x (with x and c both times log2 e it is the capped score times that).
+// Scores are mostly small beside the cap: where all of a wave's are below a quarter of it, four terms of tanh's series
+// serve (the fifth is under 2^-26). Else six below 0.35, and 1 - 2 / (e^2y + 1) beyond, whose difference cancels no more
+// than two bits.
+// FOURS: four of them at a time, where all at once would spill.
+template <int N, bool FOURS, typename X>
+__device__ __forceinline__ void cap_scores(X& x, float c, float inv_c) {
+    float most = fabsf(x[0]);
+#pragma unroll
+    for (int e = 1; e < N; ++e) most = fmaxf(most, fabsf(x[e]));
+    const float inv2 = inv_c * inv_c;
+    if (__all(most * inv_c < 0.25f)) {  // (a NaN among others does not show in `most`; the series passes it on)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float z = x[e] * x[e] * inv2;
+            float p = __builtin_fmaf(62.0f / 2835.0f, z, -17.0f / 315.0f);
+            p = __builtin_fmaf(p, z, 2.0f / 15.0f);
+            p = __builtin_fmaf(p, z, -1.0f / 3.0f);
+            x[e] = __builtin_fmaf(x[e], p * z, x[e]);
+            if (FOURS && e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float s = x[e], y = fabsf(s) * inv_c, z = s * s * inv2;
+            float p = __builtin_fmaf(-1382.0f / 155925.0f, z, 62.0f / 2835.0f);
+            p = __builtin_fmaf(p, z, -17.0f / 315.0f);
+            p = __builtin_fmaf(p, z, 2.0f / 15.0f);
+            p = __builtin_fmaf(p, z, -1.0f / 3.0f);
+            const float near = __builtin_fmaf(s, p * z, s), d = __builtin_amdgcn_exp2f(y * (2.0f * kLog2e)) + 1.0f;
+            float r = __builtin_amdgcn_rcpf(d);
+            r = __builtin_fmaf(r, __builtin_fmaf(-d, r, 1.0f), r);
+            const float far = __builtin_copysignf(c * (1.0f - 2.0f * (d < __builtin_inff() ? r : 0.0f)), s);
+            x[e] = y >= 0.35f ? far : near;
+            if (FOURS && e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+    }
 }
 
 // A block's value scale as the weights' exponent: log2 of scale / 2^v_exp. Blocks 2^60 below the largest scale count as

@@ -230,11 +230,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
                 vs[t] = st.vs[2 * t + hf];
                 if (masked || bent) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        float v = x[t][e] * factor[t];
-                        if (GEN && a.softcap > 0.0f) v = cap_score(v, cap, inv_cap);
-                        x[t][e] = v;
-                    }
+                    for (int e = 0; e < 16; ++e) x[t][e] *= factor[t];
+                    if (GEN && a.softcap > 0.0f) cap_scores<16, true>(x[t], cap, inv_cap);
                     factor[t] = 1.0f;
                 }
                 if (GEN && a.slopes)

@@ -142,15 +142,21 @@ __global__ __launch_bounds__(64 * kStepWaves, DP <= 128 ? 2 : 1) void score_step
         }
         float w[16];
         const bool bent = GEN && (a.softcap > 0.0f || a.slopes);
+        float f = factor;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = sc[e / 4][e % 4];
+        if (bent) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[e] *= factor;
+            if (a.softcap > 0.0f) cap_scores<16, false>(w, cap, inv_cap);
+            if (a.slopes)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) w[e] = __builtin_fmaf(-row.slope, fabsf((float)(row.pos - kpos[e])), w[e]);
+            f = 1.0f;
+        }
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            float v = sc[e / 4][e % 4];
-            if (bent) {
-                v *= factor;
-                if (a.softcap > 0.0f) v = cap_score(v, cap, inv_cap);
-                if (a.slopes) v = __builtin_fmaf(-row.slope, fabsf((float)(row.pos - kpos[e])), v);
-            }
-            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(v, bent ? 1.0f : factor, -row_lse));
+            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(w[e], f, -row_lse));
             w[e] = live ? y : 0.0f;
         }
         if (masked)
@@ -188,6 +194,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void score_prompt_kern
     constexpr int kSteps = DP / 16, kEach = DP / 8;  // a thread brings in kEach columns of a row: 8 threads a row
     extern __shared__ __align__(16) unsigned char smem[];
     Rows<DP>* rows = reinterpret_cast<Rows<DP>*>(smem);
+    __shared__ __align__(16) int page_pos[kWaves][kPage];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, hf = lane >> 5;
     const int h = blockIdx.x / parts, part = blockIdx.x % parts, s = blockIdx.z;
     const Kv8Seq q = kv8_seq(b, s);
@@ -203,7 +210,6 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void score_prompt_kern
     const int my_tok = (col & 3) + ((col >> 3) << 2) + (((col >> 2) & 1) << 4);
     h8 key[2][kSteps];
     float ks[2];
-    int kpos[2][16];
     const bool use_pos = GEN && (a.window > 0 || a.slopes || a.first || a.prefix);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -213,10 +219,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void score_prompt_kern
             const uint2 u = *reinterpret_cast<const uint2*>(c.k + at * (DP * kPage) + ((k / 4) * kPage + 32 * t + my_tok) * 64 + (k % 4) * 16 + hf * 8);
             key[t][k] = code_oct<F8>(u.x, u.y);
         }
-        if (use_pos)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) kpos[t][e] = c.pos[at * kPage + 32 * t + 16 * hf + e];
     }
+    if (use_pos) page_pos[wave][lane] = c.pos[at * kPage + lane];  // (the barrier before the first step comes in between)
     const int pos0 = use_pos ? c.pos[at * kPage] : 0;
     // rows that see any token of the workgroup's pages: by causality none before the first token's own, by the window
     // none from `window` behind the last one on (positions ascend strictly)
@@ -322,22 +326,33 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void score_prompt_kern
                 float factor = r.factor[col] * ks[t];
                 if (GEN && (a.softcap > 0.0f || a.slopes)) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        float y = x[t][e] * factor;
-                        if (a.softcap > 0.0f) y = cap_score(y, cap, inv_cap);
-                        if (a.slopes) y = __builtin_fmaf(-row.slope, fabsf((float)(row.pos - kpos[t][e])), y);
-                        x[t][e] = y;
-                    }
+                    for (int e = 0; e < 16; ++e) x[t][e] *= factor;
+                    if (a.softcap > 0.0f) cap_scores<16, false>(x[t], cap, inv_cap);
+                    if (a.slopes)
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) {
+                            const int4 y = *reinterpret_cast<const int4*>(&page_pos[wave][32 * t + 16 * hf + e]);
+                            const int kpos[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                            for (int n = 0; n < 4; ++n)
+                                x[t][e + n] = __builtin_fmaf(-row.slope, fabsf((float)(row.pos - kpos[n])), x[t][e + n]);
+                        }
                     factor = 1.0f;
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) x[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][e], factor, -row_lse));
                 if (masked)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int tok = p * kPage + 32 * t + 16 * hf + e;
-                        const bool yes = tok < q.len && row.first != 0x7FFFFFFF && (use_pos ? row.sees(tok, kpos[t][e]) : tok <= row.slot);
-                        x[t][e] = yes ? x[t][e] : 0.0f;
+                    for (int e = 0; e < 16; e += 4) {
+                        int4 y = make_int4(0, 0, 0, 0);
+                        if (use_pos) y = *reinterpret_cast<const int4*>(&page_pos[wave][32 * t + 16 * hf + e]);
+                        const int kpos[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            const int tok = p * kPage + 32 * t + 16 * hf + e + n;
+                            const bool yes = tok < q.len && row.first != 0x7FFFFFFF && (use_pos ? row.sees(tok, kpos[n]) : tok <= row.slot);
+                            x[t][e + n] = yes ? x[t][e + n] : 0.0f;
+                        }
                     }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[16 * t + e] += x[t][e];

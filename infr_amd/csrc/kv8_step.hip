@@ -169,12 +169,11 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
         }
         if (masked || (GEN && (a.softcap > 0.0f || a.slopes))) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                float v = x[e] * factor;
-                if (GEN && a.softcap > 0.0f) v = cap_score(v, cap, inv_cap);
-                if (GEN && a.slopes) v = __builtin_fmaf(-row.slope, fabsf((float)(row.pos - kpos[e])), v);
-                x[e] = v;
-            }
+            for (int e = 0; e < 16; ++e) x[e] *= factor;
+            if (GEN && a.softcap > 0.0f) cap_scores<16, false>(x, cap, inv_cap);
+            if (GEN && a.slopes)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = __builtin_fmaf(-row.slope, fabsf((float)(row.pos - kpos[e])), x[e]);
             f = 1.0f;
         }
         bool any = true;
