@@ -7,9 +7,6 @@
 
 namespace infr {
 
-int step_rows(int group, int max_q);
-int step_target(int cus, int64_t tiles);
-size_t step_items(int cus, int n_kv, int group, int n_seq, int max_q, int max_pages);
 size_t step_scratch(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages);
 void launch_attention_step(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch,
                            int cus, hipStream_t stream);

@@ -196,7 +196,6 @@ __device__ __forceinline__ Kv8Row kv8_row(const Kv8Batch& b, const Kv8Attn& a, c
 
 constexpr int kStepWaves = 4;   // waves of a workgroup, each a page at a time
 constexpr int kStepRows = 16;   // query rows of a workgroup, or half of them: see step_rows
-constexpr int kWholePages = 12; // sequences of up to so many pages are one piece: four pages a wave cost less than a join
 
 // Row tiles, first page any row sees, pages from there. `all`: every cached page is gone over by one tile, whether
 // rows see it or not (ScoreKv8 lets sums decay).
@@ -274,10 +273,10 @@ struct SeqCut {
     int parts, first;
 };
 // The share of sequence `want`, or, with want < 0, of the sequence that holds piece `item`. About `target` pieces are
-// aimed at, of at least one page for each wave of a workgroup. Up to 64 sequences take one round of loads, and the
+// aimed at, of at least one page for each wave of a workgroup; sequences of up to `whole` pages are one. Up to 64 sequences take one round of loads, and the
 // sequence found is passed between the lanes; more of them take a loop over the tables and another over the counts.
-__device__ __forceinline__ SeqCut find_cut(const Kv8Batch& b, const Kv8Attn& a, int n_kv, int rows, int target, bool all, int want,
-                                           int item) {
+__device__ __forceinline__ SeqCut find_cut(const Kv8Batch& b, const Kv8Attn& a, int n_kv, int rows, int target, int whole, bool all,
+                                           int want, int item) {
     const int lane = (int)(threadIdx.x & 63);
     Kv8Seq q{};
     SeqWork w{};
@@ -301,7 +300,7 @@ __device__ __forceinline__ SeqCut find_cut(const Kv8Batch& b, const Kv8Attn& a, 
                 w = seq_work(q, a, rows, all);
             }
         }
-        const int parts = s < b.n_seq ? (w.pages <= kWholePages ? 1 : (w.pages + size - 1) / size) : 0, n = n_kv * w.tiles * parts;
+        const int parts = s < b.n_seq ? (w.pages <= whole ? 1 : (w.pages + size - 1) / size) : 0, n = n_kv * w.tiles * parts;
         const int sum = wave_scan(s < b.n_seq ? n : 0);
         const unsigned long long hit = __ballot(want >= 0 ? s == want : item - before < sum);
         if (hit) {

@@ -34,10 +34,10 @@ __device__ __forceinline__ void fold(float* x, bool upper) {
 template <int DP, bool F8, bool GEN>
 __global__ __launch_bounds__(64 * kStepWaves, DP <= 128 ? 2 : 1) void score_step_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a,
                                                                                        const float* __restrict__ lse,
-                                                                                       float decay, int target) {
+                                                                                       float decay, int target, int whole) {
     constexpr int kCols = DP / 64;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    const SeqCut cut = find_cut(b, a, c.n_kv, kStepRows, target, true, -1, (int)blockIdx.x);
+    const SeqCut cut = find_cut(b, a, c.n_kv, kStepRows, target, whole, true, -1, (int)blockIdx.x);
     if (cut.s < 0 || !cut.q.ok) return;
     const int s = cut.s, parts = cut.parts, rest = (int)blockIdx.x - cut.first;
     const Kv8Seq q = cut.q;
@@ -412,9 +412,12 @@ void launch_score_dp(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, con
     if (few_rows(b.max_q, a.group)) {
         auto kernel = c.f8 ? (gen ? score_step_kernel<DP, true, true> : score_step_kernel<DP, true, false>)
                            : (gen ? score_step_kernel<DP, false, true> : score_step_kernel<DP, false, false>);
-        const unsigned items = (unsigned)step_items(cus, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);
-        hipLaunchKernelGGL(kernel, dim3(items), dim3(64 * kStepWaves), 0, stream, c, b, a, lse, decay,
-                           step_target(cus, (int64_t)b.n_seq * c.n_kv));
+        // pieces: there is no join here, so no sequence has to be whole, and three for each compute unit level out best
+        // (32 sequences' step: 27 us; two or four 29)
+        const int64_t heads = (int64_t)b.n_seq * c.n_kv;
+        const int target = 3 * cus;
+        const unsigned items = (unsigned)std::min(target + heads, heads * ((b.max_pages + kStepWaves - 1) / kStepWaves));
+        hipLaunchKernelGGL(kernel, dim3(items), dim3(64 * kStepWaves), 0, stream, c, b, a, lse, decay, target, kStepWaves);
         return;
     }
     const int parts = parts_of(cus, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);

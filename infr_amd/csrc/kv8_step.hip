@@ -29,7 +29,7 @@ constexpr int kPieceFloats = ROWS * DP + 2 * ROWS;
 template <int DP, int ROWS, bool F8, bool GEN>
 __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192 && ROWS == 8) ? 2 : 1) void step_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a,
                                                                              float* __restrict__ dst, float* __restrict__ lse,
-                                                                             float* __restrict__ scratch, int target) {
+                                                                             float* __restrict__ scratch, int target, int whole_pages) {
     constexpr int kCols = DP / 64;   // 64-column groups of a key
     constexpr int kOut = DP / 16;    // 16-column groups of a value
     constexpr int kFours = DP / 4, kThreads = 64 * kWaves;
@@ -39,7 +39,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
     static_assert(sizeof(StepQ<DP, ROWS>) <= sizeof(part_o), "the rows fit");
     __shared__ float part_m[kWaves][16], part_l[kWaves][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    const SeqCut cut = find_cut(b, a, c.n_kv, ROWS, target, false, -1, (int)blockIdx.x);
+    const SeqCut cut = find_cut(b, a, c.n_kv, ROWS, target, whole_pages, false, -1, (int)blockIdx.x);
     if (cut.s < 0) return;
     const int s = cut.s, parts = cut.parts, rest = (int)blockIdx.x - cut.first;
     const Kv8Seq q = cut.q;
@@ -321,12 +321,12 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
 template <int DP, int ROWS>
 __global__ __launch_bounds__(256) void join_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a, float* __restrict__ dst,
                                                    float* __restrict__ lse, const float* __restrict__ scratch, int target,
-                                                   int max_tiles) {
+                                                   int whole_pages, int max_tiles) {
     __shared__ __align__(16) float part[1024 / DP][DP];
     const int lane = threadIdx.x & 63;
     const int rt = blockIdx.x % max_tiles, h = blockIdx.x / max_tiles % c.n_kv, s = blockIdx.x / max_tiles / c.n_kv;
     const int r = blockIdx.y, r_all = rt * ROWS + r;
-    const SeqCut cut = find_cut(b, a, c.n_kv, ROWS, target, false, s, 0);
+    const SeqCut cut = find_cut(b, a, c.n_kv, ROWS, target, whole_pages, false, s, 0);
     const Kv8Seq q = cut.q;
     const int parts = cut.parts;
     if (r_all >= q.n * a.group || parts == 1) return;
@@ -361,23 +361,43 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8Cache c, Kv8Batch b, Kv8At
     dst[out * c.dim + d] = l == 0.0f ? 0.0f : y / l;
 }
 
+// Query rows of a workgroup: 8 where no sequence has more.
+int step_rows(int group, int max_q) { return (int64_t)max_q * group <= 8 ? 8 : kStepRows; }
 int max_tiles_of(int group, int max_q) {
     const int rows = step_rows(group, max_q);
     return (int)(((int64_t)max_q * group + rows - 1) / rows);
 }
 
+// Pieces aimed at. What runs at a time are two workgroups on a compute unit, one with more than 128 columns: with fewer
+// (sequence, head, row tile)s than that, so many pieces that they are one round together with half a piece each for the
+// rounding up (two sequences of 115000 tokens: 46 us, with half as many again 50). Else they come in rounds, and more of
+// them level out (64 sequences of 500 to 8000 tokens, 8 heads: 72 us, with two thirds of them 74).
+int step_target(int cus, int dim, int64_t tiles) {
+    const int64_t slots = dim <= 128 ? 2 * cus : cus;
+    return (int)(tiles < slots ? std::max(slots - tiles / 2, slots / 2) : dim <= 128 ? 3 * cus : 2 * cus);
+}
+// Sequences of up to so many pages are one piece: the pages a wave goes over more cost less than a join, the less so the
+// fewer compute units have work (one sequence of 700 tokens: 11.8 us whole, 12.9 in three; drafts of 16 sequences over
+// 1024 tokens of 256 columns: 28 us whole, 37 in two).
+int step_whole(int cus, int64_t tiles) { return 2 * tiles >= cus ? 24 : 12; }
+// Upper bound of the pieces: the total is cut into `target`, and each (sequence, head, row tile) rounds up once.
+size_t step_items(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages) {
+    const size_t tiles = (size_t)n_seq * n_kv * max_tiles_of(group, max_q);
+    return std::min((size_t)step_target(cus, dim, (int64_t)tiles) + tiles, tiles * (size_t)((max_pages + kWaves - 1) / kWaves));
+}
 template <int DP, int ROWS>
 void launch_step_rows(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch, int cus,
                       hipStream_t stream) {
-    const int tiles = max_tiles_of(a.group, b.max_q), target = step_target(cus, (int64_t)b.n_seq * c.n_kv * tiles);
+    const int tiles = max_tiles_of(a.group, b.max_q), target = step_target(cus, c.dim, (int64_t)b.n_seq * c.n_kv * tiles);
+    const int whole = step_whole(cus, (int64_t)b.n_seq * c.n_kv * tiles);
     const bool gen = a.softcap > 0.0f || a.window > 0 || a.slopes || a.first || a.prefix;
-    const unsigned items = (unsigned)step_items(cus, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);
+    const unsigned items = (unsigned)step_items(cus, c.dim, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);
     auto kernel = c.f8 ? (gen ? step_kernel<DP, ROWS, true, true> : step_kernel<DP, ROWS, true, false>)
                        : (gen ? step_kernel<DP, ROWS, false, true> : step_kernel<DP, ROWS, false, false>);
-    hipLaunchKernelGGL(kernel, dim3(items), dim3(64 * kWaves), 0, stream, c, b, a, dst, lse, scratch, target);
-    if (b.max_pages <= kWholePages) return;  // no sequence has two pieces
+    hipLaunchKernelGGL(kernel, dim3(items), dim3(64 * kWaves), 0, stream, c, b, a, dst, lse, scratch, target, whole);
+    if (b.max_pages <= whole) return;  // no sequence has two pieces
     hipLaunchKernelGGL((join_kernel<DP, ROWS>), dim3((unsigned)(b.n_seq * c.n_kv * tiles), (unsigned)std::min(ROWS, b.max_q * a.group)),
-                       dim3(256), 0, stream, c, b, a, dst, lse, scratch, target, tiles);
+                       dim3(256), 0, stream, c, b, a, dst, lse, scratch, target, whole, tiles);
 }
 template <int DP>
 void launch_step_dp(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch, int cus,
@@ -388,21 +408,10 @@ void launch_step_dp(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, floa
 
 }  // namespace
 
-// Query rows of a workgroup: 8 where no sequence has more.
-int step_rows(int group, int max_q) { return (int64_t)max_q * group <= 8 ? 8 : kStepRows; }
-// Pieces aimed at: two for each compute unit, which is what runs at a time (two sequences of 115000 tokens: 46 us, with
-// three 50); three where the batch has more (sequence, head, row tile)s than compute units, whose pieces differ in size
-// (64 sequences of 500 to 8000 tokens, 8 heads: 72 us, with two 74).
-int step_target(int cus, int64_t tiles) { return (tiles > cus ? 3 : 2) * cus; }
-// Upper bound of the pieces: the total is cut into `target`, and each (sequence, head, row tile) rounds up once.
-size_t step_items(int cus, int n_kv, int group, int n_seq, int max_q, int max_pages) {
-    const size_t tiles = (size_t)n_seq * n_kv * max_tiles_of(group, max_q);
-    return std::min((size_t)step_target(cus, (int64_t)tiles) + tiles, tiles * (size_t)((max_pages + kWaves - 1) / kWaves));
-}
 size_t step_scratch(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages) {
-    if (max_pages <= kWholePages) return 0;
+    if (max_pages <= step_whole(cus, (int64_t)n_seq * n_kv * max_tiles_of(group, max_q))) return 0;
     const size_t dp = (size_t)(dim + 63) / 64 * 64;
-    return step_items(cus, n_kv, group, n_seq, max_q, max_pages) * (kStepRows * dp + 2 * kStepRows) * sizeof(float);
+    return step_items(cus, dim, n_kv, group, n_seq, max_q, max_pages) * (kStepRows * dp + 2 * kStepRows) * sizeof(float);
 }
 void launch_attention_step(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch,
                            int cus, hipStream_t stream) {
