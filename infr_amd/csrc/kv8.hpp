@@ -150,21 +150,29 @@ __device__ __forceinline__ int wave_scan(int x) {
     return x;
 }
 
-// The sequence that work item `idx` belongs to, where sequence s has count(s) >= 0 of them, and in *rest its
-// number within the sequence; -1 when there are fewer items. Every lane of the wave calls it with the same idx.
+// The sequence that work item `idx` belongs to, where a sequence has count(its tables) >= 0 of them; in *rest the item's
+// number within the sequence and in *q its tables; -1 when there are fewer items. Every lane of the wave calls it with
+// the same idx: lanes look at 64 sequences at once and pass on the one found.
 template <typename F>
-__device__ __forceinline__ int find_seq(int n_seq, int idx, int* rest, F count) {
+__device__ __forceinline__ int find_seq(const Kv8Batch& b, int idx, int* rest, Kv8Seq* q, F count) {
     const int lane = (int)(threadIdx.x & 63);
-    for (int base = 0; base < n_seq; base += 64) {
-        const int n = base + lane < n_seq ? count(base + lane) : 0;
+    for (int base = 0; base < b.n_seq; base += 64) {
+        Kv8Seq mine{};
+        if (base + lane < b.n_seq) mine = kv8_seq(b, base + lane);
+        const int n = base + lane < b.n_seq ? count(mine) : 0;
         const int sum = wave_scan(n);
         const unsigned long long hit = __ballot(idx < sum);
         if (hit) {
             const int l = __builtin_ctzll(hit);
-            *rest = idx - (__shfl(sum, l) - __shfl(n, l));
+            auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+            *rest = idx - (of(sum) - of(n));
+            q->r0 = of(mine.r0);
+            q->n = of(mine.n);
+            q->len = of(mine.len);
+            q->ok = of((int)mine.ok) != 0;
             return base + l;
         }
-        idx -= __shfl(sum, 63);
+        idx -= __builtin_amdgcn_readlane(sum, 63);
     }
     return -1;
 }

@@ -18,7 +18,6 @@ namespace infr {
 
 namespace {
 
-constexpr int kSelect = 1024;
 constexpr int kMove = 256;
 constexpr int kBinBits = 11, kBins = 1 << kBinBits;
 
@@ -26,8 +25,8 @@ struct EvictSeq {
     int len, n_out;
     bool ok;
 };
-// Tokens of sequence s before and after, and whether every page either of them needs exists. Uniform over the
-// workgroup; `nthreads` threads take part.
+// Tokens of sequence s before and after, and whether every page either of them needs exists, as far as this thread has
+// looked: `nthreads` threads take part.
 __device__ __forceinline__ EvictSeq evict_seq(const Kv8Cache& c, const Kv8Evict& e, int s, int tid, int nthreads) {
     EvictSeq q;
     q.len = e.lens[s];
@@ -44,7 +43,7 @@ __device__ __forceinline__ EvictSeq evict_seq(const Kv8Cache& c, const Kv8Evict&
             ok = ok && page >= 0 && page < c.n_pages;
         }
     }
-    q.ok = __syncthreads_and(ok) != 0;
+    q.ok = ok;
     return q;
 }
 
@@ -56,6 +55,7 @@ __device__ __forceinline__ uint32_t sum_key(float x) {
 }
 
 // Exclusive prefix sum over the workgroup's threads and the total; `part` holds one entry per wave.
+template <int THREADS>
 __device__ __forceinline__ int block_scan(int x, int* part, int* total) {
     const int w = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63;
     const int sum = wave_scan(x);
@@ -64,7 +64,7 @@ __device__ __forceinline__ int block_scan(int x, int* part, int* total) {
     __syncthreads();
     int before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < kSelect / 64; ++i) {
+    for (int i = 0; i < THREADS / 64; ++i) {
         if (i < w) before += part[i];
         all += part[i];
     }
@@ -72,27 +72,19 @@ __device__ __forceinline__ int block_scan(int x, int* part, int* total) {
     return before + sum - x;
 }
 
-// EACH neighbouring tokens of a thread at a time; sequences of more than EACH * 1024 tokens go over them in rounds,
+// EACH neighbouring tokens of a thread at a time; sequences of more than EACH * THREADS tokens go over them in rounds,
 // reading the sums again for each pass.
-template <int EACH>
-__global__ __launch_bounds__(kSelect, 4) void evict_select_kernel(Kv8Cache c, Kv8Evict e) {
-    __shared__ int part[kSelect / 64];
+template <int THREADS, int EACH>
+__global__ __launch_bounds__(THREADS, 4) void evict_select_kernel(Kv8Cache c, Kv8Evict e) {
+    __shared__ int part[THREADS / 64];
     __shared__ int hist[kBins];
     __shared__ uint32_t found[2], ends[2];
     const int s = blockIdx.y, h = blockIdx.x, tid = threadIdx.x;
-    const EvictSeq q = evict_seq(c, e, s, tid, kSelect);
-    int32_t* kept = e.kept + ((size_t)s * c.n_kv + h) * e.keep;
-    for (int i = (q.ok ? q.n_out : 0) + tid; i < e.keep; i += kSelect) kept[i] = -1;
-    if (h == 0 && tid == 0) e.lens_out[s] = q.ok ? q.n_out : -1;
-    if (!q.ok) return;
-    if (q.len <= e.keep) {
-        for (int i = tid; i < q.len; i += kSelect) kept[i] = i;
-        return;
-    }
+    const EvictSeq q = evict_seq(c, e, s, tid, THREADS);
     const int32_t* pages = e.pages + (size_t)s * e.max_pages;
     const int lo = e.sink, hi = q.len - e.recent;  // candidates: more than `need` of them, as len > keep
     const int need = e.keep - e.sink - e.recent;
-    const int span = EACH * kSelect, rounds = (q.len + span - 1) / span;
+    const int span = EACH * THREADS, rounds = (q.len + span - 1) / span;
     // key of each of the thread's tokens, 0 for those that are no candidates: below every number's key
     uint32_t key[EACH];
     auto load = [&](int round) {
@@ -101,14 +93,27 @@ __global__ __launch_bounds__(kSelect, 4) void evict_select_kernel(Kv8Cache c, Kv
         for (int n = 0; n < EACH; n += 4) {
             const int j = j0 + n;  // (four tokens lie in one page)
             float4 x = make_float4(0, 0, 0, 0);
-            if (j < q.len) x = *reinterpret_cast<const float4*>(c.sums + ((size_t)pages[j / kPage] * c.n_kv + h) * kPage + j % kPage);
+            if (j < q.len) {
+                const int page = pages[j / kPage];  // (may be wrong until the check below)
+                x = *reinterpret_cast<const float4*>(c.sums + ((size_t)min(max(page, 0), c.n_pages - 1) * c.n_kv + h) * kPage + j % kPage);
+            }
             key[n] = j >= lo && j < hi ? sum_key(x.x) : 0;
             key[n + 1] = j + 1 >= lo && j + 1 < hi ? sum_key(x.y) : 0;
             key[n + 2] = j + 2 >= lo && j + 2 < hi ? sum_key(x.z) : 0;
             key[n + 3] = j + 3 >= lo && j + 3 < hi ? sum_key(x.w) : 0;
         }
     };
-    load(0);
+    const bool fits = q.len >= 0 && (int64_t)q.len <= (int64_t)e.max_pages * kPage;
+    if (fits && q.len > e.keep) load(0);
+    const bool ok = __syncthreads_and(q.ok) != 0;
+    int32_t* kept = e.kept + ((size_t)s * c.n_kv + h) * e.keep;
+    for (int i = (ok ? q.n_out : 0) + tid; i < e.keep; i += THREADS) kept[i] = -1;
+    if (h == 0 && tid == 0) e.lens_out[s] = ok ? q.n_out : -1;
+    if (!ok) return;
+    if (q.len <= e.keep) {
+        for (int i = tid; i < q.len; i += THREADS) kept[i] = i;
+        return;
+    }
     // the need-th largest key: `limit`, and how many of those equal to it stay: `ties`
     uint32_t limit = 0;
     int ties = need;
@@ -138,7 +143,7 @@ __global__ __launch_bounds__(kSelect, 4) void evict_select_kernel(Kv8Cache c, Kv
         uint32_t width = ends[1] - ends[0];  // keys in question: limit .. limit + width
         while (width > 0) {
             const int shift = max(32 - __builtin_clz(width) - kBinBits, 0);
-            for (int i = tid; i < kBins; i += kSelect) hist[i] = 0;
+            for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
             __syncthreads();
             for (int r = 0; r < rounds; ++r) {
                 if (rounds > 1) load(r);
@@ -147,13 +152,13 @@ __global__ __launch_bounds__(kSelect, 4) void evict_select_kernel(Kv8Cache c, Kv
                     if (key[n] && key[n] - limit <= width) atomicAdd(&hist[(key[n] - limit) >> shift], 1);
             }
             __syncthreads();
-            // thread i: bins from the top, kBins / kSelect of them
-            constexpr int kMine = kBins / kSelect;
+            // thread i: bins from the top, kBins / THREADS of them
+            constexpr int kMine = kBins / THREADS;
             const int top = kBins - 1 - tid * kMine;
             int mine = 0, total = 0;
 #pragma unroll
             for (int i = 0; i < kMine; ++i) mine += hist[top - i];
-            int above = block_scan(mine, part, &total);
+            int above = block_scan<THREADS>(mine, part, &total);
             if (above < ties && ties <= above + mine)
 #pragma unroll
                 for (int i = 0; i < kMine; ++i) {
@@ -180,7 +185,7 @@ __global__ __launch_bounds__(kSelect, 4) void evict_select_kernel(Kv8Cache c, Kv
         int equal = 0;
 #pragma unroll
         for (int n = 0; n < EACH; ++n) equal += need > 0 && key[n] == limit && key[n] ? 1 : 0;
-        int rank = equal_before + block_scan(equal, part, &total);
+        int rank = equal_before + block_scan<THREADS>(equal, part, &total);
         equal_before += total;
         uint32_t take = 0;
 #pragma unroll
@@ -193,7 +198,7 @@ __global__ __launch_bounds__(kSelect, 4) void evict_select_kernel(Kv8Cache c, Kv
             }
             take |= (uint32_t)yes << n;
         }
-        int at = out_before + block_scan(__builtin_popcount(take), part, &total);
+        int at = out_before + block_scan<THREADS>(__builtin_popcount(take), part, &total);
         out_before += total;
 #pragma unroll
         for (int n = 0; n < EACH; ++n)
@@ -207,16 +212,15 @@ __global__ __launch_bounds__(kMove) void evict_move_kernel(Kv8Cache c, Kv8Evict 
     __shared__ uint32_t amax[kPage];
     const int s = blockIdx.z, h = (int)blockIdx.y >> 1, po = blockIdx.x, tid = threadIdx.x;
     const bool is_v = blockIdx.y & 1;
-    const int n_out = e.lens_out[s];
-    if (n_out <= po * kPage) return;  // also -1: a sequence that was left as it is
-    const int cnt = min(kPage, n_out - po * kPage);
     const int to = e.pages_out[(size_t)s * e.out_pages + po];
     const int subs = kPage / c.block;
     // K: four lanes to a token, 16 columns of each 64; V: a lane to a token, a quarter of the columns to a wave
     const int t = is_v ? tid & 63 : tid >> 2, part = is_v ? tid >> 6 : tid & 3;
-    const bool live = t < cnt;
+    // (kept is -1 behind the last token, and all through for a sequence that was left as it is)
     const int32_t* kept = e.kept + ((size_t)s * c.n_kv + h) * e.keep + po * kPage;
-    const int j = live ? kept[t] : -1, j0 = kept[t / c.block * c.block < cnt ? t / c.block * c.block : 0];
+    const int room = min(kPage, e.keep - po * kPage), lead = t / c.block * c.block;
+    const int j = t < room ? kept[t] : -1, j0 = lead < room ? kept[lead] : -1;
+    const bool live = j >= 0;
     if (tid < kPage) amax[tid] = 0;
     // amax's top bit marks a block that has to be quantized again
     const bool in_place = !live || (j == j0 + t % c.block && j0 % c.block == 0);
@@ -295,9 +299,11 @@ __global__ __launch_bounds__(kMove) void evict_move_kernel(Kv8Cache c, Kv8Evict 
 
 void launch_evict_kv8(const Kv8Cache& c, const Kv8Evict& e, hipStream_t stream) {
     const dim3 grid((unsigned)c.n_kv, (unsigned)e.n_seq);
+    // threads for one round over the sequence where 32 tokens each are enough, no more: they all meet at the barriers
     const int64_t most = (int64_t)e.max_pages * kPage;
-    auto select = most <= 4 * kSelect ? evict_select_kernel<4> : evict_select_kernel<32>;
-    hipLaunchKernelGGL(select, grid, dim3(kSelect), 0, stream, c, e);
+    if (most <= 256 * 8) hipLaunchKernelGGL((evict_select_kernel<256, 8>), grid, dim3(256), 0, stream, c, e);
+    else if (most <= 512 * 16) hipLaunchKernelGGL((evict_select_kernel<512, 16>), grid, dim3(512), 0, stream, c, e);
+    else hipLaunchKernelGGL((evict_select_kernel<1024, 32>), grid, dim3(1024), 0, stream, c, e);
     auto pick = [&](auto f8) {
         constexpr bool F8 = decltype(f8)::value;
         return c.dp == 64 ? evict_move_kernel<64, F8> : c.dp == 128 ? evict_move_kernel<128, F8>

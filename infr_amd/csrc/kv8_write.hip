@@ -22,9 +22,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kTurn = kPage + 4;  // LDS row of value codes: 4 bytes of padding keep the columns off one bank
 
-// Pages of sequence s that get tokens.
-__device__ __forceinline__ int pages_written(const Kv8Batch& b, int s) {
-    const Kv8Seq q = kv8_seq(b, s);
+// Pages of a sequence that get tokens.
+__device__ __forceinline__ int pages_written(const Kv8Seq& q) {
     return q.ok && q.n > 0 ? (q.len - 1) / kPage - (q.len - q.n) / kPage + 1 : 0;
 }
 
@@ -36,11 +35,11 @@ __global__ __launch_bounds__(kThreads) void write_kv8_kernel(Kv8Cache c, Kv8Batc
     __shared__ uint32_t amax[kPage];
     __shared__ __align__(16) uint8_t turn[64 * kTurn];
     int rest = 0;
-    const int s = find_seq(b.n_seq, (int)blockIdx.x, &rest, [&](int i) { return pages_written(b, i); });
+    Kv8Seq q;
+    const int s = find_seq(b, (int)blockIdx.x, &rest, &q, [](const Kv8Seq& x) { return pages_written(x); });
     if (s < 0) return;
     const int h = blockIdx.y;
     const bool is_v = blockIdx.z != 0;
-    const Kv8Seq q = kv8_seq(b, s);
     const int slot0 = q.len - q.n;                       // first new token
     const int pi = slot0 / kPage + rest;                 // page of the sequence
     const int page = b.pages[(size_t)s * b.max_pages + pi];
@@ -65,9 +64,10 @@ __global__ __launch_bounds__(kThreads) void write_kv8_kernel(Kv8Cache c, Kv8Batc
 
     // this thread's columns, 16 of each 64: zero behind the sequence's end and the row's
     float r[kGroups][16];
+    // (the tail's rows are asked for together with the tag that says whether they are the block's)
     const float* src = nullptr;
     if (is_new) src = x + (size_t)(q.r0 + tok - slot0) * stride + (size_t)h * c.dim;
-    else if (is_old && raw) src = c.tail + tail_at + (size_t)(tok - open) * c.dim;
+    else if (is_old && tail_ok) src = c.tail + tail_at + (size_t)(tok - open) * c.dim;
     const bool vec = c.dim % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
 #pragma unroll
     for (int j = 0; j < kGroups; ++j) {
@@ -83,15 +83,21 @@ __global__ __launch_bounds__(kThreads) void write_kv8_kernel(Kv8Cache c, Kv8Batc
             for (int e = 0; e < 16; ++e) r[j][e] = d0 + e < c.dim ? src[d0 + e] : 0.0f;
         } else {
 #pragma unroll
+            for (int e = 0; e < 16; ++e) r[j][e] = 0.0f;
+        }
+    }
+    if (is_old && !raw)  // rows the tail does not have: at their values in the cache
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j)
+#pragma unroll
             for (int e = 0; e < 16; ++e) {
+                const int d = j * 64 + col + e;
                 r[j][e] = 0.0f;
-                if (is_old && page_ok && d0 + e < c.dim) {
-                    const size_t at = is_v ? v_at(c, page, h, t, d0 + e) : k_at(c, page, h, t, d0 + e);
+                if (page_ok && d < c.dim) {
+                    const size_t at = is_v ? v_at(c, page, h, t, d) : k_at(c, page, h, t, d);
                     r[j][e] = kv8_value<F8>((is_v ? c.v : c.k)[at]) * old_scale;
                 }
             }
-        }
-    }
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < kGroups; ++j)
