@@ -101,29 +101,27 @@ __device__ __forceinline__ float kv8_scale(uint32_t amax_bits, bool f8) {
     if (amax_bits >= 0x7F800000u) return __builtin_nanf("");
     return fmaxf(__builtin_bit_cast(float, amax_bits) / (f8 ? 448.0f : 127.0f), kMinScale);
 }
-// 1 / scale for kv8_code, to an ulp; 0 for a NaN scale, whose codes are 0.
+// 1 / scale for kv8_code; 0 for a NaN scale, whose codes are 0.
 __device__ __forceinline__ float kv8_inverse(float scale) {
-    return scale < __builtin_inff() ? __builtin_amdgcn_rcpf(scale) : 0.0f;
+    if (!(scale < __builtin_inff())) return 0.0f;
+    const float r = __builtin_amdgcn_rcpf(scale);
+    return __builtin_fmaf(__builtin_fmaf(-scale, r, 1.0f), r, r);
 }
-// Nearest code of x / scale (the correctly rounded quotient), ties to even. x * inverse is off by less than 2^-21 of
-// it; only where that leaves the code in doubt is the quotient itself formed, a few in 10^4. |x / scale| stays below
-// the largest code's rounding border: the scale is amax / code_max rounded once and the quotient once more.
+// Nearest code of x / scale, ties to even. The quotient is the correctly rounded one: x times the inverse, corrected twice
+// by its remainder, which a fused multiply-add gives exactly (Markstein's division; scales and codes keep every number in
+// it clear of overflow and of what the remainder could lose). It stays below the largest code's rounding border: the scale
+// is amax / code_max rounded once and the quotient once more.
 template <bool F8>
 __device__ __forceinline__ uint32_t kv8_code(float x, float scale, float inverse) {
-    if (inverse == 0.0f) return 0;
     float y = x * inverse;
+    y = __builtin_fmaf(__builtin_fmaf(-scale, y, x), inverse, y);
+    y = __builtin_fmaf(__builtin_fmaf(-scale, y, x), inverse, y);
+    uint32_t code;
     if constexpr (F8) {
-        uint32_t two = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y * (1.0f - 0x1p-20f), y * (1.0f + 0x1p-20f), 0, false);
-        if ((two & 0xFFu) != ((two >> 8) & 0xFFu)) {
-            y = x / scale;
-            two = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
-        }
-        return two & 0xFFu;
-    } else {
-        float n = rintf(y);
-        if (fabsf(fabsf(y - n) - 0.5f) < 0x1p-13f) n = rintf(x / scale);
-        return (uint32_t)(int)fminf(fmaxf(n, -127.0f), 127.0f) & 0xFFu;
-    }
+        y = __builtin_copysignf(y, x);  // the remainders of -0 are +0
+        code = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false) & 0xFFu;
+    } else code = (uint32_t)(int)fminf(fmaxf(rintf(y), -127.0f), 127.0f) & 0xFFu;
+    return inverse == 0.0f ? 0u : code;
 }
 template <bool F8>
 __device__ __forceinline__ float kv8_value(uint32_t code) {
@@ -139,15 +137,31 @@ __device__ __forceinline__ size_t v_at(const Kv8Cache& c, int page, int h, int t
     return (((size_t)page * c.n_kv + h) * c.dp + d) * kPage + t;
 }
 
-// Inclusive prefix sum over the 64 lanes of a wave.
+// Inclusive prefix sum over the 64 lanes of a wave: within rows of 16 lanes, then from row to row, by DPP moves (a
+// shuffle through LDS takes ten times as long, and these sums stand before everything else a kernel does).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or_zero(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
 __device__ __forceinline__ int wave_scan(int x) {
-    const int lane = (int)(threadIdx.x & 63);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
+    x += dpp_or_zero<0x111, 0xF>(x);  // one lane up, then 2, 4, 8
+    x += dpp_or_zero<0x112, 0xF>(x);
+    x += dpp_or_zero<0x114, 0xF>(x);
+    x += dpp_or_zero<0x118, 0xF>(x);
+    x += dpp_or_zero<0x142, 0xA>(x);  // the sum of row 0 to row 1, of 2 to 3
+    x += dpp_or_zero<0x143, 0xC>(x);  // of rows 0 and 1 to 2 and 3
     return x;
+}
+// Sum over the wave, in the same order of additions everywhere.
+__device__ __forceinline__ float wave_total(float x) {
+    auto step = [&](int y) { x += __builtin_bit_cast(float, y); };
+    step(dpp_or_zero<0x111, 0xF>(__builtin_bit_cast(int, x)));
+    step(dpp_or_zero<0x112, 0xF>(__builtin_bit_cast(int, x)));
+    step(dpp_or_zero<0x114, 0xF>(__builtin_bit_cast(int, x)));
+    step(dpp_or_zero<0x118, 0xF>(__builtin_bit_cast(int, x)));
+    step(dpp_or_zero<0x142, 0xA>(__builtin_bit_cast(int, x)));
+    step(dpp_or_zero<0x143, 0xC>(__builtin_bit_cast(int, x)));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 
 // The sequence that work item `idx` belongs to, where a sequence has count(its tables) >= 0 of them; in *rest the item's

@@ -286,8 +286,7 @@ __device__ __forceinline__ SeqCut find_cut(const Kv8Batch& b, const Kv8Attn& a, 
         w = seq_work(q, a, rows, all);
         total += (float)w.tiles * (float)w.pages;
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
+    total = wave_total(total);
     const int size = max((int)__builtin_ceilf(total * (float)n_kv / (float)target), kStepWaves);
     SeqCut r;
     r.s = -1;

@@ -323,7 +323,7 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8Cache c, Kv8Batch b, Kv8At
                                                    float* __restrict__ lse, const float* __restrict__ scratch, int target,
                                                    int whole_pages, int max_tiles) {
     __shared__ __align__(16) float part[1024 / DP][DP];
-    const int lane = threadIdx.x & 63;
+    __shared__ float part_m[1024 / DP], part_l[1024 / DP];
     const int rt = blockIdx.x % max_tiles, h = blockIdx.x / max_tiles % c.n_kv, s = blockIdx.x / max_tiles / c.n_kv;
     const int r = blockIdx.y, r_all = rt * ROWS + r;
     const SeqCut cut = find_cut(b, a, c.n_kv, ROWS, target, whole_pages, false, s, 0);
@@ -331,34 +331,59 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8Cache c, Kv8Batch b, Kv8At
     const int parts = cut.parts;
     if (r_all >= q.n * a.group || parts == 1) return;
     const float* first = scratch + (size_t)(cut.first + (h * cut.work.tiles + rt) * parts) * kPieceFloats<DP, ROWS>;
-    auto max_of = [&](int k) { return first[(size_t)k * kPieceFloats<DP, ROWS> + ROWS * DP + 2 * r]; };
-    auto sum_of = [&](int k) { return first[(size_t)k * kPieceFloats<DP, ROWS> + ROWS * DP + 2 * r + 1]; };
-    float m = kNoMax;
-    for (int k = lane; k < parts; k += 64) m = fmaxf(m, max_of(k));
-    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-    float l = 0.0f;
-    for (int k = lane; k < parts; k += 64) l += sum_of(k) * __builtin_amdgcn_exp2f(max_of(k) - m);
-    for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
-    const size_t out = (size_t)(q.r0 + r_all / a.group) * a.n_head + h * a.group + r_all % a.group;
-    if (lse && threadIdx.x == 0)
-        lse[out] = l == 0.0f ? -__builtin_inff() : (__builtin_amdgcn_logf(l) + m - (float)kBias) * kLn2;
-    // four columns to a thread; the threads that share them take every kGroups-th piece
+    // four columns to a thread; the threads that share them take every kGroups-th piece, each with its own maximum
     constexpr int kFours = DP / 4, kGroups = 256 / kFours;
     const int d4 = threadIdx.x % kFours, group = threadIdx.x / kFours;
-    f4 x = f4{0, 0, 0, 0};
     if (group < kGroups) {
-#pragma unroll 4
-        for (int k = group; k < parts; k += kGroups)
-            x += *reinterpret_cast<const f4*>(first + (size_t)k * kPieceFloats<DP, ROWS> + r * DP + 4 * d4) * __builtin_amdgcn_exp2f(max_of(k) - m);
+        float m = kNoMax, l = 0.0f;
+        f4 x = f4{0, 0, 0, 0};
+        constexpr int kAhead = 4;  // pieces asked for at once
+        for (int k0 = group; k0 < parts; k0 += kAhead * kGroups) {
+            float2 ml[kAhead];
+            f4 y[kAhead];
+#pragma unroll
+            for (int n = 0; n < kAhead; ++n) {
+                const int k = k0 + n * kGroups;
+                const float* piece = first + (size_t)min(k, parts - 1) * kPieceFloats<DP, ROWS>;
+                ml[n] = *reinterpret_cast<const float2*>(piece + ROWS * DP + 2 * r);
+                y[n] = *reinterpret_cast<const f4*>(piece + r * DP + 4 * d4);
+                if (k >= parts) ml[n] = make_float2(kNoMax, 0.0f);
+            }
+            float most = m;
+#pragma unroll
+            for (int n = 0; n < kAhead; ++n) most = fmaxf(most, ml[n].x);
+            const float old = __builtin_amdgcn_exp2f(m - most);
+            l *= old;
+            x *= old;
+#pragma unroll
+            for (int n = 0; n < kAhead; ++n) {
+                const float f = __builtin_amdgcn_exp2f(ml[n].x - most);
+                l = __builtin_fmaf(ml[n].y, f, l);
+                if (k0 + n * kGroups < parts) x += y[n] * f;
+            }
+            m = most;
+        }
         *reinterpret_cast<f4*>(&part[group][4 * d4]) = x;
+        if (d4 == 0) {
+            part_m[group] = m;
+            part_l[group] = l;
+        }
     }
     __syncthreads();
+    float m = kNoMax, l = 0.0f, y = 0.0f;
     const int d = threadIdx.x;
     if (d >= c.dim) return;
-    float y = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kGroups; ++k) y += part[k][d];
+    for (int k = 0; k < kGroups; ++k) m = fmaxf(m, part_m[k]);
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+        const float f = __builtin_amdgcn_exp2f(part_m[k] - m);
+        l = __builtin_fmaf(part_l[k], f, l);
+        y = __builtin_fmaf(part[k][d], f, y);
+    }
+    const size_t out = (size_t)(q.r0 + r_all / a.group) * a.n_head + h * a.group + r_all % a.group;
     dst[out * c.dim + d] = l == 0.0f ? 0.0f : y / l;
+    if (lse && d == 0) lse[out] = l == 0.0f ? -__builtin_inff() : (__builtin_amdgcn_logf(l) + m - (float)kBias) * kLn2;
 }
 
 // Query rows of a workgroup: 8 where no sequence has more.

@@ -295,6 +295,26 @@ def test_write_of_extreme_values(be, type_, value):
 
 
 @gpu
+@pytest.mark.parametrize("type_", TYPES)
+def test_write_codes_next_to_the_rounding_borders(be, type_):
+    """Values one ulp either side of, and on, the middle between two codes, for scales of any mantissa and size."""
+    rng = np.random.default_rng(34)
+    n, dim = 16 * 60, 256
+    c = orc.Cache(n // 64, 1, dim, 1, type_, 16)
+    scale = (np.exp2(rng.uniform(-60, 60, n // 16)) * np.where(rng.random(n // 16) < 0.2, 1, rng.uniform(1, 2, n // 16))).astype(np.float32)
+    codes = np.arange(0, 127) if type_ == "i8" else np.unique(np.abs(np.nan_to_num(c.decode(np.arange(256, dtype=np.uint8)))))
+    middle = ((codes[1:] + codes[:-1]) / 2).astype(np.float32)
+    x = (rng.choice(middle, (n // 16, 16, dim)) * scale[:, None, None]).astype(np.float32)
+    x = (x.view(np.int32) + rng.integers(-2, 3, x.shape)).astype(np.int32).view(np.float32) * rng.choice([-1, 1], x.shape).astype(np.float32)
+    x[:, rng.integers(0, 16), rng.integers(0, dim)] = scale * orc.CODE_MAX[type_]
+    b = orc.Batch([n], [n], [list(range(n // 64))])
+    dev = Dev(be, c)
+    dev.write(b, x.reshape(n, dim), x[::-1].reshape(n, dim))
+    orc.write(c, b, x.reshape(n, dim), x[::-1].reshape(n, dim))
+    assert_same_cache(dev.pull(), c)
+
+
+@gpu
 def test_write_leaves_alone_what_wrong_tables_name(be):
     rng = np.random.default_rng(8)
     c = orc.Cache(6, 2, 32, 3, "i8", 16, 0x3C)
