@@ -291,13 +291,18 @@ int infr_hip_embed_gather(infr_hip_t *be, int dtype, const infr_hip_buffer_t *ta
  *   lens    [n_seq]      tokens sequence s has in the cache, this call's rows among them: row i of n is token
  *                        len - n + i
  *   pages   [n_seq][max_pages]  page of token t is pages[s][t / 64]; entries behind the last token are not read
- *   pos     [rows]       position of each row; along a sequence's tokens positions ascend strictly
- *   slots   [n_seq]      tail slot of each sequence (WriteKv8), one sequence's own as long as it lives
- * Sequences may share pages that none of them writes in the call. `max_q` bounds the rows of one sequence.
+ *   pos     [rows]       position of each row: not negative, and ascending strictly along a sequence's tokens
+ *   slots   [n_seq]      tail slot of each sequence (WriteKv8), one sequence's own as long as it lives. A sequence that
+ *                        begins with a partly filled block another one wrote has its slot's tags set to -1 first
+ * Sequences may share pages that none of them writes in the call; a page that a call writes stands once in its tables.
+ * `max_q` bounds the rows of one sequence.
  * Nothing outside the buffers is touched whatever the tables hold. A sequence whose tables contradict each other
  * or the shapes (len < n, n > max_q, q_start outside [0, rows], len > 64 max_pages) gets nothing written, and its rows
- * (up to max_q of them) read as NaN. Tokens on a page outside [0, n_pages) are not written and have no sums; rows of a
- * sequence that has such tokens read as NaN, and EvictKv8 leaves the sequence as it is. */
+ * (up to max_q of them) read as NaN. Tokens on a page outside [0, n_pages) are not written and have no sums; rows whose
+ * window reaches the page read as NaN (others may), and EvictKv8 leaves the sequence as it is.
+ * Limits, above which INFR_HIP_ERR_UNSUPPORTED: n_pages 2^28, n_kv 4096, n_slots 2^24, n_seq 65535, max_pages 65535 (4194240
+ * tokens), rows 2^28, n_head 65535, max_q * n_head / n_kv 65535 * 128, n_seq * n_kv * ceil(max_q * n_head / n_kv / 128)
+ * 2^22, keep 65535 * 64. */
 typedef struct {
     /* the cache */
     uint32_t n_pages, n_kv, head_dim /* 1..256 */, n_slots, block;
@@ -365,9 +370,9 @@ int infr_hip_score_kv8(infr_hip_t *be, const infr_hip_kv8_params_t *p, const inf
 
 /* EvictKv8: cuts each sequence down to `keep` tokens per KV head: the first `sink`, the last `recent` and, of those
  * between, the ones with the largest sums (equal sums: the earlier token), in their order, on the pages pages_out
- * [n_seq][ceil(keep / 64)], with their positions and sums. pages_out must not name a page that the call reads. A block
+ * [n_seq][ceil(keep / 64)], with their positions and sums. pages_out must name no page twice and none that the call reads. A block
  * whose tokens come whole and in place from one block keeps its codes; others are quantized again from their cached
- * values. lens_out[s] (i32) is the new length, -1 for a sequence whose tables are wrong (nothing of it is written);
+ * values. A tail of what was on those pages before loses its tag. lens_out[s] (i32) is the new length, -1 for a sequence whose tables are wrong (nothing of it is written);
  * kept (i32 [n_seq][n_kv][keep]) the tokens that stayed, -1 behind the last. Operands cache, pages, lens, pages_out,
  * lens_out, kept; params the cache's, n_seq, max_pages, keep, sink, recent. */
 int infr_hip_evict_kv8(infr_hip_t *be, const infr_hip_kv8_params_t *p, const infr_hip_kv8_operands_t *o);
@@ -432,7 +437,8 @@ int infr_hip_compile(infr_hip_t *be, const infr_hip_op_t *ops, size_t n_ops, inf
 void infr_hip_plan_free(infr_hip_t *be, infr_hip_plan_t *plan);
 /* Backend::execute: bindings[i] is the buffer bound to tensor id i (NULL = unbound;
  * Bindings, backend.rs:448-483). With the same bindings as the previous call on this plan the
- * recorded launch sequence is replayed (Capabilities::decode_replay, backend.rs:155-159).
+ * recorded launch sequence is replayed (Capabilities::decode_replay, backend.rs:155-159); a plan of one or two
+ * launches issues them again instead, which takes less time.
  * Asynchronous: results are visible after infr_hip_sync or a download. */
 int infr_hip_execute(infr_hip_t *be, infr_hip_plan_t *plan, infr_hip_buffer_t *const *bindings,
                      size_t n_bindings);

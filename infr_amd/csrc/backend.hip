@@ -501,13 +501,14 @@ static const char* kv8_shape(int kind, const infr_hip_kv8_params_t& p) {
     infr_hip_kv8_layout_t l;
     if (const char* msg = kv8_layout(p, &l)) return msg;
     if (p.n_seq == 0 || p.n_seq > 65535) return "n_seq is not 1..65535";
-    if (p.max_pages == 0 || p.max_pages > 0x7FFFFFFFu / infr::kPage) return "max_pages out of range";
+    // (grids have pages of a sequence, sequences and row tiles in their 16-bit dimensions; tokens stay far inside 32 bits)
+    if (p.max_pages == 0 || p.max_pages > 65535) return "max_pages is not 1..65535";
     if (kind == INFR_OP_EVICT_KV8) {
-        if (p.keep == 0 || p.keep > 0x7FFFFFFFu - infr::kPage) return "keep out of range";
+        if (p.keep == 0 || p.keep > 65535u * infr::kPage) return "keep out of range";
         if ((uint64_t)p.sink + p.recent > p.keep) return "sink + recent exceeds keep";
         return nullptr;
     }
-    if (p.rows == 0 || p.rows > 0x7FFFFFFFu || p.max_q == 0 || p.max_q > p.rows) return "rows or max_q out of range";
+    if (p.rows == 0 || p.rows > (1u << 28) || p.max_q == 0 || p.max_q > p.rows) return "rows or max_q out of range";
     if (kind == INFR_OP_WRITE_KV8) {
         const uint32_t width = p.n_kv * p.head_dim;
         if (p.n_slots == 0) return "a cache that is written needs tail slots";
@@ -515,7 +516,9 @@ static const char* kv8_shape(int kind, const infr_hip_kv8_params_t& p) {
         return nullptr;
     }
     if (p.n_head == 0 || p.n_head > 65535 || p.n_head % p.n_kv != 0) return "n_head is not a multiple of n_kv";
-    if ((uint64_t)p.max_q * (p.n_head / p.n_kv) > 0x7FFFFFFFu) return "max_q out of range";
+    const uint64_t tiles = ((uint64_t)p.max_q * (p.n_head / p.n_kv) + 127) / 128;  // of the form for many rows
+    if (tiles > 65535) return "max_q out of range";
+    if ((uint64_t)p.n_seq * p.n_kv * tiles > (1u << 22)) return "n_seq times n_kv times row tiles of max_q out of range";
     if (p.x_stride && p.x_stride < (uint64_t)p.n_head * p.head_dim) return "row stride below a row's length";
     if (!(p.softcap >= 0.0f) || p.softcap > 3.0e38f || !(p.scale >= -3.0e38f && p.scale <= 3.0e38f)) return "scale or softcap out of range";
     if (p.window > 0x7FFFFFFFu) return "window out of range";

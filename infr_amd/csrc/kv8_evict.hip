@@ -222,6 +222,13 @@ __global__ __launch_bounds__(kMove) void evict_move_kernel(Kv8Cache c, Kv8Evict 
     const int j = t < room ? kept[t] : -1, j0 = lead < room ? kept[lead] : -1;
     const bool live = j >= 0;
     if (tid < kPage) amax[tid] = 0;
+    // a tail that holds rows of what was on this page before does not hold those that come now
+    if (kept[0] >= 0)
+        for (int i = tid; i < c.n_slots; i += kMove) {
+            int32_t* tag = c.tag + (((size_t)i * c.n_kv + h) * 2 + (is_v ? 1 : 0)) * 2;
+            const int block = tag[0];
+            if (block >= 0 && block / subs == to) tag[0] = -1;
+        }
     // amax's top bit marks a block that has to be quantized again
     const bool in_place = !live || (j == j0 + t % c.block && j0 % c.block == 0);
     __syncthreads();

@@ -296,6 +296,9 @@ def evict(c, b_pages, lens, pages_out, keep, sink, recent):
                 order.sort(key=lambda t: (0 if np.isnan(mass[t]) else 1, 0.0 if np.isnan(mass[t]) else -mass[t], t))
                 src = np.sort(np.concatenate([np.flatnonzero(must), np.array(order[:keep - sink - recent], int)]))
             kept[s, h, :n_out] = src
+            for page in pages_out[s, :-(-n_out // PAGE)]:  # tails of what was on the new pages before
+                tag = c.tag[:, h, :, 0]
+                tag[(tag >= 0) & (tag // (PAGE // c.block) == page)] = -1
             for t0 in range(0, n_out, c.block):
                 to, at = int(pages_out[s, t0 // PAGE]), t0 % PAGE
                 toks = src[t0:t0 + c.block]

@@ -146,7 +146,8 @@ def write_op(**kw):
     (dict(dtype=DType.Q8_0), "dtype"), (dict(n_pages=0), "n_pages"), (dict(n_kv=0), "n_kv"), (dict(n_kv=5000), "n_kv"),
     (dict(n_slots=0), "tail slots"), (dict(rows=0), "rows"), (dict(max_q=0), "max_q"), (dict(max_q=4), "max_q"),
     (dict(n_seq=0), "n_seq"), (dict(n_seq=70000), "n_seq"), (dict(max_pages=0), "max_pages"),
-    (dict(max_pages=1 << 26), "max_pages"), (dict(k_stride=127), "stride"), (dict(v_stride=1), "stride")])
+    (dict(max_pages=1 << 26), "max_pages"), (dict(max_pages=65536), "max_pages"), (dict(rows=(1 << 28) + 1), "rows"),
+    (dict(k_stride=127), "stride"), (dict(v_stride=1), "stride")])
 def test_write_refuses(kw, word):
     assert kv8_supported(write_op()) is None
     assert word in kv8_supported(write_op(**kw))
@@ -166,7 +167,16 @@ def test_attention_and_score_refuse(kind, kw, word):
         assert "decay" in kv8_supported(op(decay=math.nan))
 
 
-@pytest.mark.parametrize("kw,word", [(dict(keep=0), "keep"), (dict(sink=40, recent=25), "exceeds"), (dict(keep=0x7FFFFFFF), "keep"),
+@pytest.mark.parametrize("kind", [AttentionKv8, ScoreKv8])
+@pytest.mark.parametrize("n_kv,n_head,n_seq,max_q,word", [
+    (2, 4, 1, 65535 * 64, None), (2, 4, 1, 65535 * 64 + 1, "max_q"), (4096, 4096, 1024, 128, None), (4096, 4096, 1024, 129, "row tiles"),
+    (4096, 4096, 1025, 1, "row tiles"), (1, 65535, 65535, 1, "row tiles"), (64, 64, 65535, 1, None)])
+def test_calls_larger_than_a_launch_are_refused(kind, n_kv, n_head, n_seq, max_q, word):
+    why = kv8_supported(kind(*[None] * 7, Kv8(4, n_kv, 64, 1), Kv8Batch(1 << 28, n_seq, max_q, 65535), n_head=n_head))
+    assert why is None if word is None else word in why
+
+
+@pytest.mark.parametrize("kw,word", [(dict(keep=0), "keep"), (dict(keep=65535 * 64 + 1), "keep"), (dict(sink=40, recent=25), "exceeds"), (dict(keep=0x7FFFFFFF), "keep"),
                                      (dict(sink=0xFFFFFFFF, recent=2), "exceeds")])
 def test_evict_refuses(kw, word):
     def op(**k):
@@ -648,6 +658,30 @@ def test_evict(be, type_, block, dim, keep, sink, recent):
         c.sums[p] = rng.random((len(p), 2, 64)) ** 4
     out = [free[s * n_out:(s + 1) * n_out].tolist() for s in range(len(lens))]
     check_evict(be, c, pages, lens, out, keep, sink, recent)
+
+
+@gpu
+@pytest.mark.parametrize("type_", TYPES)
+def test_evict_there_and_back_leaves_no_stale_tail(be, type_):
+    """A sequence moves to other pages and back to its first ones, with other tokens, before it goes on: the tail's tag
+    then names the block that is open, but its rows are not that block's. A bystander's tail stays."""
+    rng = np.random.default_rng(25)
+    c, pages, free = filled(rng, type_, 32, 2, 40, (75, 90), spare=4)
+    old = [[int(x) for x in p] for p in pages]
+    for p in pages:
+        c.sums[p] = rng.random((len(p), 2, 64))
+    there = [[int(free[0]), int(free[1])]]
+    before = c.tag.copy()
+    assert before[0, 0, 0, 0] == old[0][1] * 2 and before[0, 0, 0, 1] == 11
+    check_evict(be, c, old[:1], (75,), there, 74, 2, 3)
+    check_evict(be, c, there, (74,), [old[0]], 73, 2, 3)
+    assert (c.tag[0, :, :, 0] == -1).all() and np.array_equal(c.tag[1], before[1])
+    b = orc.Batch([1, 1], [74, 91], old, slots=[0, 1], pos=[75, 90])
+    k, v = rows_of(rng, b, c)
+    dev = Dev(be, c)
+    dev.write(b, k, v)
+    orc.write(c, b, k, v)
+    assert_same_cache(dev.pull(), c)
 
 
 @gpu
