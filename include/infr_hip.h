@@ -272,8 +272,8 @@ int infr_hip_embed_gather(infr_hip_t *be, int dtype, const infr_hip_buffer_t *ta
  *
  * The cache is ONE buffer of `n_pages` pages of 64 tokens, each page for all `n_kv` KV heads. Keys and values
  * are 8-bit codes; `block` (16, 32 or 64) tokens of one head share an f32 scale:
- *   I8       scale = max(amax / 127, 2^-96), code = x / scale to the nearest, ties to even
- *   F8_E4M3  scale = max(amax / 448, 2^-96), code = e4m3(x / scale), to the nearest, ties to even
+ *   I8       scale = max(amax * f32(1 / 127), 2^-96), code = x / scale to the nearest, ties to even
+ *   F8_E4M3  scale = max(amax * f32(1 / 448), 2^-96), code = e4m3(x / scale), to the nearest, ties to even
  * A block that holds a value which is not finite has the scale NaN and zero codes: what sees any of its tokens
  * is NaN. infr_hip_kv8_layout gives the parts' offsets; with DP = head_dim rounded up to 64 they are
  *   k        u8  [n_pages][n_kv][DP / 64][64 tokens][64]
@@ -346,7 +346,8 @@ int infr_hip_kv8_layout(const infr_hip_kv8_params_t *p, infr_hip_kv8_layout_t *o
 int infr_hip_kv8_supported(int kind, const infr_hip_kv8_params_t *p, const char **why);
 
 /* WriteKv8: rows x (K) and v, f32 [rows][n_kv * head_dim], become tokens of the cache, with their positions and
- * sums of 0. Operands x, v, cache, pos, pages, q_start, lens, slots. The codes of a block are those of all its tokens
+ * sums of 0; slots of a page behind a sequence's last token keep what they hold. Operands x, v, cache, pos, pages, q_start,
+ * lens, slots. The codes of a block are those of all its tokens
  * quantized at once, however many calls they came in; tokens of a block whose rows the tail has no longer (the
  * sequence was cut back behind a block that had closed, or moved to other pages) count at their cached values. */
 int infr_hip_write_kv8(infr_hip_t *be, const infr_hip_kv8_params_t *p, const infr_hip_kv8_operands_t *o);

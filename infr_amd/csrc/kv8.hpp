@@ -96,10 +96,11 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Batch& b, int s) {
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
 
-// Scale of a block from the largest absolute value's bits; a value that is not finite makes it NaN.
+// Scale of a block from the largest absolute value's bits, by one multiplication with the reciprocal that is nearest in
+// f32; a value that is not finite makes it NaN.
 __device__ __forceinline__ float kv8_scale(uint32_t amax_bits, bool f8) {
     if (amax_bits >= 0x7F800000u) return __builtin_nanf("");
-    return fmaxf(__builtin_bit_cast(float, amax_bits) / (f8 ? 448.0f : 127.0f), kMinScale);
+    return fmaxf(__builtin_bit_cast(float, amax_bits) * (f8 ? 1.0f / 448.0f : 1.0f / 127.0f), kMinScale);
 }
 // 1 / scale for kv8_code; 0 for a NaN scale, whose codes are 0.
 __device__ __forceinline__ float kv8_inverse(float scale) {
@@ -110,7 +111,7 @@ __device__ __forceinline__ float kv8_inverse(float scale) {
 // Nearest code of x / scale, ties to even. The quotient is the correctly rounded one: x times the inverse, corrected twice
 // by its remainder, which a fused multiply-add gives exactly (Markstein's division; scales and codes keep every number in
 // it clear of overflow and of what the remainder could lose). It stays below the largest code's rounding border: the scale
-// is amax / code_max rounded once and the quotient once more.
+// is within 2^-23 of amax / code_max and the quotient is rounded once more.
 template <bool F8>
 __device__ __forceinline__ uint32_t kv8_code(float x, float scale, float inverse) {
     float y = x * inverse;

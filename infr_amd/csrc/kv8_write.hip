@@ -98,6 +98,14 @@ __global__ __launch_bounds__(kThreads) void write_kv8_kernel(Kv8Cache c, Kv8Batc
                     r[j][e] = kv8_value<F8>((is_v ? c.v : c.k)[at]) * old_scale;
                 }
             }
+    // value codes go out in segments: 16 tokens of one column to a thread. Blocks are whole 16s, so a segment is written or
+    // left, but for the codes behind the sequence's end in the last one, which are put back as they were.
+    const int vd = tid >> 2, vt = (tid & 3) * 16, seg = (pi * kPage + vt) / c.block;
+    const int seg_n = seg >= slot0 / c.block ? q.len - pi * kPage - vt : 0;
+    uint4 was[kGroups];
+    if (is_v && page_ok && seg_n > 0 && seg_n < 16)
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) was[j] = *reinterpret_cast<const uint4*>(c.v + v_at(c, page, h, vt, j * 64 + vd));
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < kGroups; ++j)
@@ -117,19 +125,23 @@ __global__ __launch_bounds__(kThreads) void write_kv8_kernel(Kv8Cache c, Kv8Batc
 #pragma unroll
         for (int e = 0; e < 16; ++e) w[e / 4] |= kv8_code<F8>(r[j][e], scale, inverse) << (8 * (e % 4));
         if (!is_v) {
-            if (touched) *reinterpret_cast<uint4*>(c.k + k_at(c, page, h, t, j * 64 + col)) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (is_new || is_old) *reinterpret_cast<uint4*>(c.k + k_at(c, page, h, t, j * 64 + col)) = make_uint4(w[0], w[1], w[2], w[3]);
             continue;
         }
         __syncthreads();  // (page_ok is the workgroup's)
 #pragma unroll
         for (int e = 0; e < 16; ++e) turn[(col + e) * kTurn + t] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
         __syncthreads();
-        // thread -> 16 tokens of one column; blocks are whole 16s, so a segment is written or left as a whole
-        const int d = tid >> 2, t0 = (tid & 3) * 16;
-        const int first = (pi * kPage + t0) / c.block;
-        if (first >= slot0 / c.block && first <= (q.len - 1) / c.block) {
-            const uint32_t* src = reinterpret_cast<const uint32_t*>(turn + d * kTurn + t0);
-            *reinterpret_cast<uint4*>(c.v + v_at(c, page, h, t0, j * 64 + d)) = make_uint4(src[0], src[1], src[2], src[3]);
+        if (seg_n > 0) {
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(turn + vd * kTurn + vt);
+            uint4 y = make_uint4(src[0], src[1], src[2], src[3]);
+            if (seg_n < 16) {
+                auto below = [&](int n) { return n >= 4 ? 0xFFFFFFFFu : n > 0 ? (1u << (8 * n)) - 1u : 0u; };
+                auto put = [&](uint32_t x, uint32_t old, int n) { return (x & below(n)) | (old & ~below(n)); };
+                y = make_uint4(put(y.x, was[j].x, seg_n), put(y.y, was[j].y, seg_n - 4), put(y.z, was[j].z, seg_n - 8),
+                               put(y.w, was[j].w, seg_n - 12));
+            }
+            *reinterpret_cast<uint4*>(c.v + v_at(c, page, h, vt, j * 64 + vd)) = y;
         }
     }
     if (!is_v && page_ok && is_new && (tid & 3) == 0) {

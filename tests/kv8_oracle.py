@@ -49,7 +49,7 @@ class Cache:
         if bits.size and bits.max() >= 0x7F800000:
             return np.float32(np.nan), np.zeros(x.shape, np.uint8)
         amax = bits.max().view(np.float32) if bits.size else np.float32(0)
-        scale = max(np.float32(amax / CODE_MAX[self.type]), np.float32(2.0 ** -96))
+        scale = max(np.float32(amax * (np.float32(1) / CODE_MAX[self.type])), np.float32(2.0 ** -96))
         y = (x / scale).astype(np.float32)
         if self.type == "i8":
             return scale, np.rint(y).clip(-127, 127).astype(np.int8).view(np.uint8)
@@ -146,9 +146,9 @@ def write(c, b, k, v):
                         continue
                     scale, codes = c.quantize(np.stack([rows[t] for t in toks]))
                     c.scale_of(part)[page, h, t0 % PAGE // c.block] = scale
-                    for i in range(c.block):
-                        c.put_codes(part, page, h, t0 % PAGE + i, codes[i] if i < len(toks) else 0)
-                        if part == "k" and i < len(toks) and t0 + i >= begin:
+                    for i in range(len(toks)):
+                        c.put_codes(part, page, h, t0 % PAGE + i, codes[i])
+                        if part == "k" and t0 + i >= begin:
                             c.pos[page, h, t0 % PAGE + i] = b.pos[r0 + t0 + i - begin]
                             c.sums[page, h, t0 % PAGE + i] = 0
                 if slot_ok:
