@@ -18,6 +18,8 @@
 //   Error                    error.rs:5-25         Error (ErrorKind mirrors the enum; where the
 //                                                  reference panics on a programmer error this
 //                                                  throws ErrorKind::Invalid instead)
+//   (none: the reference keeps its KV cache and    Kv8, Kv8Batch, op::WriteKv8, op::AttentionKv8,
+//    attention on another backend)                 op::ScoreKv8, op::EvictKv8
 //   trait Backend            backend.rs:486-662    HipBackend: name, capabilities, alloc,
 //                                                  alloc_uninit, upload, download, copy_buffer,
 //                                                  compile, execute, sync
@@ -27,6 +29,7 @@
 #ifndef INFR_HIP_HPP
 #define INFR_HIP_HPP
 
+#include <cmath>
 #include <cstdint>
 #include <cstring>
 #include <optional>
@@ -46,7 +49,7 @@ enum class DType : int {
     Q5_0 = INFR_DTYPE_Q5_0, Q5_1 = INFR_DTYPE_Q5_1, Q8_0 = INFR_DTYPE_Q8_0, Q2K = INFR_DTYPE_Q2_K,
     Q3K = INFR_DTYPE_Q3_K, Q4K = INFR_DTYPE_Q4_K,
     Q5K = INFR_DTYPE_Q5_K, Q6K = INFR_DTYPE_Q6_K, IQ4NL = INFR_DTYPE_IQ4_NL, IQ4XS = INFR_DTYPE_IQ4_XS, TQ1_0 = INFR_DTYPE_TQ1_0, TQ2_0 = INFR_DTYPE_TQ2_0, MXFP4 = INFR_DTYPE_MXFP4, NVFP4 = INFR_DTYPE_NVFP4, I32 = 26,
-    BF16 = INFR_DTYPE_BF16, Q2_0 = INFR_DTYPE_Q2_0,
+    BF16 = INFR_DTYPE_BF16, Q2_0 = INFR_DTYPE_Q2_0, I8 = INFR_DTYPE_I8, F8E4M3 = INFR_DTYPE_F8_E4M3,
 };
 
 inline const char* dtype_name(DType d) {
@@ -72,6 +75,8 @@ inline const char* dtype_name(DType d) {
     case DType::I32: return "I32";
     case DType::BF16: return "BF16";
     case DType::Q2_0: return "Q2_0";
+    case DType::I8: return "I8";
+    case DType::F8E4M3: return "F8E4M3";
     }
     return "?";
 }
@@ -79,6 +84,7 @@ inline const char* dtype_name(DType d) {
 // (elements, bytes) of one block; crates/infr-core/src/decode_spec.rs:255-381.
 inline std::pair<size_t, size_t> block_layout(DType d) {
     if (d == DType::I32) return {1, 4};
+    if (d == DType::I8 || d == DType::F8E4M3) return {1, 1};
     int e = 0, b = 0;
     if (!infr_block_layout((int)d, &e, &b)) throw std::invalid_argument("unknown dtype");
     return {(size_t)e, (size_t)b};
@@ -130,6 +136,29 @@ enum class Activation : int { Silu = INFR_ACT_SILU, Gelu = INFR_ACT_GELU, Sigmoi
 // crates/infr-core/src/graph.rs:76-85
 enum class MoeGating : int { Softmax = INFR_GATING_SOFTMAX, Sigmoid = INFR_GATING_SIGMOID, SqrtSoftplus = INFR_GATING_SQRT_SOFTPLUS };
 
+// Geometry of an 8-bit KV cache (infr_hip.h): pages of 64 tokens, `block` tokens of a head to a scale.
+struct Kv8 {
+    uint32_t n_pages, n_kv, head_dim, n_slots;
+    DType dtype = DType::I8;
+    uint32_t block = 16;
+    infr_hip_kv8_params_t params() const {
+        infr_hip_kv8_params_t p{};
+        p.n_pages = n_pages; p.n_kv = n_kv; p.head_dim = head_dim; p.n_slots = n_slots;
+        p.block = block; p.dtype = (int)dtype;
+        return p;
+    }
+    // byte offsets of the cache buffer's parts, and its size
+    infr_hip_kv8_layout_t layout() const {
+        infr_hip_kv8_layout_t out{};
+        const infr_hip_kv8_params_t p = params();
+        if (const int rc = infr_hip_kv8_layout(&p, &out)) throw Error((ErrorKind)rc, "kv8: geometry is not supported");
+        return out;
+    }
+    size_t nbytes() const { return layout().bytes; }
+};
+// Shape of a call's batch: rows in all, sequences, most rows of one sequence, width of the page table.
+struct Kv8Batch { uint32_t rows, n_seq, max_q, max_pages; };
+
 namespace op {
 // graph.rs:177-191
 struct Linear { TensorId x, weight, dst; uint32_t m, in_f, out_f; uint64_t w_off = 0; };
@@ -167,10 +196,45 @@ struct GatedActFused {
 struct Add { TensorId a, b, dst; };
 // graph.rs:853-865
 struct EmbedGather { TensorId ids, table, dst; uint32_t rows, ne; float scale = 1.0f; };
+// The 8-bit KV cache (infr_hip_write_kv8 .. infr_hip_evict_kv8); offsets and strides in floats, 0: rows side by side.
+struct WriteKv8 {
+    TensorId k, v, cache, pos, pages, q_start, lens, slots;
+    Kv8 geom; Kv8Batch batch;
+    uint32_t k_off = 0, k_stride = 0, v_off = 0, v_stride = 0;
+};
+struct AttentionKv8 {
+    TensorId q, cache, dst, pos, pages, q_start, lens;
+    Kv8 geom; Kv8Batch batch;
+    uint32_t n_head;
+    std::optional<float> scale;  // none: 1 / sqrt(head_dim)
+    float softcap = 0.0f;
+    uint32_t window = 0;
+    bool causal = true;
+    std::optional<TensorId> first, prefix, slopes, lse;
+    uint32_t q_off = 0, q_stride = 0;
+};
+struct ScoreKv8 {
+    TensorId q, cache, lse, pos, pages, q_start, lens;
+    Kv8 geom; Kv8Batch batch;
+    uint32_t n_head;
+    float decay = 1.0f;
+    std::optional<float> scale;
+    float softcap = 0.0f;
+    uint32_t window = 0;
+    bool causal = true;
+    std::optional<TensorId> first, prefix, slopes;
+    uint32_t q_off = 0, q_stride = 0;
+};
+struct EvictKv8 {
+    TensorId cache, pages, lens, pages_out, lens_out, kept;
+    Kv8 geom;
+    uint32_t n_seq, max_pages, keep, sink = 0, recent = 0;
+};
 }  // namespace op
 
 using Op = std::variant<op::Linear, op::MoeFfn, op::RmsNorm, op::RmsNormAdd, op::GatedAct,
-                        op::GatedActFused, op::Add, op::EmbedGather>;
+                        op::GatedActFused, op::Add, op::EmbedGather, op::WriteKv8, op::AttentionKv8,
+                        op::ScoreKv8, op::EvictKv8>;
 
 // crates/infr-core/src/graph.rs:1317-1460: ordered op list over declared tensors.
 class Graph {
@@ -382,6 +446,46 @@ private:
         c.x = v.ids.v; c.weight = v.table.v; c.dst = v.dst.v; c.m = v.rows; c.in_f = v.ne; c.scale = v.scale;
         c.w_numel = g.desc(v.table).numel();
         c.w_dtype = (int)g.desc(v.table).dtype;
+    }
+    // what the ops of the 8-bit KV cache with a batch have in common
+    template <typename T>
+    static void fill_kv8(const T& v, infr_hip_op_t& c) {
+        c.kv = v.geom.params();
+        c.kv.rows = v.batch.rows; c.kv.n_seq = v.batch.n_seq; c.kv.max_q = v.batch.max_q; c.kv.max_pages = v.batch.max_pages;
+        c.kv_cache = v.cache.v; c.kv_pos = v.pos.v; c.kv_pages = v.pages.v; c.kv_q_start = v.q_start.v; c.kv_lens = v.lens.v;
+    }
+    template <typename T>
+    static void fill_kv8_attn(const T& v, infr_hip_op_t& c) {
+        fill_kv8(v, c);
+        c.x = v.q.v; c.kv.x_off = v.q_off; c.kv.x_stride = v.q_stride; c.kv.n_head = v.n_head;
+        c.kv.scale = v.scale ? *v.scale : (float)(1.0 / std::sqrt((double)v.geom.head_dim));
+        c.kv.softcap = v.softcap; c.kv.window = v.window; c.kv.causal = v.causal;
+        c.kv.has_first = v.first.has_value(); c.kv_first = v.first ? v.first->v : 0;
+        c.kv.has_prefix = v.prefix.has_value(); c.kv_prefix = v.prefix ? v.prefix->v : 0;
+        c.kv.has_slopes = v.slopes.has_value(); c.kv_slopes = v.slopes ? v.slopes->v : 0;
+    }
+    static void fill(const Graph&, const op::WriteKv8& v, infr_hip_op_t& c) {
+        c.kind = INFR_OP_WRITE_KV8;
+        fill_kv8(v, c);
+        c.x = v.k.v; c.kv_v = v.v.v; c.kv_slots = v.slots.v;
+        c.kv.x_off = v.k_off; c.kv.x_stride = v.k_stride; c.kv.v_off = v.v_off; c.kv.v_stride = v.v_stride;
+    }
+    static void fill(const Graph&, const op::AttentionKv8& v, infr_hip_op_t& c) {
+        c.kind = INFR_OP_ATTENTION_KV8;
+        fill_kv8_attn(v, c);
+        c.dst = v.dst.v; c.kv.has_lse = v.lse.has_value(); c.kv_lse = v.lse ? v.lse->v : 0;
+    }
+    static void fill(const Graph&, const op::ScoreKv8& v, infr_hip_op_t& c) {
+        c.kind = INFR_OP_SCORE_KV8;
+        fill_kv8_attn(v, c);
+        c.kv_lse = v.lse.v; c.kv.decay = v.decay;
+    }
+    static void fill(const Graph&, const op::EvictKv8& v, infr_hip_op_t& c) {
+        c.kind = INFR_OP_EVICT_KV8;
+        c.kv = v.geom.params();
+        c.kv.n_seq = v.n_seq; c.kv.max_pages = v.max_pages; c.kv.keep = v.keep; c.kv.sink = v.sink; c.kv.recent = v.recent;
+        c.kv_cache = v.cache.v; c.kv_pages = v.pages.v; c.kv_lens = v.lens.v;
+        c.kv_pages_out = v.pages_out.v; c.kv_lens_out = v.lens_out.v; c.kv_kept = v.kept.v;
     }
 
     infr_hip_t* h_ = nullptr;
