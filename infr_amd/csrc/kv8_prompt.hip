@@ -7,6 +7,8 @@
 // page's codes are requested before the current page is multiplied and written behind it, one barrier a page); a
 // wave's scores, softmax and output stay in its registers. Tokens are dealt to the MFMA's rows so that a lane holds
 // 16 neighbours: one block's scale, and P.V's operand as it stands.
+// With few row tiles a workgroup takes 64 rows instead, two waves to 32 of them, each with half of every page's tokens, and
+// joins their results in LDS at the end.
 // Pages no row of the workgroup sees are not visited; pages all rows of a wave see take no mask.
 #include "kv8_attn.hpp"
 #include "kv8_device.hpp"
@@ -18,12 +20,14 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kCols = 32;                // query rows of a wave
-constexpr int kRows = kCols * kWaves;    // and of a workgroup
 constexpr int kBias = 10;
 constexpr float kLag = 4.0f;
 
-template <int DP>
-constexpr int kPieceFloats = kRows * DP + 2 * kRows;
+// Waves that share 32 query rows, each with 64 / KS tokens of every page; rows of a workgroup.
+template <int KS>
+constexpr int kRows = kCols * kWaves / KS;
+template <int DP, int KS>
+constexpr int kPieceFloats = kRows<KS> * DP + 2 * kRows<KS>;
 
 // A page's first DC columns in LDS. Rows are padded by 16 bytes: neighbours then start four banks apart.
 template <int DC>
@@ -36,13 +40,15 @@ struct Stage {
 };
 
 // DC: the columns that are computed with, head_dim rounded up to 32.
-template <int DP, int DC, bool F8, bool GEN>
+template <int DP, int DC, int KS, bool F8, bool GEN>
 __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a,
                                                                             float* __restrict__ dst, float* __restrict__ lse,
                                                                             float* __restrict__ scratch, int tiles, int parts) {
     constexpr int kSteps = DC / 16;  // of the scores' sum
     constexpr int kOut = DC / 32;    // output tiles
     constexpr int kLoads = DP / 64;  // 16-byte pieces of K, and of V, that a thread brings in
+    constexpr int kHalves = 2 / KS;  // of a page that a wave takes
+    constexpr int kRows = infr::kRows<KS>;
     extern __shared__ __align__(16) unsigned char smem[];
     Stage<DC>* stage = reinterpret_cast<Stage<DC>*>(smem);
     __shared__ int first_page[kWaves], last_page[kWaves];
@@ -52,7 +58,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
     const Kv8Seq q = kv8_seq(b, s);
     const int n_rows = q.n * a.group;
     if (rt * kRows >= n_rows) return;
-    const int rr = rt * kRows + wave * kCols + col;
+    const int half0 = KS == 2 ? wave & 1 : 0;  // first of the wave's halves
+    const int rr = rt * kRows + wave / KS * kCols + col;
     const bool live = rr < n_rows;
     const int i = live ? rr / a.group : q.n - 1, head = h * a.group + (live ? rr % a.group : 0);
     const Kv8Row row = kv8_row(b, a, q, s, i, head);
@@ -205,15 +212,15 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
         const bool more = p + 1 < p1;
         if (more) fetch(p + 1);
         if (p >= w0 && p < w1) {
-            // x[t][e]: token 32 t + 16 hf + e of the page
-            f16x x[2];
+            // x[t][e]: token 32 (half0 + t) + 16 hf + e of the page
+            f16x x[kHalves];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) x[t] = (f16x)(0.0f);
+            for (int t = 0; t < kHalves; ++t) x[t] = (f16x)(0.0f);
 #pragma unroll
             for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const h8 key = *reinterpret_cast<const h8*>(&st.k[t * 32 + my_tok][k * 16 + hf * 8]);
+                for (int t = 0; t < kHalves; ++t) {
+                    const h8 key = *reinterpret_cast<const h8*>(&st.k[(half0 + t) * 32 + my_tok][k * 16 + hf * 8]);
                     x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, qh[k], x[t], 0, 0, 0);
                     x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, ql[k], x[t], 0, 0, 0);
                 }
@@ -221,13 +228,14 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
             const bool masked = (p + 1) * kPage > min(full_hi, q.len) ||
                                 (use_pos && (last_pos - st.pos[0] >= row.window || last_first > st.pos[0]));
             const bool bent = GEN && (a.softcap > 0.0f || a.slopes);
-            float high = -__builtin_inff(), factor[2], vs[2];
-            bool any[2] = {true, true};
+            float high = -__builtin_inff(), factor[kHalves], vs[kHalves];
+            bool any[kHalves];
             int e_now = -200;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                factor[t] = row_factor * st.ks[2 * t + hf];
-                vs[t] = st.vs[2 * t + hf];
+            for (int t = 0; t < kHalves; ++t) {
+                factor[t] = row_factor * st.ks[2 * (half0 + t) + hf];
+                vs[t] = st.vs[2 * (half0 + t) + hf];
+                any[t] = true;
                 if (masked || bent) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) x[t][e] *= factor[t];
@@ -237,17 +245,17 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
                 if (GEN && a.slopes)
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) {
-                        const f4 y = *reinterpret_cast<const f4*>(&st.rel[t * 32 + hf * 16 + e]);
+                        const f4 y = *reinterpret_cast<const f4*>(&st.rel[(half0 + t) * 32 + hf * 16 + e]);
 #pragma unroll
                         for (int n = 0; n < 4; ++n) x[t][e + n] = __builtin_fmaf(-row.slope, fabsf(my_rel - y[n]), x[t][e + n]);
                     }
                 if (masked) {
-                    const int tok0 = p * kPage + t * 32 + hf * 16;
+                    const int tok0 = p * kPage + (half0 + t) * 32 + hf * 16;
                     any[t] = false;
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) {
                         int4 y = make_int4(0, 0, 0, 0);
-                        if (use_pos) y = *reinterpret_cast<const int4*>(&st.pos[t * 32 + hf * 16 + e]);
+                        if (use_pos) y = *reinterpret_cast<const int4*>(&st.pos[(half0 + t) * 32 + hf * 16 + e]);
                         const int kpos[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                         for (int n = 0; n < 4; ++n) {
@@ -266,7 +274,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
             }
             if (__any(fabsf(high) > kLargeScore))
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
+                for (int t = 0; t < kHalves; ++t) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) x[t][e] *= factor[t];
                     factor[t] = 1.0f;
@@ -283,9 +291,9 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
                 v_exp = new_exp;
             }
             // weights times the values' scale in one exponential; their sum is divided by it
-            h8 wh[4], wl[4];
+            h8 wh[2 * kHalves], wl[2 * kHalves];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < kHalves; ++t) {
                 v_bad = v_bad || (any[t] && vs[t] != vs[t]);
                 const float lift = any[t] ? scale_log(vs[t], v_exp) : 0.0f, base = (float)kBias - top + lift;
                 float run = 0.0f, w[16];
@@ -306,8 +314,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
 #pragma unroll
             for (int k = 0; k < kOut; ++k)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {  // tokens 32 (t / 2) + 16 hf + 8 (t % 2) ..
-                    const h8 val = *reinterpret_cast<const h8*>(&st.v[k * 32 + col][(t / 2) * 32 + hf * 16 + (t % 2) * 8]);
+                for (int t = 0; t < 2 * kHalves; ++t) {  // tokens 32 (half0 + t / 2) + 16 hf + 8 (t % 2) ..
+                    const h8 val = *reinterpret_cast<const h8*>(&st.v[k * 32 + col][(half0 + t / 2) * 32 + hf * 16 + (t % 2) * 8]);
                     o[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(val, wh[t], o[k], 0, 0, 0);
                     o[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(val, wl[t], o[k], 0, 0, 0);
                 }
@@ -316,6 +324,34 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
         __syncthreads();
     }
     bad = __syncthreads_or(bad) != 0;
+    if constexpr (KS == 2) {  // the second halves' results join the first's, register by register, through the pages' LDS
+        float* mine = reinterpret_cast<float*>(smem) + wave / 2 * (kOut * 16 + 4) * 64 + lane;
+        if (half0 == 1) {
+#pragma unroll
+            for (int k = 0; k < kOut; ++k)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mine[(k * 16 + e) * 64] = o[k][e];
+            mine[kOut * 16 * 64] = top;
+            mine[(kOut * 16 + 1) * 64] = sum;
+            mine[(kOut * 16 + 2) * 64] = (float)v_exp;
+            mine[(kOut * 16 + 3) * 64] = v_bad ? 1.0f : 0.0f;
+        }
+        __syncthreads();
+        if (half0 == 1) return;
+        const float top2 = mine[kOut * 16 * 64], new_top = fmaxf(top, top2);
+        const int exp2 = (int)mine[(kOut * 16 + 2) * 64], new_exp = max(v_exp, exp2);
+        const float f1 = __builtin_amdgcn_exp2f(top - new_top), f2 = __builtin_amdgcn_exp2f(top2 - new_top);
+        const float o1 = v_exp == -200 ? 0.0f : f1 * __builtin_amdgcn_exp2f((float)(v_exp - new_exp));
+        const float o2 = exp2 == -200 ? 0.0f : f2 * __builtin_amdgcn_exp2f((float)(exp2 - new_exp));
+#pragma unroll
+        for (int k = 0; k < kOut; ++k)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[k][e] = __builtin_fmaf(mine[(k * 16 + e) * 64], o2, o[k][e] * o1);
+        sum = __builtin_fmaf(mine[(kOut * 16 + 1) * 64], f2, sum * f1);
+        v_bad = v_bad || mine[(kOut * 16 + 3) * 64] != 0.0f;
+        top = new_top;
+        v_exp = new_exp;
+    }
     sum = halves_sum(sum);
     if (halves_max(v_bad ? 1.0f : 0.0f) > 0.0f)
 #pragma unroll
@@ -323,8 +359,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
     if (!live) return;
     const float nan = __builtin_nanf(""), up = __builtin_amdgcn_exp2f((float)max(v_exp, -126));
     if (parts > 1) {
-        float* piece = scratch + ((((size_t)s * c.n_kv + h) * tiles + rt) * parts + part) * kPieceFloats<DP>;
-        const int r = wave * kCols + col;
+        float* piece = scratch + ((((size_t)s * c.n_kv + h) * tiles + rt) * parts + part) * kPieceFloats<DP, KS>;
+        const int r = wave / KS * kCols + col;
 #pragma unroll
         for (int k = 0; k < kOut; ++k)
 #pragma unroll
@@ -359,21 +395,22 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
 }
 
 // Joins the pieces of the rows of one (sequence, head, row tile), a wave at a time per row.
-template <int DP>
+template <int DP, int KS>
 __global__ __launch_bounds__(kThreads) void join_rows_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a, float* __restrict__ dst,
                                                              float* __restrict__ lse, const float* __restrict__ scratch,
                                                              int tiles, int parts) {
+    constexpr int kRows = infr::kRows<KS>;
     const int lane = threadIdx.x & 63;
     const int rt = blockIdx.x % tiles, h = blockIdx.x / tiles % c.n_kv, s = blockIdx.x / tiles / c.n_kv;
     const int r = (int)blockIdx.y * kWaves + ((int)threadIdx.x >> 6), r_all = rt * kRows + r;
     const Kv8Seq q = kv8_seq(b, s);
     if (r_all >= q.n * a.group) return;
-    const float* first = scratch + (((size_t)s * c.n_kv + h) * tiles + rt) * parts * kPieceFloats<DP>;
+    const float* first = scratch + (((size_t)s * c.n_kv + h) * tiles + rt) * parts * kPieceFloats<DP, KS>;
     float m = kNoMax, l = 0.0f;
-    for (int k = 0; k < parts; ++k) m = fmaxf(m, first[(size_t)k * kPieceFloats<DP> + kRows * DP + r]);
+    for (int k = 0; k < parts; ++k) m = fmaxf(m, first[(size_t)k * kPieceFloats<DP, KS> + kRows * DP + r]);
     float x[DP / 64] = {};  // (columns behind head_dim are whatever the scratch held; they are not stored)
     for (int k = 0; k < parts; ++k) {
-        const float* piece = first + (size_t)k * kPieceFloats<DP>;
+        const float* piece = first + (size_t)k * kPieceFloats<DP, KS>;
         const float f = __builtin_amdgcn_exp2f(piece[kRows * DP + r] - m);
         l += piece[kRows * DP + kRows + r] * f;
 #pragma unroll
@@ -386,29 +423,50 @@ __global__ __launch_bounds__(kThreads) void join_rows_kernel(Kv8Cache c, Kv8Batc
     if (lse && lane == 0) lse[at] = l == 0.0f ? -__builtin_inff() : (__builtin_amdgcn_logf(l) + m - (float)kBias) * kLn2;
 }
 
-int tiles_of(int group, int max_q) { return (int)(((int64_t)max_q * group + kRows - 1) / kRows); }
-
-// Pieces each row tile's pages are cut into: enough for two workgroups on each compute unit, of at least eight pages.
-int parts_of(int cus, int n_kv, int group, int n_seq, int max_q, int max_pages) {
-    const int64_t wgs = (int64_t)n_seq * n_kv * tiles_of(group, max_q);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus / wgs, max_pages / 8));
+int tiles_of(int group, int max_q, int ks) {
+    const int rows = kCols * kWaves / ks;
+    return (int)(((int64_t)max_q * group + rows - 1) / rows);
 }
 
+// How a call is cut up. Two waves to 32 rows halve a workgroup's time per page and double what is spent on bringing pages
+// into LDS: better while the time is that of the longest row tiles, which is up to four tiles of 128 rows for a compute
+// unit (one / two ways, 32 heads of 128, 8 KV heads: 512 tokens 30 / 22 us, 1024 51 / 40, 2048 104 / 99, four times 1024
+// 109 / 125, 4096 300 / 328; three packed prompts, 16 heads of 80: 88 / 67).
+struct Cut {
+    int ks, tiles, parts;
+};
+Cut cut_of(int cus, int n_kv, int group, int n_seq, int max_q, int max_pages) {
+    Cut c;
+    c.ks = (int64_t)n_seq * n_kv * tiles_of(group, max_q, 1) < (int64_t)4 * cus ? 2 : 1;
+    c.tiles = tiles_of(group, max_q, c.ks);
+    // pieces each row tile's pages are cut into: enough for two workgroups on each compute unit, of at least eight pages
+    const int64_t wgs = (int64_t)n_seq * n_kv * c.tiles;
+    c.parts = (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus / wgs, max_pages / 8));
+    return c;
+}
+
+template <int DP, int DC, int KS>
+void launch_prompt_ks(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch, const Cut& cut,
+                      hipStream_t stream) {
+    const bool gen = a.softcap > 0.0f || a.window > 0 || a.slopes || a.first || a.prefix;
+    auto kernel = c.f8 ? (gen ? prompt_kernel<DP, DC, KS, true, true> : prompt_kernel<DP, DC, KS, true, false>)
+                       : (gen ? prompt_kernel<DP, DC, KS, false, true> : prompt_kernel<DP, DC, KS, false, false>);
+    const size_t lds = 2 * sizeof(Stage<DC>);
+    static_assert(2 * sizeof(Stage<DC>) >= kWaves / 2 * (DC / 2 + 4) * 64 * sizeof(float), "the second halves' results fit");
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    // heads side by side: workgroups go round the XCDs in this order, so a head's pages stay in one L2
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(c.n_kv * cut.parts), (unsigned)b.n_seq, (unsigned)cut.tiles), dim3(kThreads), lds,
+                       stream, c, b, a, dst, lse, scratch, cut.tiles, cut.parts);
+    if (cut.parts > 1)
+        hipLaunchKernelGGL((join_rows_kernel<DP, KS>), dim3((unsigned)(b.n_seq * c.n_kv * cut.tiles), kRows<KS> / kWaves),
+                           dim3(kThreads), 0, stream, c, b, a, dst, lse, scratch, cut.tiles, cut.parts);
+}
 template <int DP, int DC>
 void launch_prompt_dc(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch, int cus,
                       hipStream_t stream) {
-    const bool gen = a.softcap > 0.0f || a.window > 0 || a.slopes || a.first || a.prefix;
-    const int tiles = tiles_of(a.group, b.max_q), parts = parts_of(cus, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);
-    auto kernel = c.f8 ? (gen ? prompt_kernel<DP, DC, true, true> : prompt_kernel<DP, DC, true, false>)
-                       : (gen ? prompt_kernel<DP, DC, false, true> : prompt_kernel<DP, DC, false, false>);
-    const size_t lds = 2 * sizeof(Stage<DC>);
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    // heads side by side: workgroups go round the XCDs in this order, so a head's pages stay in one L2
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(c.n_kv * parts), (unsigned)b.n_seq, (unsigned)tiles), dim3(kThreads), lds, stream,
-                       c, b, a, dst, lse, scratch, tiles, parts);
-    if (parts > 1)
-        hipLaunchKernelGGL(join_rows_kernel<DP>, dim3((unsigned)(b.n_seq * c.n_kv * tiles), kRows / kWaves), dim3(kThreads), 0,
-                           stream, c, b, a, dst, lse, scratch, tiles, parts);
+    const Cut cut = cut_of(cus, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);
+    if (cut.ks == 2) launch_prompt_ks<DP, DC, 2>(c, b, a, dst, lse, scratch, cut, stream);
+    else launch_prompt_ks<DP, DC, 1>(c, b, a, dst, lse, scratch, cut, stream);
 }
 template <int DP>
 void launch_prompt_dp(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch, int cus,
@@ -423,9 +481,9 @@ bool prompt_takes(int max_q, int group) {
     return (int64_t)max_q * group > 32;
 }
 size_t prompt_scratch(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages) {
-    const int parts = parts_of(cus, n_kv, group, n_seq, max_q, max_pages);
-    const size_t dp = (size_t)(dim + 63) / 64 * 64;
-    return parts == 1 ? 0 : (size_t)n_seq * n_kv * tiles_of(group, max_q) * parts * (kRows * dp + 2 * kRows) * sizeof(float);
+    const Cut cut = cut_of(cus, n_kv, group, n_seq, max_q, max_pages);
+    const size_t dp = (size_t)(dim + 63) / 64 * 64, rows = kCols * kWaves / cut.ks;
+    return cut.parts == 1 ? 0 : (size_t)n_seq * n_kv * cut.tiles * cut.parts * (rows * dp + 2 * rows) * sizeof(float);
 }
 void launch_attention_prompt(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch,
                              int cus, hipStream_t stream) {
