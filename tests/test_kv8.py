@@ -433,6 +433,29 @@ def test_attention_modes(be, type_, kw, news, lens):
 
 
 @gpu
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("kw", [{}, *MODES], ids=lambda k: "-".join(f"{a}{b}" for a, b in k.items()))
+@pytest.mark.parametrize("dim,n_head,news,lens", [(96, 6, (150, 70), (150, 70)), (128, 4, (130, 0), (200, 3)), (200, 2, (90, 33), (90, 200))])
+def test_attention_modes_in_a_batch_of_many_rows(be, type_, kw, dim, n_head, news, lens):
+    """max_q and rows far above what the sequences have: such a call takes tiles of 128 rows. One sequence's cache holds
+    a value that is not finite."""
+    rng = np.random.default_rng(len(kw) + dim)
+    rows = 512 * 128 // n_head + 1
+    c, pages, _ = filled(rng, type_, 16, 2, dim, lens)
+    c.v_scale[pages[0][1], 1, 0] = np.nan
+    m = mode_of(kw, n_head, news, lens, rng)
+    if m.first is not None:
+        m.first = np.concatenate([m.first, np.zeros(rows - len(m.first), int)])
+    b = orc.Batch(list(news), list(lens), pages, rows=rows, max_q=rows)
+    q = rng.standard_normal((rows, n_head * dim)).astype(np.float32)
+    out, lse = Dev(be, c).attention(b, m, q)
+    want, want_l, tol, ltol = orc.attention(c, b, m, q)
+    close(out, want, tol)
+    close(lse, want_l, ltol)
+    assert (out[sum(news):] == 7.0).all()
+
+
+@gpu
 @pytest.mark.parametrize("news", [(1,), (2,), (40,)])
 def test_attention_over_positions_with_gaps(be, news):
     """As after an eviction: positions ascend with gaps, the masks and the bias go by them."""
