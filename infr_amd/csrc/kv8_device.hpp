@@ -273,8 +273,9 @@ struct SeqCut {
     int parts, first;
 };
 // The share of sequence `want`, or, with want < 0, of the sequence that holds piece `item`. About `target` pieces are
-// aimed at, of at least one page for each wave of a workgroup; sequences of up to `whole` pages are one. Up to 64 sequences take one round of loads, and the
-// sequence found is passed between the lanes; more of them take a loop over the tables and another over the counts.
+// aimed at, of at least one page for each wave of a workgroup; sequences of up to `whole` pages are one. Up to 64
+// sequences take one round of loads, and the sequence found is passed between the lanes; more of them take a loop over the
+// tables and another over the counts.
 __device__ __forceinline__ SeqCut find_cut(const Kv8Batch& b, const Kv8Attn& a, int n_kv, int rows, int target, int whole, bool all,
                                            int want, int item) {
     const int lane = (int)(threadIdx.x & 63);

@@ -33,7 +33,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
     constexpr int kCols = DP / 64;   // 64-column groups of a key
     constexpr int kOut = DP / 16;    // 16-column groups of a value
     constexpr int kFours = DP / 4, kThreads = 64 * kWaves;
-    constexpr int kPart = 16 * (DP + 4);
+    constexpr int kPart = ROWS * (DP + 4);
     constexpr bool PACK = ROWS == 8;   // columns 8..15 are the low parts of columns 0..7
     __shared__ __align__(16) float part_o[kWaves * kPart];  // the waves' outputs; before, the query rows
     static_assert(sizeof(StepQ<DP, ROWS>) <= sizeof(part_o), "the rows fit");
@@ -269,7 +269,13 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
     // (a wave that has seen nothing has sum 0 and O 0; exp2 of its maximum's distance is 0)
     const float mine = __builtin_amdgcn_exp2f(top - all_top) * (v_exp == -200 ? 0.0f : __builtin_amdgcn_exp2f((float)v_exp));
 #pragma unroll
-    for (int k = 0; k < kOut; ++k) *reinterpret_cast<f4*>(&part_o[wave * kPart + col * (DP + 4) + k * 16 + 4 * g]) = o[k] * mine;
+    for (int k = 0; k < kOut; ++k) {
+        f4 y = o[k];
+        if (PACK)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] += from_other_eight(y[e]);
+        if (col < ROWS) *reinterpret_cast<f4*>(&part_o[wave * kPart + col * (DP + 4) + k * 16 + 4 * g]) = y * mine;
+    }
     __syncthreads();
     const bool whole = parts == 1;
     const int rows = min(ROWS, n_rows - rt * ROWS), tid = threadIdx.x;
@@ -300,7 +306,6 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
 #pragma unroll
         for (int k = 0; k < kWaves; ++k) {
             x += *reinterpret_cast<const f4*>(&part_o[k * kPart + r * (DP + 4) + d]);
-            if (PACK) x += *reinterpret_cast<const f4*>(&part_o[k * kPart + (r + 8) * (DP + 4) + d]);
             m = fmaxf(m, part_m[k][r]);
         }
 #pragma unroll
@@ -393,36 +398,52 @@ int max_tiles_of(int group, int max_q) {
     return (int)(((int64_t)max_q * group + rows - 1) / rows);
 }
 
-// Pieces aimed at. What runs at a time are two workgroups on a compute unit, one with more than 128 columns: with fewer
-// (sequence, head, row tile)s than that, so many pieces that they are one round together with half a piece each for the
-// rounding up (two sequences of 115000 tokens: 46 us, with half as many again 50). Else they come in rounds, and more of
-// them level out (64 sequences of 500 to 8000 tokens, 8 heads: 72 us, with two thirds of them 74).
-int step_target(int cus, int dim, int64_t tiles) {
+bool takes_gen(const Kv8Attn& a) { return a.softcap > 0.0f || a.window > 0 || a.slopes || a.first || a.prefix; }
+
+// How a call is cut up.
+struct StepCut {
+    int tiles;     // row tiles of a sequence at most
+    int target;    // pieces aimed at
+    int whole;     // pages of a sequence that is one piece
+    bool join;     // a sequence can have more than one
+    size_t items;  // upper bound of the pieces
+};
+// gen: the form with caps and masks by position.
+StepCut step_cut(int cus, int dim, bool gen, int window, int n_kv, int group, int n_seq, int max_q, int max_pages) {
+    StepCut c;
+    c.tiles = max_tiles_of(group, max_q);
+    const int64_t tiles = (int64_t)n_seq * n_kv * c.tiles;
+    // What runs at a time are two workgroups on a compute unit, one with more than 128 columns: with fewer
+    // (sequence, head, row tile)s than that, so many pieces that they are one round together with half a piece each for the
+    // rounding up (two sequences of 115000 tokens: 46 us, with half as many again 50). Else they come in rounds, and more of
+    // them level out (64 sequences of 500 to 8000 tokens, 8 heads: 72 us, with two thirds of them 74).
     const int64_t slots = dim <= 128 ? 2 * cus : cus;
-    return (int)(tiles < slots ? std::max(slots - tiles / 2, slots / 2) : dim <= 128 ? 3 * cus : 2 * cus);
-}
-// Sequences of up to so many pages are one piece: the pages a wave goes over more cost less than a join, the less so the
-// fewer compute units have work (one sequence of 700 tokens: 11.8 us whole, 12.9 in three; drafts of 16 sequences over
-// 1024 tokens of 256 columns: 28 us whole, 37 in two).
-int step_whole(int cus, int64_t tiles) { return 2 * tiles >= cus ? 24 : 12; }
-// Upper bound of the pieces: the total is cut into `target`, and each (sequence, head, row tile) rounds up once.
-size_t step_items(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages) {
-    const size_t tiles = (size_t)n_seq * n_kv * max_tiles_of(group, max_q);
-    return std::min((size_t)step_target(cus, dim, (int64_t)tiles) + tiles, tiles * (size_t)((max_pages + kWaves - 1) / kWaves));
+    c.target = (int)(tiles < slots ? std::max(slots - tiles / 2, slots / 2) : dim <= 128 ? 3 * cus : 2 * cus);
+    // Up to which length a sequence stays in one piece: where half the compute units have one already, the pages a wave
+    // goes over more cost less than a join (8 heads, whole / cut: 64 sequences of 1000 tokens 27 / 35 us, 32 sequences'
+    // drafts over 1024 tokens of 256 columns 33 / 54; but 64 of 500 to 2000 tokens 43 / 39). With fewer it is a join's time
+    // against a page's: 12 / 8 pages at 128 columns (one sequence of 700 tokens 10.2 / 10.6 us; 16 sequences of 700
+    // 11.9 / 13.5), 8 / 12 with masks (drafts of 16 sequences 19 / 23), 4 / 12 at 256 columns (drafts of 4 sequences
+    // 16 / 24 us, one sequence of 700 tokens 12.7 / 15).
+    c.whole = 2 * tiles > cus ? 24 : dim > 128 ? 4 : gen ? 8 : 12;
+    // a window bounds the pages gone over: `window` tokens and one less than the call's rows
+    const int64_t most = window > 0 ? std::min<int64_t>(max_pages, ((int64_t)window + max_q + 125) / kPage) : max_pages;
+    c.join = most > c.whole;
+    // the total is cut into `target`, and each (sequence, head, row tile) rounds up once
+    c.items = std::min((size_t)c.target + (size_t)tiles, (size_t)tiles * (size_t)((max_pages + kWaves - 1) / kWaves));
+    return c;
 }
 template <int DP, int ROWS>
 void launch_step_rows(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch, int cus,
                       hipStream_t stream) {
-    const int tiles = max_tiles_of(a.group, b.max_q), target = step_target(cus, c.dim, (int64_t)b.n_seq * c.n_kv * tiles);
-    const int whole = step_whole(cus, (int64_t)b.n_seq * c.n_kv * tiles);
-    const bool gen = a.softcap > 0.0f || a.window > 0 || a.slopes || a.first || a.prefix;
-    const unsigned items = (unsigned)step_items(cus, c.dim, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);
+    const bool gen = takes_gen(a);
+    const StepCut cut = step_cut(cus, c.dim, gen, a.window, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);
     auto kernel = c.f8 ? (gen ? step_kernel<DP, ROWS, true, true> : step_kernel<DP, ROWS, true, false>)
                        : (gen ? step_kernel<DP, ROWS, false, true> : step_kernel<DP, ROWS, false, false>);
-    hipLaunchKernelGGL(kernel, dim3(items), dim3(64 * kWaves), 0, stream, c, b, a, dst, lse, scratch, target, whole);
-    if (b.max_pages <= whole) return;  // no sequence has two pieces
-    hipLaunchKernelGGL((join_kernel<DP, ROWS>), dim3((unsigned)(b.n_seq * c.n_kv * tiles), (unsigned)std::min(ROWS, b.max_q * a.group)),
-                       dim3(256), 0, stream, c, b, a, dst, lse, scratch, target, whole, tiles);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)cut.items), dim3(64 * kWaves), 0, stream, c, b, a, dst, lse, scratch, cut.target, cut.whole);
+    if (cut.join)
+        hipLaunchKernelGGL((join_kernel<DP, ROWS>), dim3((unsigned)(b.n_seq * c.n_kv * cut.tiles), (unsigned)std::min(ROWS, b.max_q * a.group)),
+                           dim3(256), 0, stream, c, b, a, dst, lse, scratch, cut.target, cut.whole, cut.tiles);
 }
 template <int DP>
 void launch_step_dp(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch, int cus,
@@ -434,9 +455,10 @@ void launch_step_dp(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, floa
 }  // namespace
 
 size_t step_scratch(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages) {
-    if (max_pages <= step_whole(cus, (int64_t)n_seq * n_kv * max_tiles_of(group, max_q))) return 0;
+    // (for the shape alone: what joins most often)
+    const StepCut cut = step_cut(cus, dim, true, 0, n_kv, group, n_seq, max_q, max_pages);
     const size_t dp = (size_t)(dim + 63) / 64 * 64;
-    return step_items(cus, dim, n_kv, group, n_seq, max_q, max_pages) * (kStepRows * dp + 2 * kStepRows) * sizeof(float);
+    return cut.join ? cut.items * (kStepRows * dp + 2 * kStepRows) * sizeof(float) : 0;
 }
 void launch_attention_step(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch,
                            int cus, hipStream_t stream) {

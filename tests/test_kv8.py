@@ -481,6 +481,19 @@ def test_attention_long_axis(be, type_, news):
 
 
 @gpu
+@pytest.mark.parametrize("news", [1, 3])
+@pytest.mark.parametrize("dim,pages_whole", [(64, 8), (160, 4)])
+def test_attention_windows_around_a_whole_piece(be, news, dim, pages_whole):
+    """Long sequences whose windows reach as many pages as one workgroup takes, one less and one more, from every 7th slot
+    of a page."""
+    rng = np.random.default_rng(15)
+    lens = tuple(range(940, 1010, 7))
+    c, pages, _ = filled(rng, "i8", 16, 1, dim, lens)
+    for window in (pages_whole * 64 - 62 - news, pages_whole * 64 - 61 - news, pages_whole * 64 - 126 - news):
+        check_attention(be, c, pages, [news] * len(lens), list(lens), orc.Mode(1, window=window))
+
+
+@gpu
 @pytest.mark.parametrize("news", [1, 40])
 def test_attention_many_sequences(be, news):
     rng = np.random.default_rng(13)
