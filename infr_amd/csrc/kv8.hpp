@@ -124,6 +124,43 @@ __device__ __forceinline__ uint32_t kv8_code(float x, float scale, float inverse
     } else code = (uint32_t)(int)fminf(fmaxf(rintf(y), -127.0f), 127.0f) & 0xFFu;
     return inverse == 0.0f ? 0u : code;
 }
+// Codes without the corrections: the quotient's product with an inverse a little above and with one a little below it. The
+// inverse is within 2^-23 of 1 / scale and the correctly rounded quotient within 2^-24 of the true one, so with 2^-22 to
+// either side the two products enclose it; rounding is monotone, so where both give one code it is the quotient's. Where
+// they do not, `doubt` says so (about one code in 10^5) and kv8_code decides.
+struct Kv8Bounds {
+    float lo, hi;
+};
+__device__ __forceinline__ Kv8Bounds kv8_bounds(float inverse) { return {inverse * (1.0f - 0x1p-22f), inverse * (1.0f + 0x1p-22f)}; }
+// Four codes side by side. The int8 codes come out of one fused multiply-add each: added to 1.5 * 2^23 a product is rounded
+// to whole numbers, ties to even, and stands in the sum's low bits.
+template <bool F8>
+__device__ __forceinline__ uint32_t kv8_codes(const float* x, Kv8Bounds inv, uint32_t* doubt) {
+    if constexpr (F8) {
+        int a = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv.lo, x[1] * inv.lo, 0, false);
+        a = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv.lo, x[3] * inv.lo, a, true);
+        int b = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv.hi, x[1] * inv.hi, 0, false);
+        b = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv.hi, x[3] * inv.hi, b, true);
+        *doubt |= (uint32_t)(a ^ b);
+        return (uint32_t)a;
+    } else {
+        uint32_t a[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            a[e] = __builtin_bit_cast(uint32_t, __builtin_fmaf(x[e], inv.lo, 12582912.0f));
+            *doubt |= a[e] ^ __builtin_bit_cast(uint32_t, __builtin_fmaf(x[e], inv.hi, 12582912.0f));
+        }
+        return __builtin_amdgcn_perm(a[1], a[0], 0x0C0C0400u) | __builtin_amdgcn_perm(a[3], a[2], 0x04000C0Cu);
+    }
+}
+// The same in doubt.
+template <bool F8>
+__device__ __forceinline__ uint32_t kv8_codes_exact(const float* x, float scale, float inverse) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w |= kv8_code<F8>(x[e], scale, inverse) << (8 * e);
+    return w;
+}
 template <bool F8>
 __device__ __forceinline__ float kv8_value(uint32_t code) {
     if constexpr (F8) return __builtin_amdgcn_cvt_f32_fp8((int)code, 0);

@@ -18,6 +18,8 @@ namespace infr {
 
 namespace {
 
+typedef short s2 __attribute__((ext_vector_type(2)));
+
 constexpr int kMove = 256;
 constexpr int kBinBits = 11, kBins = 1 << kBinBits;
 
@@ -200,9 +202,7 @@ __global__ __launch_bounds__(THREADS, 4) void evict_select_kernel(Kv8Cache c, Kv
         }
         int at = out_before + block_scan<THREADS>(__builtin_popcount(take), part, &total);
         out_before += total;
-#pragma unroll
-        for (int n = 0; n < EACH; ++n)
-            if ((take >> n) & 1) kept[at++] = j0 + n;
+        for (; take; take &= take - 1) kept[at++] = j0 + __builtin_ctz(take);
     }
 }
 
@@ -257,10 +257,17 @@ __global__ __launch_bounds__(kMove) void evict_move_kernel(Kv8Cache c, Kv8Evict 
     const bool again = amax[t / c.block] >> 31;
     __syncthreads();
     if (again) {
-        uint32_t top = 0;
+        // the token's code of the largest size, by pairs of 16-bit numbers: every product with the scale is monotone in it
+        s2 high = s2{0, 0}, low = s2{0, 0};
         auto look = [&](uint32_t w) {
-#pragma unroll
-            for (int n = 0; n < 4; ++n) top = max(top, abs_bits(kv8_value<F8>((w >> (8 * n)) & 255u) * old));
+            if constexpr (F8) {
+                high = __builtin_elementwise_max(high, __builtin_bit_cast(s2, w & 0x007F007Fu));
+                high = __builtin_elementwise_max(high, __builtin_bit_cast(s2, (w >> 8) & 0x007F007Fu));
+            } else {
+                const s2 odd = __builtin_bit_cast(s2, w) >> 8, even = __builtin_bit_cast(s2, w << 8) >> 8;
+                high = __builtin_elementwise_max(high, __builtin_elementwise_max(odd, even));
+                low = __builtin_elementwise_min(low, __builtin_elementwise_min(odd, even));
+            }
         };
         if (live && !is_v)
 #pragma unroll
@@ -268,15 +275,21 @@ __global__ __launch_bounds__(kMove) void evict_move_kernel(Kv8Cache c, Kv8Evict 
         if (live && is_v)
 #pragma unroll
             for (int d = 0; d < kColumns / 4; ++d) look(vw[d]);
-        atomicMax(&amax[t / c.block], top | 0x80000000u);
+        const int most = max(max((int)high[0], (int)high[1]), -min((int)low[0], (int)low[1]));
+        const float value = F8 ? kv8_value<F8>((uint32_t)most) : (float)most;
+        atomicMax(&amax[t / c.block], (live ? abs_bits(value * old) : 0u) | 0x80000000u);
     }
     __syncthreads();
     const float scale = again ? kv8_scale(amax[t / c.block] & 0x7FFFFFFFu, F8) : old, inverse = kv8_inverse(scale);
+    const Kv8Bounds bounds = kv8_bounds(inverse);
     auto code = [&](uint32_t w) {
-        uint32_t r = 0;
+        float x[4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) r |= kv8_code<F8>(kv8_value<F8>((w >> (8 * n)) & 255u) * old, scale, inverse) << (8 * n);
-        return r;
+        for (int n = 0; n < 4; ++n) x[n] = kv8_value<F8>((w >> (8 * n)) & 255u) * old;
+        uint32_t doubt = 0;
+        uint32_t r = kv8_codes<F8>(x, bounds, &doubt);
+        if (doubt) r = kv8_codes_exact<F8>(x, scale, inverse);
+        return inverse == 0.0f ? 0u : r;
     };
     if (!live) return;
     if (t % c.block == 0 && part == 0) scales[dst * subs + t / c.block] = scale;

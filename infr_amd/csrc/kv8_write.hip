@@ -117,13 +117,19 @@ __global__ __launch_bounds__(kThreads) void write_kv8_kernel(Kv8Cache c, Kv8Batc
     __syncthreads();
     for (int o = 0; o < c.block; ++o) top = max(top, amax[sub * c.block + o]);
     const float scale = kv8_scale(top, F8), inverse = kv8_inverse(scale);
+    const Kv8Bounds bounds = kv8_bounds(inverse);
     if (page_ok && touched && t % c.block == 0 && (tid & 3) == 0) scales[scale_at] = scale;
 #pragma unroll
     for (int j = 0; j < kGroups; ++j) {
         if (!page_ok) continue;
-        uint32_t w[4] = {0, 0, 0, 0};
+        uint32_t w[4], doubt = 0;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) w[e / 4] |= kv8_code<F8>(r[j][e], scale, inverse) << (8 * (e % 4));
+        for (int e = 0; e < 4; ++e) w[e] = kv8_codes<F8>(&r[j][4 * e], bounds, &doubt);
+        if (__any(doubt))
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = kv8_codes_exact<F8>(&r[j][4 * e], scale, inverse);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = inverse == 0.0f ? 0u : w[e];
         if (!is_v) {
             if (is_new || is_old) *reinterpret_cast<uint4*>(c.k + k_at(c, page, h, t, j * 64 + col)) = make_uint4(w[0], w[1], w[2], w[3]);
             continue;
