@@ -8,7 +8,11 @@
 //
 // The pages of all sequences are cut into pieces of one size, found on the device from the lengths: long sequences
 // get many workgroups, short ones one, and no piece is empty. A sequence in one piece writes its result; the pieces
-// of others are joined by a second kernel, in their order. (A join by the workgroup that comes last to its row tile
+// of others are joined by a second kernel, in their order.
+// Measured (8 KV heads of 128, 32 heads): one token of 64 sequences of 500 to 8000 tokens 69 us, 5.2 TB/s, 63 us and 5.7
+// TB/s of it the first kernel (a pass that only reads: 7.1 TB/s); two sequences of 115000 tokens, 4 KV heads, 45 us, 5.2
+// TB/s; one of 700 tokens 9.8 us, launch and dependent loads; drafts of 4 tokens of 16 sequences, window 1024, capped, 8
+// KV heads of 256, 26 us, bound by what one wave does for a page. (A join by the workgroup that comes last to its row tile
 // saves that launch but costs its own round trips past the L2, which the XCDs do not share: 53 us against 49 for two
 // sequences of 115000 tokens, 48 against 44 for drafts of four tokens.)
 #include "kv8_attn.hpp"

@@ -9,7 +9,9 @@
 // One workgroup per (page that gets tokens, head, K or V): 64 tokens x 64 columns at a time, four lanes to a
 // token, 16 columns each, so that a token's 64 columns are one 256-byte read and its key codes one 64-byte
 // segment; value codes turn in LDS. Bound by HBM on 8 bytes read and 2 written per column of a token; a single
-// token per sequence is bound by the launch.
+// token per sequence is bound by the launch and four dependent loads (tables, page, tag and tail, codes).
+// Measured (8 heads of 128): 8192 tokens of four prompts 23.8 us, 3.5 TB/s read and written (a copy: 5.1); one token
+// of each of 64 sequences 8.3 us.
 #include <algorithm>
 #include <type_traits>
 
