@@ -4,7 +4,7 @@
 // Few rows (at most 16 of a KV head): bound by reading the keys once. As in the attention a wave takes a page at a
 // time; the 16 query rows' weights of a token are summed over the 16 lanes that hold them, each lane keeping one
 // token at the end.
-// Many rows: bound by the matrix cores, 2 head_dim flops a pair, twice that in f16 products. A wave keeps a page's
+// Many rows: bound by the matrix cores and the exponential, 2 head_dim flops a pair, twice that in f16 products. A wave keeps a page's
 // keys in registers as f16, four pages a workgroup, and 32 query rows at a time go through LDS, turned into hi + lo
 // once for the four waves (two buffers, one barrier a step). Where pages are few, the rows are cut into parts whose
 // sums a second kernel adds in their order, so that the same call gives the same bits.
