@@ -4,8 +4,8 @@
 // attention weight (equal sums: the lower slot), in their order. Two launches:
 //   select  one workgroup per (sequence, head), each thread with a run of neighbouring tokens whose sums stay in its
 //           registers: the smallest kept sum is found by counting in 2048 bins over the range of the sums, then over
-//           the bin it lies in, 11 bits a pass (integer counts in LDS: the same in any order); two prefix sums then
-//           give every kept token its place. Bound by the passes' latency.
+//           the bin it lies in, 11 bits a pass (integer counts in LDS: the same in any order), until at most 64 are
+//           left, which a wave ranks; two prefix sums then give every kept token its place. Bound by the passes' latency.
 //   move    one workgroup per (new page, head, K or V): gathers the kept tokens' codes, 16-byte pieces of K rows and
 //           single bytes of V^T rows, a lane to a token, so that a wave's bytes lie in as few lines as the tokens'
 //           pages allow. A block whose tokens come whole and in place from one block keeps its codes and scale; the
@@ -84,7 +84,8 @@ template <int THREADS, int EACH>
 __global__ __launch_bounds__(THREADS, 4) void evict_select_kernel(Kv8Cache c, Kv8Evict e) {
     __shared__ int part[THREADS / 64];
     __shared__ int hist[kBins];
-    __shared__ uint32_t found[2], ends[2];
+    __shared__ uint32_t found[3], ends[2], few[64];
+    __shared__ int n_few;
     const int s = blockIdx.y, h = blockIdx.x, tid = threadIdx.x;
     const EvictSeq q = evict_seq(c, e, s, tid, THREADS);
     const int32_t* pages = e.pages + (size_t)s * e.max_pages;
@@ -150,6 +151,7 @@ __global__ __launch_bounds__(THREADS, 4) void evict_select_kernel(Kv8Cache c, Kv
         while (width > 0) {
             const int shift = max(32 - __builtin_clz(width) - kBinBits, 0);
             for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
+            if (tid == 0) n_few = 0;
             __syncthreads();
             for (int r = 0; r < rounds; ++r) {
                 if (rounds > 1) load(r);
@@ -172,6 +174,7 @@ __global__ __launch_bounds__(THREADS, 4) void evict_select_kernel(Kv8Cache c, Kv
                     if (above < ties && ties <= above + n) {
                         found[0] = (uint32_t)(top - i);
                         found[1] = (uint32_t)(ties - above);
+                        found[2] = (uint32_t)n;
                     }
                     above += n;
                 }
@@ -180,6 +183,27 @@ __global__ __launch_bounds__(THREADS, 4) void evict_select_kernel(Kv8Cache c, Kv
             width = min(size, width - base);
             limit += base;
             ties = (int)found[1];
+            const int n_bin = __builtin_amdgcn_readfirstlane((int)found[2]);
+            if (width > 0 && n_bin <= 64) {  // few enough for every wave to rank them by itself, a lane to each
+                for (int r = 0; r < rounds; ++r) {
+                    if (rounds > 1) load(r);
+#pragma unroll
+                    for (int n = 0; n < EACH; ++n)
+                        if (key[n] && key[n] - limit <= width) few[atomicAdd(&n_few, 1)] = key[n];
+                }
+                __syncthreads();
+                const uint32_t mine = (tid & 63) < n_bin ? few[tid & 63] : 0;
+                int above = 0, upto = 0;
+                for (int i = 0; i < n_bin; ++i) {
+                    const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)mine, i);
+                    above += other > mine ? 1 : 0;
+                    upto += other >= mine ? 1 : 0;
+                }
+                const int l = __builtin_ctzll(__ballot((tid & 63) < n_bin && above < ties && ties <= upto));
+                limit = (uint32_t)__builtin_amdgcn_readlane((int)mine, l);
+                ties -= __builtin_amdgcn_readlane(above, l);
+                width = 0;
+            }
             __syncthreads();
         }
     }
