@@ -12,9 +12,11 @@
 // Measured (8 KV heads of 128, 32 heads): one token of 64 sequences of 500 to 8000 tokens 69 us, 5.2 TB/s, 63 us and 5.7
 // TB/s of it the first kernel (a pass that only reads: 7.1 TB/s); two sequences of 115000 tokens, 4 KV heads, 45 us, 5.2
 // TB/s; one of 700 tokens 9.8 us, launch and dependent loads; drafts of 4 tokens of 16 sequences, window 1024, capped, 8
-// KV heads of 256, 26 us, bound by what one wave does for a page. (A join by the workgroup that comes last to its row tile
+// KV heads of 256, 22 us, bound by what one wave does for half a page. (A join by the workgroup that comes last to its row tile
 // saves that launch but costs its own round trips past the L2, which the XCDs do not share: 53 us against 49 for two
 // sequences of 115000 tokens, 48 against 44 for drafts of four tokens.)
+#include <type_traits>
+
 #include "kv8_attn.hpp"
 #include "kv8_device.hpp"
 
@@ -22,7 +24,9 @@ namespace infr {
 
 namespace {
 
-constexpr int kWaves = kStepWaves;
+// Waves of a workgroup that take TOK tokens of a page at a time: together four pages.
+template <int TOK>
+constexpr int kWaves = kPage / TOK * kStepWaves;
 constexpr int kBias = 10;    // softmax weights are 2^kBias at the running maximum ..
 constexpr float kLag = 4.0f; // .. which may lag behind the true one by this many powers of two
 
@@ -30,13 +34,15 @@ constexpr float kLag = 4.0f; // .. which may lag behind the true one by this man
 template <int DP, int ROWS>
 constexpr int kPieceFloats = ROWS * DP + 2 * ROWS;
 
-template <int DP, int ROWS, bool F8, bool GEN>
-__global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192 && ROWS == 8) ? 2 : 1) void step_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a,
+template <int DP, int ROWS, int TOK, bool F8, bool GEN>
+__global__ __launch_bounds__(64 * kWaves<TOK>, DP == 64 ? 3 : DP == 128 || (DP == 192 && ROWS == 8) || TOK == 32 ? 2 : 1) void step_kernel(Kv8Cache c, Kv8Batch b, Kv8Attn a,
                                                                              float* __restrict__ dst, float* __restrict__ lse,
                                                                              float* __restrict__ scratch, int target, int whole_pages) {
     constexpr int kCols = DP / 64;   // 64-column groups of a key
     constexpr int kOut = DP / 16;    // 16-column groups of a value
-    constexpr int kFours = DP / 4, kThreads = 64 * kWaves;
+    constexpr int kWaves = infr::kWaves<TOK>, kFours = DP / 4, kThreads = 64 * kWaves;
+    constexpr int kShare = kPage / TOK;                  // waves that share a page
+    constexpr int kMine = TOK / 4, kTiles = TOK / 16;    // tokens of a lane; row tiles of the MFMA
     constexpr int kPart = ROWS * (DP + 4);
     constexpr bool PACK = ROWS == 8;   // columns 8..15 are the low parts of columns 0..7
     __shared__ __align__(16) float part_o[kWaves * kPart];  // the waves' outputs; before, the query rows
@@ -81,36 +87,39 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
     const int32_t* table = b.pages + (size_t)s * b.max_pages;
     const int subs = kPage / c.block;
     const uint32_t kv_stride = (uint32_t)DP * kPage;
-    uint4 kf[4][kCols], vf[kOut];
+    using VCodes = typename std::conditional<TOK == 64, uint4, uint2>::type;
+    uint4 kf[kTiles][kCols];
+    VCodes vf[kOut];
     float ks = 0.0f, vs = 0.0f;
     int page = 0, ids = 0, pos0 = 0;
+    const int half = wave % kShare * TOK;  // the wave's first token in a page
     // lane n holds the wave's n-th next page
     auto load_ids = [&](int p) {
-        const int at = p + lane * kWaves;
+        const int at = p + lane * kStepWaves;
         ids = at < p1 ? table[at] : 0;
         if (ids < 0 || ids >= c.n_pages) ids = -1;
         if (__any(ids < 0)) bad = true;
     };
     auto load_keys = [&](int n) {
         page = max(__builtin_amdgcn_readlane(ids, n), 0);
-        const uint8_t* kp = c.k + ((size_t)page * c.n_kv + h) * kv_stride + (16 * (col >> 2) + (col & 3)) * 64 + 16 * g;
+        const uint8_t* kp = c.k + ((size_t)page * c.n_kv + h) * kv_stride + (half + kMine * (col >> 2) + (col & 3)) * 64 + 16 * g;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < kTiles; ++t)
 #pragma unroll
             for (int j = 0; j < kCols; ++j) kf[t][j] = load_stream(kp + j * kPage * 64 + t * 4 * 64);
-        const size_t sc = ((size_t)page * c.n_kv + h) * subs + g * 16 / c.block;
+        const size_t sc = ((size_t)page * c.n_kv + h) * subs + (half + g * kMine) / c.block;
         ks = c.ks[sc];
         vs = c.vs[sc];
         if (use_pos) pos0 = c.pos[((size_t)page * c.n_kv + h) * kPage];
     };
-    int p = p0 + wave, n = 0;
+    int p = p0 + wave / kShare, n = 0;
     if (p < p1) {
         load_ids(p);
         load_keys(0);
     }
     // the query rows as hi + lo
     StepQ<DP, ROWS>& rows_q = *reinterpret_cast<StepQ<DP, ROWS>*>(part_o);
-    stage_rows<DP, ROWS>(rows_q, c, a, q, h, rt * ROWS);
+    if (kWaves == 4 || wave < 4) stage_rows<DP, ROWS>(rows_q, c, a, q, h, rt * ROWS);  // (whole waves, 256 threads)
     __syncthreads();
     h8 qh[2 * kCols], ql[PACK ? 1 : 2 * kCols];
 #pragma unroll
@@ -121,24 +130,27 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
     }
     const float row_factor = rows_q.factor[col % ROWS];
     while (p < p1) {
-        const uint8_t* vp = c.v + ((size_t)page * c.n_kv + h) * kv_stride + col * kPage + 16 * g;
+        const uint8_t* vp = c.v + ((size_t)page * c.n_kv + h) * kv_stride + col * kPage + half + kMine * g;
 #pragma unroll
-        for (int k = 0; k < kOut; ++k) vf[k] = load_stream(vp + k * 16 * kPage);
+        for (int k = 0; k < kOut; ++k) {
+            if constexpr (TOK == 64) vf[k] = load_stream(vp + k * 16 * kPage);
+            else vf[k] = *reinterpret_cast<const uint2*>(vp + k * 16 * kPage);  // (the other half of the line is another wave's)
+        }
         // (positions ascend: what the tile's last row's window and document allow at the page's first token, all rows do)
         const bool masked = (p + 1) * kPage > min(all_see, q.len) || (use_pos && (last_pos - pos0 >= row.window || last_first > pos0));
-        int kpos[16];
+        int kpos[kMine];
         if (use_pos && (masked || a.slopes)) {
-            const int4* pp = reinterpret_cast<const int4*>(c.pos + ((size_t)page * c.n_kv + h) * kPage + 16 * g);
+            const int4* pp = reinterpret_cast<const int4*>(c.pos + ((size_t)page * c.n_kv + h) * kPage + half + kMine * g);
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
+            for (int t = 0; t < kTiles; ++t) {
                 const int4 x = pp[t];
                 kpos[4 * t] = x.x, kpos[4 * t + 1] = x.y, kpos[4 * t + 2] = x.z, kpos[4 * t + 3] = x.w;
             }
         }
-        // scores: sc[t][i] is token 16 g + 4 t + i of the page
-        f4 sc[4];
+        // scores: sc[t][i] is token kMine g + 4 t + i of the wave's
+        f4 sc[kTiles];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < kTiles; ++t) {
             sc[t] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < kCols; ++j) {
@@ -151,12 +163,12 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
                 }
             }
         }
-        const int tok0 = p * kPage + 16 * g;
+        const int tok0 = p * kPage + half + kMine * g;
         const float factor = row_factor * ks;
         const float vs_now = vs;
         const bool tail = (p + 1) * kPage > q.len;
         // the next page's keys are on their way from here
-        const int np = p + kWaves;
+        const int np = p + kStepWaves;
         if (np < p1) {
             if (++n == 64) {
                 load_ids(np);
@@ -164,27 +176,27 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
             }
             load_keys(n);
         }
-        float x[16], f = factor;
+        float x[kMine], f = factor;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < kMine; ++e) {
             float v = sc[e / 4][e % 4];
             if (PACK) v += from_other_eight(v);
             x[e] = v;
         }
         if (masked || (GEN && (a.softcap > 0.0f || a.slopes))) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] *= factor;
-            if (GEN && a.softcap > 0.0f) cap_scores<16, false>(x, cap, inv_cap);
+            for (int e = 0; e < kMine; ++e) x[e] *= factor;
+            if (GEN && a.softcap > 0.0f) cap_scores<kMine, false>(x, cap, inv_cap);
             if (GEN && a.slopes)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = __builtin_fmaf(-row.slope, fabsf((float)(row.pos - kpos[e])), x[e]);
+                for (int e = 0; e < kMine; ++e) x[e] = __builtin_fmaf(-row.slope, fabsf((float)(row.pos - kpos[e])), x[e]);
             f = 1.0f;
         }
         bool any = true;
         if (masked) {
             any = false;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
+            for (int e = 0; e < kMine; ++e) {
                 const int tok = tok0 + e;
                 const bool yes = tok < q.len && (use_pos ? row.sees(tok, kpos[e]) : tok <= row.slot);
                 any = any || yes;
@@ -193,11 +205,11 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
         }
         float high = x[0];
 #pragma unroll
-        for (int e = 1; e < 16; ++e) high = fmaxf(high, x[e]);
+        for (int e = 1; e < kMine; ++e) high = fmaxf(high, x[e]);
         high *= f;
         if (__any(fabsf(high) > kLargeScore)) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] *= f;
+            for (int e = 0; e < kMine; ++e) x[e] *= f;
             f = 1.0f;
         }
         const int e_now = scale_exponent(vs_now, any);
@@ -215,16 +227,16 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
         // weights times the values' scale in one exponential; their sum is divided by it
         v_bad = v_bad || (any && vs_now != vs_now);
         const float lift = any ? scale_log(vs_now, v_exp) : 0.0f, base = (float)kBias - top + lift;
-        float w[16], run = 0.0f;
+        float w[kMine], run = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < kMine; ++e) {
             w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], f, base));
             run += w[e];
         }
         sum = __builtin_fmaf(run, __builtin_amdgcn_exp2f(-lift), sum);
-        h8 wh[2], wl[PACK ? 1 : 2];
+        h8 wh[kMine / 8], wl[PACK ? 1 : kMine / 8];
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < kMine / 8; ++k)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 h2 hi, lo;
@@ -234,12 +246,12 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
                 if (!PACK) wl[k][2 * e] = lo[0], wl[k][2 * e + 1] = lo[1];
             }
         if (F8 && tail) {  // what stands behind the last token may be NaN as a code
-            const int left = min(max(q.len - tok0, 0), 16);
+            const int left = min(max(q.len - tok0, 0), kMine);
 #pragma unroll
             for (int k = 0; k < kOut; ++k) {
                 uint32_t* u = reinterpret_cast<uint32_t*>(&vf[k]);
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
+                for (int t = 0; t < kTiles; ++t) {
                     const int m = min(max(left - 4 * t, 0), 4);
                     u[t] = m == 4 ? u[t] : u[t] & ((1u << (8 * m)) - 1u);
                 }
@@ -247,12 +259,13 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : DP == 128 || (DP == 192
         }
 #pragma unroll
         for (int k = 0; k < kOut; ++k) {
-            const h8 lo = code_oct<F8>(vf[k].x, vf[k].y), hi = code_oct<F8>(vf[k].z, vf[k].w);
+            const h8 lo = code_oct<F8>(vf[k].x, vf[k].y);
             o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wh[0], o[k], 0, 0, 0);
-            o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wh[1], o[k], 0, 0, 0);
-            if constexpr (!PACK) {
-                o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wl[0], o[k], 0, 0, 0);
-                o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wl[1], o[k], 0, 0, 0);
+            if constexpr (!PACK) o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wl[0], o[k], 0, 0, 0);
+            if constexpr (TOK == 64) {
+                const h8 hi = code_oct<F8>(vf[k].z, vf[k].w);
+                o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wh[1], o[k], 0, 0, 0);
+                if constexpr (!PACK) o[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wl[1], o[k], 0, 0, 0);
             }
         }
         p = np;
@@ -410,6 +423,7 @@ struct StepCut {
     int target;    // pieces aimed at
     int whole;     // pages of a sequence that is one piece
     bool join;     // a sequence can have more than one
+    bool half;     // waves take half a page at a time
     size_t items;  // upper bound of the pieces
 };
 // gen: the form with caps and masks by position.
@@ -428,13 +442,18 @@ StepCut step_cut(int cus, int dim, bool gen, int window, int n_kv, int group, in
     // drafts over 1024 tokens of 256 columns 33 / 54; but 64 of 500 to 2000 tokens 43 / 39). With fewer it is a join's time
     // against a page's: 12 / 8 pages at 128 columns (one sequence of 700 tokens 10.2 / 10.6 us; 16 sequences of 700
     // 11.9 / 13.5), 8 / 12 with masks (drafts of 16 sequences 19 / 23), 4 / 12 at 256 columns (drafts of 4 sequences
-    // 16 / 24 us, one sequence of 700 tokens 12.7 / 15).
+    // 16 / 24 us, one sequence of 700 tokens 12.7 / 15; all with whole pages to a wave).
     c.whole = 2 * tiles > cus ? 24 : dim > 128 ? 4 : gen ? 8 : 12;
     // a window bounds the pages gone over: `window` tokens and one less than the call's rows
     const int64_t most = window > 0 ? std::min<int64_t>(max_pages, ((int64_t)window + max_q + 125) / kPage) : max_pages;
     c.join = most > c.whole;
+    // More than 128 columns leave a compute unit one wave a SIMD, and nothing to do while it waits, unless a wave takes half
+    // a page; but that reads V in pieces of 32 bytes, which costs where reading is the bound: half up to 64 pages for a
+    // compute unit (256 columns, half / whole pages: drafts of 16 sequences 22.5 / 26.7 us, of 32 26 / 33, one token of 64
+    // sequences of 700 43 / 45, of 16 of 500 to 8000 42.4 / 42.9, of 64 of them 152 / 134).
+    c.half = dim > 128 && tiles * most <= (int64_t)64 * cus;
     // the total is cut into `target`, and each (sequence, head, row tile) rounds up once
-    c.items = std::min((size_t)c.target + (size_t)tiles, (size_t)tiles * (size_t)((max_pages + kWaves - 1) / kWaves));
+    c.items = std::min((size_t)c.target + (size_t)tiles, (size_t)tiles * (size_t)((max_pages + kStepWaves - 1) / kStepWaves));
     return c;
 }
 template <int DP, int ROWS>
@@ -442,9 +461,19 @@ void launch_step_rows(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, fl
                       hipStream_t stream) {
     const bool gen = takes_gen(a);
     const StepCut cut = step_cut(cus, c.dim, gen, a.window, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);
-    auto kernel = c.f8 ? (gen ? step_kernel<DP, ROWS, true, true> : step_kernel<DP, ROWS, true, false>)
-                       : (gen ? step_kernel<DP, ROWS, false, true> : step_kernel<DP, ROWS, false, false>);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)cut.items), dim3(64 * kWaves), 0, stream, c, b, a, dst, lse, scratch, cut.target, cut.whole);
+    auto launch = [&](auto tok) {
+        constexpr int TOK = decltype(tok)::value;
+        auto kernel = c.f8 ? (gen ? step_kernel<DP, ROWS, TOK, true, true> : step_kernel<DP, ROWS, TOK, true, false>)
+                           : (gen ? step_kernel<DP, ROWS, TOK, false, true> : step_kernel<DP, ROWS, TOK, false, false>);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)cut.items), dim3(64 * kWaves<TOK>), 0, stream, c, b, a, dst, lse, scratch, cut.target,
+                           cut.whole);
+    };
+    bool half = false;
+    if constexpr (DP > 128) {
+        half = cut.half;
+        if (half) launch(std::integral_constant<int, 32>{});
+    }
+    if (!half) launch(std::integral_constant<int, 64>{});
     if (cut.join)
         hipLaunchKernelGGL((join_kernel<DP, ROWS>), dim3((unsigned)(b.n_seq * c.n_kv * cut.tiles), (unsigned)std::min(ROWS, b.max_q * a.group)),
                            dim3(256), 0, stream, c, b, a, dst, lse, scratch, cut.target, cut.whole, cut.tiles);

@@ -481,6 +481,24 @@ def test_attention_long_axis(be, type_, news):
 
 
 @gpu
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("dim", [130, 192, 256])
+@pytest.mark.parametrize("news,lens", [((1, 1), (150, 70)), ((4, 3), (500, 129))])
+def test_attention_wide_heads_and_wide_page_tables(be, type_, dim, news, lens):
+    """Tables for far longer sequences than there are, as a server keeps them: waves take whole pages then."""
+    rng = np.random.default_rng(dim)
+    c, pages, _ = filled(rng, type_, 32, 2, dim, lens)
+    for kw in [{}, dict(window=10 ** 6), *MODES]:
+        m = mode_of(kw, 6, news, lens, rng)
+        b = orc.Batch(list(news), list(lens), pages, max_pages=9000)
+        q = rng.standard_normal((b.rows, 6 * dim)).astype(np.float32)
+        out, lse = Dev(be, c).attention(b, m, q)
+        want, want_l, tol, ltol = orc.attention(c, b, m, q)
+        close(out, want, tol)
+        close(lse, want_l, ltol)
+
+
+@gpu
 @pytest.mark.parametrize("news", [1, 3])
 @pytest.mark.parametrize("dim,pages_whole", [(64, 8), (160, 4)])
 def test_attention_windows_around_a_whole_piece(be, news, dim, pages_whole):
