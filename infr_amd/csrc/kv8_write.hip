@@ -70,24 +70,27 @@ __global__ __launch_bounds__(kThreads) void write_kv8_kernel(Kv8Cache c, Kv8Batc
     const float* src = nullptr;
     if (is_new) src = x + (size_t)(q.r0 + tok - slot0) * stride + (size_t)h * c.dim;
     else if (is_old && tail_ok) src = c.tail + tail_at + (size_t)(tok - open) * c.dim;
-    const bool vec = c.dim % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+    auto load = [&](const float* src) {
+        const bool vec = c.dim % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
 #pragma unroll
-    for (int j = 0; j < kGroups; ++j) {
-        const int d0 = j * 64 + col;
-        if (src && vec && d0 + 16 <= c.dim) {
+        for (int j = 0; j < kGroups; ++j) {
+            const int d0 = j * 64 + col;
+            if (src && vec && d0 + 16 <= c.dim) {
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const float4 y = *reinterpret_cast<const float4*>(src + d0 + e);
-                r[j][e] = y.x, r[j][e + 1] = y.y, r[j][e + 2] = y.z, r[j][e + 3] = y.w;
+                for (int e = 0; e < 16; e += 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(src + d0 + e);
+                    r[j][e] = y.x, r[j][e + 1] = y.y, r[j][e + 2] = y.z, r[j][e + 3] = y.w;
+                }
+            } else if (src) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) r[j][e] = d0 + e < c.dim ? src[d0 + e] : 0.0f;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) r[j][e] = 0.0f;
             }
-        } else if (src) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) r[j][e] = d0 + e < c.dim ? src[d0 + e] : 0.0f;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) r[j][e] = 0.0f;
         }
-    }
+    };
+    load(src);
     if (is_old && !raw)  // rows the tail does not have: at their values in the cache
 #pragma unroll
         for (int j = 0; j < kGroups; ++j)
@@ -163,16 +166,28 @@ __global__ __launch_bounds__(kThreads) void write_kv8_kernel(Kv8Cache c, Kv8Batc
     const int last = (q.len - 1) / c.block * c.block;    // first token of that block
     const int lpage = b.pages[(size_t)s * b.max_pages + last / kPage];
     const bool lpage_ok = lpage >= 0 && lpage < c.n_pages;
-    if (last == open && is_old && !raw && page_ok)       // rows only the cache had, at their values there
+    int row = tok - last;  // of the tail; this thread's token when its page has the block
+    bool put = tok >= last && (is_new || (is_old && !raw && page_ok));  // (rows only the cache had go there at their values)
+    if (pi != last / kPage) {
+        row = t;
+        put = last + t < q.len;
+        load(put ? x + (size_t)(q.r0 + last + t - slot0) * stride + (size_t)h * c.dim : nullptr);
+    }
+    if (put) {
+        float* to = c.tail + tail_at + (size_t)row * c.dim;
 #pragma unroll
-        for (int j = 0; j < kGroups; ++j)
+        for (int j = 0; j < kGroups; ++j) {
+            const int d0 = j * 64 + col;
+            if (c.dim % 4 == 0 && d0 + 16 <= c.dim) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (j * 64 + col + e < c.dim) c.tail[tail_at + (size_t)(tok - open) * c.dim + j * 64 + col + e] = r[j][e];
-    const int from = max(last, slot0), n = (q.len - from) * c.dim;
-    for (int i = tid; i < n; i += kThreads) {
-        const int o = i / c.dim, d = i % c.dim;
-        c.tail[tail_at + (size_t)(from - last + o) * c.dim + d] = x[(size_t)(q.r0 + from - slot0 + o) * stride + (size_t)h * c.dim + d];
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<float4*>(to + d0 + e) = make_float4(r[j][e], r[j][e + 1], r[j][e + 2], r[j][e + 3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (d0 + e < c.dim) to[d0 + e] = r[j][e];
+            }
+        }
     }
     if (tid == 0) {
         tag[0] = lpage_ok ? lpage * subs + last % kPage / c.block : -1;
