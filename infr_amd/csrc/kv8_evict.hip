@@ -11,9 +11,9 @@
 //           pages allow. A block whose tokens come whole and in place from one block keeps its codes and scale; the
 //           others are quantized again from code * scale. Bound by the lines of V that hold any kept token, and by how
 //           fast pieces of 64 bytes from all over the cache come in.
-// Measured (8 heads of 128): eight sequences of 9000 to 32000 tokens cut to 4096 99.7 us, 29 us select and 70 us move, which
+// Measured (8 heads of 128): eight sequences of 9000 to 32000 tokens cut to 4096 98.6 us, 28 us select and 70 us move, which
 // reads 121 MB and writes 68 (2.7 TB/s; without the gathers of V 34 us less; V's codes through LDS for 8-byte stores, or
-// neighbouring new pages on one XCD: no less). Four of 1050 to 1100 tokens cut to 1024: 19.2 us.
+// neighbouring new pages on one XCD: no less). Four of 1050 to 1100 tokens cut to 1024: 17.4 us.
 #include <type_traits>
 
 #include "kv8.hpp"

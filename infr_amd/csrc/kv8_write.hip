@@ -10,8 +10,9 @@
 // token, 16 columns each, so that a token's 64 columns are one 256-byte read and its key codes one 64-byte
 // segment; value codes turn in LDS. Bound by HBM on 8 bytes read and 2 written per column of a token; a single
 // token per sequence is bound by the launch and four dependent loads (tables, page, tag and tail, codes).
-// Measured (8 heads of 128): 8192 tokens of four prompts 23.8 us, 3.5 TB/s read and written (a copy: 5.1); one token
-// of each of 64 sequences 8.3 us.
+// Measured (8 heads of 128): 8192 tokens of four prompts 17.9 us, 4.6 TB/s read and written (a copy: 5.1); one token
+// of each of 64 sequences 8.2 us. (More workgroups on a compute unit by fewer registers spill: 30 us and 18. Codes only
+// where a wave has tokens to write: 19.4 us, the branches keep the loads apart.)
 #include <algorithm>
 #include <type_traits>
 
