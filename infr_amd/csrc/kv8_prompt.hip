@@ -431,21 +431,30 @@ int tiles_of(int group, int max_q, int ks) {
     return (int)(((int64_t)max_q * group + rows - 1) / rows);
 }
 
-// How a call is cut up. Two waves to 32 rows halve a workgroup's time per page and double what is spent on bringing pages
-// into LDS: better while the time is that of the longest row tiles, which is up to four tiles of 128 rows for a compute
-// unit (one / two ways, 32 heads of 128, 8 KV heads: 512 tokens 30 / 22 us, 1024 51 / 40, 2048 104 / 99, four times 1024
-// 109 / 125, 4096 300 / 328; three packed prompts, 16 heads of 80: 88 / 67).
+// How a call is cut up.
 struct Cut {
     int ks, tiles, parts;
 };
-Cut cut_of(int cus, int n_kv, int group, int n_seq, int max_q, int max_pages) {
+// Row tiles for waves that share rows by ks, and the parts their pages are cut into: enough for two workgroups on each
+// compute unit, of at least eight pages.
+Cut cut_for(int ks, int cus, int n_kv, int group, int n_seq, int max_q, int max_pages) {
     Cut c;
-    c.ks = (int64_t)n_seq * n_kv * tiles_of(group, max_q, 1) < (int64_t)4 * cus ? 2 : 1;
-    c.tiles = tiles_of(group, max_q, c.ks);
-    // pieces each row tile's pages are cut into: enough for two workgroups on each compute unit, of at least eight pages
+    c.ks = ks;
+    c.tiles = tiles_of(group, max_q, ks);
     const int64_t wgs = (int64_t)n_seq * n_kv * c.tiles;
     c.parts = (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus / wgs, max_pages / 8));
     return c;
+}
+// Two waves to 32 rows halve a workgroup's time per page and double what is spent on bringing pages into LDS: better while
+// the time is that of the longest row tiles, which is up to four tiles of 128 rows for a compute unit (one / two ways, 32
+// heads of 128, 8 KV heads: 512 tokens 30 / 22 us, 1024 51 / 40, 2048 104 / 99, four times 1024 109 / 125, 4096 300 / 328;
+// three packed prompts, 16 heads of 80: 88 / 67), two with more than 128 columns, where a compute unit holds one workgroup
+// (256 columns: 1024 tokens 96 / 80, 2048 197 / 252). Not where the twice as many tiles leave less than half the parts
+// (300 rows each behind 3000 and 1500 tokens, three parts / one: 82 / 98).
+Cut cut_of(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages) {
+    const Cut one = cut_for(1, cus, n_kv, group, n_seq, max_q, max_pages), two = cut_for(2, cus, n_kv, group, n_seq, max_q, max_pages);
+    const bool few = (int64_t)n_seq * n_kv * one.tiles < (int64_t)(dim <= 128 ? 4 : 2) * cus;
+    return few && 2 * two.parts >= one.parts ? two : one;
 }
 
 template <int DP, int DC, int KS>
@@ -467,7 +476,7 @@ void launch_prompt_ks(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, fl
 template <int DP, int DC>
 void launch_prompt_dc(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch, int cus,
                       hipStream_t stream) {
-    const Cut cut = cut_of(cus, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);
+    const Cut cut = cut_of(cus, c.dim, c.n_kv, a.group, b.n_seq, b.max_q, b.max_pages);
     if (cut.ks == 2) launch_prompt_ks<DP, DC, 2>(c, b, a, dst, lse, scratch, cut, stream);
     else launch_prompt_ks<DP, DC, 1>(c, b, a, dst, lse, scratch, cut, stream);
 }
@@ -484,7 +493,7 @@ bool prompt_takes(int max_q, int group) {
     return (int64_t)max_q * group > 32;
 }
 size_t prompt_scratch(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages) {
-    const Cut cut = cut_of(cus, n_kv, group, n_seq, max_q, max_pages);
+    const Cut cut = cut_of(cus, dim, n_kv, group, n_seq, max_q, max_pages);
     const size_t dp = (size_t)(dim + 63) / 64 * 64, rows = kCols * kWaves / cut.ks;
     return cut.parts == 1 ? 0 : (size_t)n_seq * n_kv * cut.tiles * cut.parts * (rows * dp + 2 * rows) * sizeof(float);
 }
