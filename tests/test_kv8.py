@@ -456,6 +456,27 @@ def test_attention_modes_in_a_batch_of_many_rows(be, type_, kw, dim, n_head, new
 
 
 @gpu
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("dim", [64, 200])
+@pytest.mark.parametrize("kw", [{}, dict(softcap=30.0, window=700, slopes=True, prefix=True, first=True), dict(causal=False)], ids=str)
+def test_attention_of_a_chunk_in_three_parts(be, type_, dim, kw):
+    """Tiles of 128 rows whose pages are cut into parts: a bound on the rows that leaves a few workgroups to each tile."""
+    rng = np.random.default_rng(dim)
+    rows, news, lens = 10240, (150,), (2000,)
+    c, pages, _ = filled(rng, type_, 64, 2, dim, lens)
+    m = mode_of(kw, 2, news, lens, rng)
+    if m.first is not None:
+        m.first = np.concatenate([m.first, np.zeros(rows - len(m.first), int)])
+    b = orc.Batch(list(news), list(lens), pages, rows=rows, max_q=rows, max_pages=40)
+    q = rng.standard_normal((rows, 2 * dim)).astype(np.float32)
+    out, lse = Dev(be, c).attention(b, m, q)
+    want, want_l, tol, ltol = orc.attention(c, b, m, q)
+    close(out, want, tol)
+    close(lse, want_l, ltol)
+    assert (out[150:] == 7.0).all()
+
+
+@gpu
 @pytest.mark.parametrize("news", [(1,), (2,), (40,)])
 def test_attention_over_positions_with_gaps(be, news):
     """As after an eviction: positions ascend with gaps, the masks and the bias go by them."""
