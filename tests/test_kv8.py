@@ -953,6 +953,35 @@ def test_plans_that_share_the_scratch(be):
 
 
 @gpu
+def test_two_backends_at_once(be):
+    """Calls of two backends, each on its own stream and scratch, that nothing waits between."""
+    rng = np.random.default_rng(35)
+    other = I.HipBackend(0)
+    try:
+        calls = []
+        for k in range(6):
+            owner = (be, other)[k % 2]
+            c, pages, _ = filled(rng, "i8", 16, 2, 64, (2500 + k, 70))
+            b = orc.Batch([1 + k, 40], [2500 + k, 70], pages)
+            m = orc.Mode(4, window=0 if k < 3 else 900)
+            q = rng.standard_normal((b.rows, 256)).astype(np.float32)
+            dev = Dev(owner, c)
+            up = owner.upload_new
+            op = AttentionKv8(up(q), dev.cache, up(np.zeros((b.rows, 256), np.float32)), geom=geom_of(c), batch=batch_of(b),
+                              lse=up(np.zeros((b.rows, 4), np.float32)), **dev.tables(b), **dev.mode(m))
+            calls.append((owner, op, orc.attention(c, b, m, q)))
+        for _ in range(20):
+            for owner, op, _ in calls:
+                owner.run_kv8(op)
+        for owner, op, (want, want_l, tol, ltol) in calls:
+            close(owner.download(op.dst, np.empty(want.shape, np.float32)), want, tol)
+            close(owner.download(op.lse, np.empty(want_l.shape, np.float32)), want_l, ltol)
+    finally:
+        calls = dev = op = None  # its buffers go first
+        other.close()
+
+
+@gpu
 def test_refusals_of_operands(be):
     rng = np.random.default_rng(32)
     c, pages, _ = filled(rng, "i8", 16, 2, 64, (70,))
