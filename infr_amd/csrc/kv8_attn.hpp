@@ -11,9 +11,6 @@ size_t step_scratch(int cus, int dim, int n_kv, int group, int n_seq, int max_q,
 void launch_attention_step(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch,
                            int cus, hipStream_t stream);
 
-// Whether the form for many rows takes this shape (its tiles of 128 rows, at 32 a quarter full, against two tiles of 16
-// of the other: drafts of 16 sequences).
-bool prompt_takes(int max_q, int group);
 size_t prompt_scratch(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages);
 void launch_attention_prompt(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, float* dst, float* lse, float* scratch,
                              int cus, hipStream_t stream);

@@ -489,9 +489,6 @@ void launch_prompt_dp(const Kv8Cache& c, const Kv8Batch& b, const Kv8Attn& a, fl
 
 }  // namespace
 
-bool prompt_takes(int max_q, int group) {
-    return (int64_t)max_q * group > 32;
-}
 size_t prompt_scratch(int cus, int dim, int n_kv, int group, int n_seq, int max_q, int max_pages) {
     const Cut cut = cut_of(cus, dim, n_kv, group, n_seq, max_q, max_pages);
     const size_t dp = (size_t)(dim + 63) / 64 * 64, rows = kCols * kWaves / cut.ks;
