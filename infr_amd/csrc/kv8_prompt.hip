@@ -69,13 +69,14 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
 
     // Tokens the row can see at all lie in [lo, hi): positions ascend strictly and are not negative, so a token is at
     // least as far from the row in positions as in tokens, and none with a position below `prefix` lies behind it. A
-    // document that begins behind the row has none of the tokens up to the row's own.
+    // document that begins behind the row has none of the tokens up to the row's own; one that begins at 0 or before has
+    // all there are (and a distance to it may not fit an int).
     int lo = 0x7FFFFFFF, hi = 0;
     if (live && q.ok) {
         const int slot = q.len - q.n + i;
         lo = 0;
         if (a.window > 0) lo = max(lo, slot - a.window + 1);
-        if (a.first) lo = max(lo, row.pos >= row.first ? slot - (row.pos - row.first) : slot + 1);
+        if (a.first && row.first > 0) lo = max(lo, row.pos >= row.first ? slot - (row.pos - row.first) : slot + 1);
         hi = a.causal ? max(slot + 1, min(a.prefix ? row.prefix : 0, q.len)) : q.len;
     }
     int last_pos = live ? row.pos : -0x7FFFFFFF - 1, last_first = live ? row.first : -0x7FFFFFFF - 1;

@@ -51,3 +51,20 @@ def test_documents_that_begin_behind_every_row(be, type_, kw, form, news):
     sums, stol = orc.score(c, b, m, q, lse, 1.0)
     dev.score(b, m, q, lse)
     assert (np.abs(dev.pull().sums - sums) <= stol).all()
+
+
+@gpu
+@pytest.mark.parametrize("form,news", [("few rows", 3), ("64 rows", 150), ("128 rows", 150), ("128 rows in parts", 150)])
+@pytest.mark.parametrize("first", [-2 ** 31, -2 ** 31 + 5, -1])
+def test_documents_that_begin_before_all_positions(be, form, news, first):
+    """No position is negative: such a document's beginning masks nothing, also where positions have gaps."""
+    rng = np.random.default_rng(41)
+    n_len = 180
+    pos = np.cumsum(rng.integers(1, 6, n_len)).astype(np.int32)
+    c, pages, _ = filled(rng, "i8", 32, 2, 64, (n_len,), pos=pos)
+    b = batch_in_form(form, (news,), (n_len,), pages, pos=pos[n_len - news:])
+    q = rng.standard_normal((b.rows, 4 * 64)).astype(np.float32)
+    out, lse = Dev(be, c).attention(b, orc.Mode(4, first=np.full(b.rows, first)), q)
+    want, want_l, tol, ltol = orc.attention(c, b, orc.Mode(4), q)
+    close(out, want, tol)
+    close(lse, want_l, ltol)
