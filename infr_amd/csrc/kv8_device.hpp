@@ -161,15 +161,27 @@ __device__ __forceinline__ void cap_scores(X& x, float c, float inv_c) {
     }
 }
 
-// A block's value scale as the weights' exponent: log2 of scale / 2^v_exp. Blocks 2^60 below the largest scale count as
-// if they were that near: nothing of them reaches the result, and the weights keep clear of the smallest numbers.
-__device__ __forceinline__ float scale_log(float scale, int v_exp) {
-    const float l = __builtin_amdgcn_logf(scale * __builtin_amdgcn_exp2f(-(float)max(v_exp, -126)));
-    return l >= -60.0f ? l : l < -60.0f ? -60.0f : 0.0f;  // a NaN scale is the caller's
+// Softmax weights go into P.V times the scale of their value's block and 2^(kBias - v_exp). v_exp follows the largest product
+// of weight and scale, so that what carries the row keeps its bits however far its scale is below that of a block of next
+// to no weight (with v_exp by the scales alone, a block 2^24 below such a one lost 8e-5 of its sum, at 2^36 all of it).
+// Weights count from the running maximum `top`, and so does v_exp; both may lag behind by 2^kLag, which keeps the
+// products below 2^15 (f16 ends at 2^16). The largest one stands at 2^9 or above: what is 2^-34 of it is below f16's
+// smallest numbers and rounded away.
+constexpr int kBias = 11;
+constexpr float kLag = 4.0f;
+constexpr float kNoExp = -400.0f;  // v_exp before the first token: below any product's exponent
+
+// Exponent that the product of a block's scale and its largest weight stays below; -inf for a NaN scale and where no
+// token is seen (`high` is -inf then).
+__device__ __forceinline__ float product_exponent(float scale, float high, float top) {
+    const int e = (int)((__builtin_bit_cast(uint32_t, scale) >> 23) & 255u) - 126;
+    return scale < __builtin_inff() ? (float)e + (high - top) : -__builtin_inff();
 }
-// The scale's exponent; -200 for a NaN scale and for blocks no token of which is seen.
-__device__ __forceinline__ int scale_exponent(float scale, bool any) {
-    return any && scale < __builtin_inff() ? (int)((__builtin_bit_cast(uint32_t, scale) >> 23) & 255u) - 127 : -200;
+// A block's value scale as the weights' exponent: log2 of scale / 2^v_exp. Weights of 2^-60 and less are 0 in f16, and from
+// there on the exponent stays as it is, so that their sum, which is divided by it again, keeps clear of the smallest numbers.
+__device__ __forceinline__ float scale_log(float scale, float v_exp) {
+    const float l = __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(scale)) + ((float)__builtin_amdgcn_frexp_expf(scale) - v_exp);
+    return scale < __builtin_inff() ? fmaxf(l, -60.0f) : 0.0f;  // a NaN scale is the caller's
 }
 
 // What one query row sees, and its bias.

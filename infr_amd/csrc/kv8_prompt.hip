@@ -23,8 +23,6 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kCols = 32;                // query rows of a wave
-constexpr int kBias = 10;
-constexpr float kLag = 4.0f;
 
 // Waves that share 32 query rows, each with 64 / KS tokens of every page; rows of a workgroup.
 template <int KS>
@@ -147,7 +145,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
 #pragma unroll
     for (int k = 0; k < kOut; ++k) o[k] = (f16x)(0.0f);
     float top = kNoMax, sum = 0.0f;
-    int v_exp = -200;
+    float v_exp = kNoExp;  // O's unit: 2^v_exp / 2^kBias
     bool bad = !q.ok, v_bad = false;  // v_bad: the row sees a token whose value is NaN
 
     const int32_t* table = b.pages + (size_t)s * b.max_pages;
@@ -233,9 +231,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
             const bool masked = (p + 1) * kPage > min(full_hi, q.len) ||
                                 (use_pos && (last_pos - st.pos[0] >= row.window || last_first > st.pos[0]));
             const bool bent = GEN && (a.softcap > 0.0f || a.slopes);
-            float high = -__builtin_inff(), factor[kHalves], vs[kHalves];
+            float high = -__builtin_inff(), factor[kHalves], vs[kHalves], highs[kHalves];
             bool any[kHalves];
-            int e_now = -200;
 #pragma unroll
             for (int t = 0; t < kHalves; ++t) {
                 factor[t] = row_factor * st.ks[2 * (half0 + t) + hf];
@@ -274,8 +271,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
                 float most = x[t][0];
 #pragma unroll
                 for (int e = 1; e < 16; ++e) most = fmaxf(most, x[t][e]);
-                high = fmaxf(high, most * factor[t]);
-                e_now = max(e_now, scale_exponent(vs[t], any[t]));
+                highs[t] = most * factor[t];
+                high = fmaxf(high, highs[t]);
             }
             if (__any(fabsf(high) > kLargeScore))
 #pragma unroll
@@ -284,12 +281,16 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
                     for (int e = 0; e < 16; ++e) x[t][e] *= factor[t];
                     factor[t] = 1.0f;
                 }
-            if (__any(high > top + kLag || e_now > v_exp)) {
-                const float new_top = fmaxf(top, halves_max(high));
-                const int new_exp = max(v_exp, (int)halves_max((float)e_now));
-                const float keep = __builtin_amdgcn_exp2f(top - new_top);
-                const float keep_o = v_exp == -200 ? 0.0f : keep * __builtin_amdgcn_exp2f((float)(v_exp - new_exp));
-                sum *= keep;
+            auto product = [&](float over) {
+                float e = product_exponent(vs[0], highs[0], over);
+                if (kHalves == 2) e = fmaxf(e, product_exponent(vs[kHalves - 1], highs[kHalves - 1], over));
+                return e;
+            };
+            if (__any(high > top + kLag || product(top) > v_exp + kLag)) {
+                const float new_top = fmaxf(top, halves_max(high)), down = top - new_top;
+                const float new_exp = fmaxf(fmaxf(__builtin_ceilf(v_exp + down), __builtin_ceilf(halves_max(product(new_top)))), kNoExp);
+                const float keep_o = __builtin_amdgcn_exp2f(v_exp + down - new_exp);
+                sum *= __builtin_amdgcn_exp2f(down);
 #pragma unroll
                 for (int k = 0; k < kOut; ++k) o[k] *= keep_o;
                 top = new_top;
@@ -338,16 +339,15 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
                 for (int e = 0; e < 16; ++e) mine[(k * 16 + e) * 64] = o[k][e];
             mine[kOut * 16 * 64] = top;
             mine[(kOut * 16 + 1) * 64] = sum;
-            mine[(kOut * 16 + 2) * 64] = (float)v_exp;
+            mine[(kOut * 16 + 2) * 64] = v_exp;
             mine[(kOut * 16 + 3) * 64] = v_bad ? 1.0f : 0.0f;
         }
         __syncthreads();
         if (half0 == 1) return;
         const float top2 = mine[kOut * 16 * 64], new_top = fmaxf(top, top2);
-        const int exp2 = (int)mine[(kOut * 16 + 2) * 64], new_exp = max(v_exp, exp2);
+        const float e1 = v_exp + (top - new_top), e2 = mine[(kOut * 16 + 2) * 64] + (top2 - new_top), new_exp = fmaxf(fmaxf(e1, e2), kNoExp);
         const float f1 = __builtin_amdgcn_exp2f(top - new_top), f2 = __builtin_amdgcn_exp2f(top2 - new_top);
-        const float o1 = v_exp == -200 ? 0.0f : f1 * __builtin_amdgcn_exp2f((float)(v_exp - new_exp));
-        const float o2 = exp2 == -200 ? 0.0f : f2 * __builtin_amdgcn_exp2f((float)(exp2 - new_exp));
+        const float o1 = __builtin_amdgcn_exp2f(e1 - new_exp), o2 = __builtin_amdgcn_exp2f(e2 - new_exp);
 #pragma unroll
         for (int k = 0; k < kOut; ++k)
 #pragma unroll
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
 #pragma unroll
         for (int k = 0; k < kOut; ++k) o[k] = (f16x)(__builtin_nanf(""));
     if (!live) return;
-    const float nan = __builtin_nanf(""), up = __builtin_amdgcn_exp2f((float)max(v_exp, -126));
+    const float nan = __builtin_nanf(""), up = __builtin_amdgcn_exp2f(v_exp);
     if (parts > 1) {
         float* piece = scratch + ((((size_t)s * c.n_kv + h) * tiles + rt) * parts + part) * kPieceFloats<DP, KS>;
         const int r = wave / KS * kCols + col;

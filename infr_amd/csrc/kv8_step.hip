@@ -27,8 +27,6 @@ namespace {
 // Waves of a workgroup that take TOK tokens of a page at a time: together four pages.
 template <int TOK>
 constexpr int kWaves = kPage / TOK * kStepWaves;
-constexpr int kBias = 10;    // softmax weights are 2^kBias at the running maximum ..
-constexpr float kLag = 4.0f; // .. which may lag behind the true one by this many powers of two
 
 // O, maxima and sums of a piece: f32 [rows][DP], then [rows] pairs of a maximum and a sum.
 template <int DP, int ROWS>
@@ -81,7 +79,7 @@ __global__ __launch_bounds__(64 * kWaves<TOK>, DP == 64 ? 3 : DP == 128 || (DP =
 #pragma unroll
     for (int k = 0; k < kOut; ++k) o[k] = f4{0, 0, 0, 0};
     float top = kNoMax, sum = 0.0f;
-    int v_exp = -200;       // values are scaled by 2^-v_exp
+    float v_exp = kNoExp;  // O's unit: 2^v_exp / 2^kBias
     bool bad = !q.ok, v_bad = false;  // v_bad: the row sees a token whose value is NaN
 
     const int32_t* table = b.pages + (size_t)s * b.max_pages;
@@ -212,13 +210,11 @@ __global__ __launch_bounds__(64 * kWaves<TOK>, DP == 64 ? 3 : DP == 128 || (DP =
             for (int e = 0; e < kMine; ++e) x[e] *= f;
             f = 1.0f;
         }
-        const int e_now = scale_exponent(vs_now, any);
-        if (__any(high > top + kLag || e_now > v_exp)) {
-            const float new_top = fmaxf(top, quads_max(high));
-            const int new_exp = max(v_exp, (int)quads_max((float)e_now));
-            const float keep = __builtin_amdgcn_exp2f(top - new_top);
-            const float keep_o = v_exp == -200 ? 0.0f : keep * __builtin_amdgcn_exp2f((float)(v_exp - new_exp));
-            sum *= keep;
+        if (__any(high > top + kLag || product_exponent(vs_now, high, top) > v_exp + kLag)) {
+            const float new_top = fmaxf(top, quads_max(high)), down = top - new_top;
+            const float new_exp = fmaxf(fmaxf(__builtin_ceilf(v_exp + down), __builtin_ceilf(quads_max(product_exponent(vs_now, high, new_top)))), kNoExp);
+            const float keep_o = __builtin_amdgcn_exp2f(v_exp + down - new_exp);
+            sum *= __builtin_amdgcn_exp2f(down);
 #pragma unroll
             for (int k = 0; k < kOut; ++k) o[k] *= keep_o;
             top = new_top;
@@ -284,7 +280,7 @@ __global__ __launch_bounds__(64 * kWaves<TOK>, DP == 64 ? 3 : DP == 128 || (DP =
 #pragma unroll
     for (int k = 0; k < kWaves; ++k) all_top = fmaxf(all_top, part_m[k][col]);
     // (a wave that has seen nothing has sum 0 and O 0; exp2 of its maximum's distance is 0)
-    const float mine = __builtin_amdgcn_exp2f(top - all_top) * (v_exp == -200 ? 0.0f : __builtin_amdgcn_exp2f((float)v_exp));
+    const float mine = __builtin_amdgcn_exp2f(v_exp + (top - all_top));
 #pragma unroll
     for (int k = 0; k < kOut; ++k) {
         f4 y = o[k];

@@ -68,3 +68,69 @@ def test_documents_that_begin_before_all_positions(be, form, news, first):
     want, want_l, tol, ltol = orc.attention(c, b, orc.Mode(4), q)
     close(out, want, tol)
     close(lse, want_l, ltol)
+
+
+# ---------------------------------------------------------------- weights
+
+def weights_of(c, b, m, q, head):
+    """(p, largest p is 1; scores; which pairs see each other; sum |q k| of each pair) of sequence 0, f64 [rows, tokens]."""
+    n, n_len = int(b.q_start[1]), int(b.lens[0])
+    sc, see, size = orc.scores(c, b, m, q, 0, 0, n, n_len, head)
+    sc = np.where(see, sc, -np.inf)
+    return np.exp(sc - sc.max(-1, keepdims=True)), sc, see, size
+
+
+def relative_tolerance(c, b, m, q, head):
+    """What the weighted sum of values may be off, [rows, dim], relative to the sum of |weight * value| of its column.
+
+    A weight is off by its score's error (a sum of dim products, 2^-24 for each addition and 2^-22 for the operand and the
+    products' roundings, each of |q k|; 2^-21 of the score itself, which counts in log2 units from the row's largest;
+    2^-20 for the exponential and the scales' logarithm) and by 2^-22 for its two halves. Below that a product of weight and scale
+    counts to 2^-33 of the row's largest. The sums over n tokens add n * 2^-24 and the quotient doubles it all."""
+    p, sc, see, size = weights_of(c, b, m, q, head)
+    h = head // (m.n_head // c.n_kv)
+    n_len = int(b.lens[0])
+    v = np.abs(c.values("v", b.pages[0], h, n_len))
+    scale = np.repeat(c.v_scale[b.pages[0, :-(-n_len // 64)], h].reshape(-1).astype(np.float64), c.block)[:n_len]
+    far = np.where(see, sc.max(-1, keepdims=True) - sc, 0)
+    eps = size * (c.dim * 2.0 ** -24 + 2.0 ** -22) + (np.abs(np.where(see, sc, 0)) + far) * 2.0 ** -21 + 2.0 ** -20 + 2.0 ** -22
+    least = (p * scale).max(-1, keepdims=True) * 2.0 ** -33 / scale  # of a weight, in units of p
+    l = p.sum(-1, keepdims=True)
+    return ((p * eps) @ v + (p @ v) * (p * eps).sum(-1, keepdims=True) / l + 2 * n_len * 2.0 ** -24 * (p @ v) + np.where(see, least, 0) @ v) / l
+
+
+@gpu
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("block,at", [(16, 0), (16, 130), (64, 0), (64, 128)])
+@pytest.mark.parametrize("form,news", [("few rows", 1), ("few rows", 7), ("64 rows", 140), ("128 rows", 140), ("128 rows in parts", 140)])
+def test_a_block_of_large_values_and_next_to_no_weight(be, type_, dim, block, at, form, news):
+    """The weight lies on blocks whose scale is far below another visible block's: their values keep their bits."""
+    if dim > 128 and form == "128 rows":
+        pytest.skip("the same code as with 64 columns, on inputs of 130 MB")
+    rng = np.random.default_rng(42)
+    n_len = 150
+    for ratio in (0, 14, 24, 30, 40, 52, 57, 64, 90):
+        c = orc.Cache(5, 2, dim, 1, type_, block)
+        pages = [[4, 0, 2]]
+        new = orc.Batch([n_len], [n_len], pages)
+        k, v = (rng.standard_normal((n_len, 2 * dim)).astype(np.float32) for _ in range(2))
+        k.reshape(n_len, 2, dim)[:, :, 0] = 0
+        big = slice(at, min(at + block, n_len))
+        v[big] *= np.float32(2.0 ** ratio)
+        k[big] = 0
+        k.reshape(n_len, 2, dim)[big, :, 0] = -40
+        orc.write(c, new, k, v)
+        b = batch_in_form(form, (news,), (n_len,), pages)
+        m = orc.Mode(4, scale=1.0, causal=False)
+        q = np.zeros((b.rows, 4, dim), np.float32)
+        q[..., 0] = 1
+        q[:, 1::2, 1:] = 0.03 * rng.standard_normal((b.rows, 2, dim - 1))
+        q = q.reshape(b.rows, -1)
+        out, lse = Dev(be, c).attention(b, m, q)
+        want, want_l, _, ltol = orc.attention(c, b, m, q)
+        close(lse, want_l, ltol)
+        for head in range(4):
+            cols = slice(head * dim, (head + 1) * dim)
+            off = np.abs(out[:news, cols] - want[:news, cols]) / relative_tolerance(c, b, m, q, head)
+            assert off.max() <= 1, f"2^{ratio}, head {head}: {off.max():.3g} tolerances"
