@@ -361,8 +361,8 @@ int infr_hip_write_kv8(infr_hip_t *be, const infr_hip_kv8_params_t *p, const inf
  *   window == 0, or pos_r - pos_j < window
  *   pos_j >= first[r]                                   (i32 [rows], optional: where the row's document begins)
  * A row that sees nothing is 0 with lse = -inf. Operands x (q), cache, dst, pos, pages, q_start, lens, then by has_*
- * first, prefix, slopes (f32 [n_head]), lse. Sums are f32 and f32 operands keep 22 bits in the matrix products; of a
- * softmax weight those count that are above 2^-33 of the row's largest product of a weight and its block's value scale. */
+ * first, prefix, slopes (f32 [n_head]), lse. Sums are f32 and f32 operands keep 23 bits, to the nearest, in the matrix products;
+ * of a softmax weight those count that are above 2^-33 of the row's largest product of a weight and its block's value scale. */
 int infr_hip_attention_kv8(infr_hip_t *be, const infr_hip_kv8_params_t *p, const infr_hip_kv8_operands_t *o);
 
 /* ScoreKv8: sums_j = decay * sums_j + the weights exp(s_rj - lse[r, h]) that the call's rows and the heads of j's

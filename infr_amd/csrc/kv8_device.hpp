@@ -2,9 +2,9 @@
 // numbers, the scores' softcap, bias and masks.
 //
 // Matrix products run on the f16 MFMA. Every code of either type is exact in f16; an f32 operand x goes in as
-// hi + lo, hi = f16(x) and lo = f16(x - hi), two products instead of one, so that 22 bits of it count (f16 alone
+// hi + lo, hi = f16(x) and lo = f16(x - hi), two products instead of one, so that 23 bits of it count (f16 alone
 // would leave 11, which shows in an f32 result). Query rows are scaled by a power of two that puts their largest
-// value at 2^14, softmax weights by 2^10, so that the smallest f16 number stands far below what counts.
+// value at 2^14, softmax weights by 2^11, so that the smallest f16 number stands far below what counts.
 //
 // Layouts follow from S^T = K Q^T: with tokens as the MFMA's rows and query rows as its columns, a lane's scores
 // all belong to one query row, the softmax statistics of a row live in the lanes that hold its output, and the
@@ -55,12 +55,15 @@ __device__ __forceinline__ h8 code_oct(uint32_t a, uint32_t b) {
     return h8{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
 }
 
-// a, b = hi + lo, both rounded towards zero (one instruction for two numbers): 22 bits of each remain.
+// a, b = hi + lo, both rounded to the nearest (one instruction for two numbers): 23 bits of each remain, and what falls off
+// falls to either side.
+__device__ __forceinline__ h2 nearest_pair(float a, float b) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    return __builtin_convertvector(f2{a, b}, h2);
+}
 __device__ __forceinline__ void split_pair(float a, float b, h2* hi, h2* lo) {
-    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-    const auto l = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], -1.0f, a), __builtin_fmaf((float)h[1], -1.0f, b));
-    *hi = __builtin_bit_cast(h2, h);
-    *lo = __builtin_bit_cast(h2, l);
+    *hi = nearest_pair(a, b);
+    *lo = nearest_pair(__builtin_fmaf((float)(*hi)[0], -1.0f, a), __builtin_fmaf((float)(*hi)[1], -1.0f, b));
 }
 
 // f over lanes l and l ^ 32.

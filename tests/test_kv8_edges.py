@@ -134,3 +134,34 @@ def test_a_block_of_large_values_and_next_to_no_weight(be, type_, dim, block, at
             cols = slice(head * dim, (head + 1) * dim)
             off = np.abs(out[:news, cols] - want[:news, cols]) / relative_tolerance(c, b, m, q, head)
             assert off.max() <= 1, f"2^{ratio}, head {head}: {off.max():.3g} tolerances"
+
+
+@gpu
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("form,news", [("few rows", 1), ("few rows", 4), ("few rows", 8), ("64 rows", 64), ("128 rows", 64), ("128 rows in parts", 64)])
+def test_small_weights_are_rounded_to_the_nearest(be, type_, form, news):
+    """One token has all but 2^-19 of the weight and the value 0: what is left are weights near the smallest ones that
+    count, in steps of 2^-24 where the largest product of weight and scale is at 2^10 or above. Each is off by half a step
+    at most, and all of a row by the same."""
+    rng = np.random.default_rng(43)
+    c = orc.Cache(3, 2, 64, 1, type_, 64)
+    pages = [[1]]
+    new = orc.Batch([64], [64], pages)
+    k, v = np.zeros((64, 2, 64), np.float32), np.ones((64, 2, 64), np.float32)
+    k[1:, :, 0] = -1
+    v[0] = 0
+    orc.write(c, new, k.reshape(64, -1), v.reshape(64, -1))
+    b = batch_in_form(form, (news,), (64,), pages)
+    m = orc.Mode(4, scale=1.0, causal=False)
+    q = np.zeros((b.rows, 4, 64), np.float32)
+    q[..., 0] = rng.uniform(16, 18, (b.rows, 4))
+    q = q.reshape(b.rows, -1)
+    out, _ = Dev(be, c).attention(b, m, q)
+    want = orc.attention(c, b, m, q)[0]
+    for head in range(4):
+        cols = slice(head * 64, (head + 1) * 64)
+        p = weights_of(c, b, m, q, head)[0]
+        # half a step of each of 63 weights, of a largest one that stands at 2^10 or above; 2^-16 covers the f32 arithmetic
+        tol = 63 * 2.0 ** -35 / p.sum(-1, keepdims=True) + 2.0 ** -16 * want[:news, cols]
+        off = np.abs(out[:news, cols] - want[:news, cols]) / tol
+        assert off.max() <= 1, f"head {head}: {off.max():.3g} tolerances"
