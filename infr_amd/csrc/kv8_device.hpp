@@ -173,6 +173,9 @@ __device__ __forceinline__ void cap_scores(X& x, float c, float inv_c) {
 constexpr int kBias = 11;
 constexpr float kLag = 4.0f;
 constexpr float kNoExp = -400.0f;  // v_exp before the first token: below any product's exponent
+// A piece of a row's keys leaves its own softmax's output, no larger than the values are, with its maximum and its sum of
+// weights; the latter by 2^-kSumDown, which is below 1 for 2^22 tokens, so that outputs times sums are no larger either.
+constexpr int kSumDown = 40;
 
 // Exponent that the product of a block's scale and its largest weight stays below; -inf for a NaN scale and where no
 // token is seen (`high` is -inf then).

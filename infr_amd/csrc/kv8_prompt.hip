@@ -362,7 +362,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
 #pragma unroll
         for (int k = 0; k < kOut; ++k) o[k] = (f16x)(__builtin_nanf(""));
     if (!live) return;
-    const float nan = __builtin_nanf(""), up = __builtin_amdgcn_exp2f(v_exp);
+    // (the unit comes last: before it the numbers are of ordinary size, whatever the values are)
+    const float nan = __builtin_nanf(""), up = __builtin_amdgcn_exp2f(v_exp), scale = bad ? nan : sum == 0.0f ? 0.0f : 1.0f / sum;
     if (parts > 1) {
         float* piece = scratch + ((((size_t)s * c.n_kv + h) * tiles + rt) * parts + part) * kPieceFloats<DP, KS>;
         const int r = wave / KS * kCols + col;
@@ -370,15 +371,14 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
         for (int k = 0; k < kOut; ++k)
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
-                *reinterpret_cast<f4*>(&piece[r * DP + k * 32 + 2 * e + 4 * hf]) = f4{o[k][e], o[k][e + 1], o[k][e + 2], o[k][e + 3]} * up;
+                *reinterpret_cast<f4*>(&piece[r * DP + k * 32 + 2 * e + 4 * hf]) = f4{o[k][e], o[k][e + 1], o[k][e + 2], o[k][e + 3]} * scale * up;
         if (hf == 0) {
             piece[kRows * DP + r] = top;
-            piece[kRows * DP + kRows + r] = bad ? nan : sum;
+            piece[kRows * DP + kRows + r] = bad ? nan : sum * pow2(-kSumDown);
         }
         return;
     }
     const size_t at = (size_t)(q.r0 + i) * a.n_head + head;
-    const float scale = bad ? nan : sum == 0.0f ? 0.0f : up / sum;
     float* out = dst + at * c.dim;
     const bool vec = c.dim % 4 == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
 #pragma unroll
@@ -386,7 +386,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
             const int d = k * 32 + 2 * e + 4 * hf;
-            const f4 y = f4{o[k][e], o[k][e + 1], o[k][e + 2], o[k][e + 3]} * scale;
+            const f4 y = f4{o[k][e], o[k][e + 1], o[k][e + 2], o[k][e + 3]} * scale * up;
             if (vec) {
                 if (d < c.dim) *reinterpret_cast<f4*>(out + d) = y;
             } else {
@@ -416,8 +416,8 @@ __global__ __launch_bounds__(kThreads) void join_rows_kernel(Kv8Cache c, Kv8Batc
     float x[DP / 64] = {};  // (columns behind head_dim are whatever the scratch held; they are not stored)
     for (int k = 0; k < parts; ++k) {
         const float* piece = first + (size_t)k * kPieceFloats<DP, KS>;
-        const float f = __builtin_amdgcn_exp2f(piece[kRows * DP + r] - m);
-        l += piece[kRows * DP + kRows + r] * f;
+        const float f = piece[kRows * DP + kRows + r] * __builtin_amdgcn_exp2f(piece[kRows * DP + r] - m);
+        l += f;
 #pragma unroll
         for (int j = 0; j < DP / 64; ++j) x[j] += piece[r * DP + j * 64 + lane] * f;
     }
@@ -425,7 +425,7 @@ __global__ __launch_bounds__(kThreads) void join_rows_kernel(Kv8Cache c, Kv8Batc
 #pragma unroll
     for (int j = 0; j < DP / 64; ++j)
         if (j * 64 + lane < c.dim) dst[at * c.dim + j * 64 + lane] = l == 0.0f ? 0.0f : l != l ? l : x[j] / l;
-    if (lse && lane == 0) lse[at] = l == 0.0f ? -__builtin_inff() : (__builtin_amdgcn_logf(l) + m - (float)kBias) * kLn2;
+    if (lse && lane == 0) lse[at] = l == 0.0f ? -__builtin_inff() : (__builtin_amdgcn_logf(l) + m - (float)(kBias - kSumDown)) * kLn2;
 }
 
 int tiles_of(int group, int max_q, int ks) {

@@ -28,7 +28,7 @@ namespace {
 template <int TOK>
 constexpr int kWaves = kPage / TOK * kStepWaves;
 
-// O, maxima and sums of a piece: f32 [rows][DP], then [rows] pairs of a maximum and a sum.
+// Outputs, maxima and sums of a piece: f32 [rows][DP], then [rows] pairs of a maximum and a sum.
 template <int DP, int ROWS>
 constexpr int kPieceFloats = ROWS * DP + 2 * ROWS;
 
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(64 * kWaves<TOK>, DP == 64 ? 3 : DP == 128 || (DP =
     constexpr bool PACK = ROWS == 8;   // columns 8..15 are the low parts of columns 0..7
     __shared__ __align__(16) float part_o[kWaves * kPart];  // the waves' outputs; before, the query rows
     static_assert(sizeof(StepQ<DP, ROWS>) <= sizeof(part_o), "the rows fit");
-    __shared__ float part_m[kWaves][16], part_l[kWaves][16];
+    __shared__ float part_m[kWaves][16], part_l[kWaves][16], part_e[kWaves][16], row_e[16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const SeqCut cut = find_cut(b, a, c.n_kv, ROWS, target, whole_pages, false, -1, (int)blockIdx.x);
     if (cut.s < 0) return;
@@ -274,13 +274,17 @@ __global__ __launch_bounds__(64 * kWaves<TOK>, DP == 64 ? 3 : DP == 128 || (DP =
     if (g == 0) {
         part_m[wave][col] = top;
         part_l[wave][col] = sum;
+        part_e[wave][col] = v_exp;
     }
     const bool any_bad = __syncthreads_or(bad) != 0;
-    float all_top = kNoMax;
+    float all_top = kNoMax, all_exp = kNoExp;
 #pragma unroll
     for (int k = 0; k < kWaves; ++k) all_top = fmaxf(all_top, part_m[k][col]);
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) all_exp = fmaxf(all_exp, part_e[k][col] + (part_m[k][col] - all_top));
+    if (wave == 0 && g == 0) row_e[col] = all_exp;
     // (a wave that has seen nothing has sum 0 and O 0; exp2 of its maximum's distance is 0)
-    const float mine = __builtin_amdgcn_exp2f(v_exp + (top - all_top));
+    const float mine = __builtin_amdgcn_exp2f(v_exp + (top - all_top) - all_exp);
 #pragma unroll
     for (int k = 0; k < kOut; ++k) {
         f4 y = o[k];
@@ -323,14 +327,15 @@ __global__ __launch_bounds__(64 * kWaves<TOK>, DP == 64 ? 3 : DP == 128 || (DP =
         }
 #pragma unroll
         for (int k = 0; k < kWaves; ++k) l += part_l[k][r] * __builtin_amdgcn_exp2f(part_m[k][r] - m);
+        // (the unit comes last: before it the numbers are of ordinary size, whatever the values are)
+        x = x * (l == 0.0f ? 0.0f : 1.0f / l) * __builtin_amdgcn_exp2f(row_e[r]);
         if (any_bad) x = f4{nan, nan, nan, nan}, l = nan;
         if (!whole) {
             *reinterpret_cast<f4*>(piece + r * DP + d) = x;
-            if (d == 0) *reinterpret_cast<float2*>(piece + ROWS * DP + 2 * r) = make_float2(m, l);
+            if (d == 0) *reinterpret_cast<float2*>(piece + ROWS * DP + 2 * r) = make_float2(m, l * pow2(-kSumDown));
             continue;
         }
-        const float scale = l == 0.0f ? 0.0f : 1.0f / l;
-        store_out(r, d, x * scale);
+        store_out(r, d, x);
         if (lse && d == 0) lse[out_row(r)] = lse_of(l, m);
     }
 }
@@ -375,8 +380,8 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8Cache c, Kv8Batch b, Kv8At
             x *= old;
 #pragma unroll
             for (int n = 0; n < kAhead; ++n) {
-                const float f = __builtin_amdgcn_exp2f(ml[n].x - most);
-                l = __builtin_fmaf(ml[n].y, f, l);
+                const float f = ml[n].y * __builtin_amdgcn_exp2f(ml[n].x - most);
+                l += f;
                 if (k0 + n * kGroups < parts) x += y[n] * f;
             }
             m = most;
@@ -401,7 +406,7 @@ __global__ __launch_bounds__(256) void join_kernel(Kv8Cache c, Kv8Batch b, Kv8At
     }
     const size_t out = (size_t)(q.r0 + r_all / a.group) * a.n_head + h * a.group + r_all % a.group;
     dst[out * c.dim + d] = l == 0.0f ? 0.0f : y / l;
-    if (lse && d == 0) lse[out] = l == 0.0f ? -__builtin_inff() : (__builtin_amdgcn_logf(l) + m - (float)kBias) * kLn2;
+    if (lse && d == 0) lse[out] = l == 0.0f ? -__builtin_inff() : (__builtin_amdgcn_logf(l) + m - (float)(kBias - kSumDown)) * kLn2;
 }
 
 // Query rows of a workgroup: 8 where no sequence has more.

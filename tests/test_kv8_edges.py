@@ -165,3 +165,27 @@ def test_small_weights_are_rounded_to_the_nearest(be, type_, form, news):
         tol = 63 * 2.0 ** -35 / p.sum(-1, keepdims=True) + 2.0 ** -16 * want[:news, cols]
         off = np.abs(out[:news, cols] - want[:news, cols]) / tol
         assert off.max() <= 1, f"head {head}: {off.max():.3g} tolerances"
+
+
+@gpu
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("dim", [64, 200])
+@pytest.mark.parametrize("size", [2.0 ** 100, 2.0 ** 125])
+@pytest.mark.parametrize("form,news,n_len", [("few rows", 1, 150), ("few rows", 7, 150), ("few rows", 1, 3001), ("64 rows", 140, 150), ("128 rows", 140, 150),
+                                             ("128 rows in parts", 140, 1500)])
+def test_values_next_to_the_largest(be, type_, dim, size, form, news, n_len):
+    """Weighted means of finite values are finite."""
+    rng = np.random.default_rng(44)
+    c = orc.Cache(-(-n_len // 64), 1, dim, 1, type_, 16)
+    pages = [rng.permutation(c.n_pages).tolist()]
+    new = orc.Batch([n_len], [n_len], pages)
+    k = rng.standard_normal((n_len, dim)).astype(np.float32)
+    v = (rng.uniform(0.5, 1.5, (n_len, dim)) * size).astype(np.float32)
+    orc.write(c, new, k, v)
+    b = batch_in_form(form, (news,), (n_len,), pages)
+    m = orc.Mode(4)
+    q = rng.standard_normal((b.rows, 4 * dim)).astype(np.float32)
+    out, lse = Dev(be, c).attention(b, m, q)
+    want, want_l, tol, ltol = orc.attention(c, b, m, q)
+    close(out, want, tol)
+    close(lse, want_l, ltol)
