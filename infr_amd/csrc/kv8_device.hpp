@@ -125,21 +125,23 @@ __device__ __forceinline__ bool rows_vec(const Kv8Cache& c, const Kv8Attn& a) {
     return c.dim % 4 == 0 && a.q_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0;
 }
 
+// 1 / c, finite for every c > 0: a score of 0 is capped to 0, whatever c is.
+__device__ __forceinline__ float inverse_cap(float c) { return c > 0.0f ? fminf(1.0f / c, 3.4028234e38f) : 0.0f; }
+
 // x[i] = c * tanh(x[i] / c), to the last bits of x (with x and c both times log2 e it is the capped score times that).
 // Scores are mostly small beside the cap: where all of a wave's are below a quarter of it, four terms of tanh's series
 // serve (the fifth is under 2^-26). Else six below 0.35, and 1 - 2 / (e^2y + 1) beyond, whose difference cancels no more
 // than two bits.
-// FOURS: four of them at a time, where all at once would spill.
+// FOURS: four of them at a time, where all at once would spill. inv_c: inverse_cap(c).
 template <int N, bool FOURS, typename X>
 __device__ __forceinline__ void cap_scores(X& x, float c, float inv_c) {
     float most = fabsf(x[0]);
 #pragma unroll
     for (int e = 1; e < N; ++e) most = fmaxf(most, fabsf(x[e]));
-    const float inv2 = inv_c * inv_c;
     if (__all(most * inv_c < 0.25f)) {  // (a NaN among others does not show in `most`; the series passes it on)
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const float z = x[e] * x[e] * inv2;
+            const float y = x[e] * inv_c, z = y * y;
             float p = __builtin_fmaf(62.0f / 2835.0f, z, -17.0f / 315.0f);
             p = __builtin_fmaf(p, z, 2.0f / 15.0f);
             p = __builtin_fmaf(p, z, -1.0f / 3.0f);
@@ -149,7 +151,7 @@ __device__ __forceinline__ void cap_scores(X& x, float c, float inv_c) {
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const float s = x[e], y = fabsf(s) * inv_c, z = s * s * inv2;
+            const float s = x[e], y = fabsf(s) * inv_c, z = y * y;
             float p = __builtin_fmaf(-1382.0f / 155925.0f, z, 62.0f / 2835.0f);
             p = __builtin_fmaf(p, z, -17.0f / 315.0f);
             p = __builtin_fmaf(p, z, 2.0f / 15.0f);

@@ -51,7 +51,7 @@ __global__ __launch_bounds__(64 * kStepWaves, DP <= 128 ? 2 : 1) void score_step
     const bool live = col < q.n * a.group;
     const int i = live ? col / a.group : max(q.n - 1, 0), head = h * a.group + (live ? col % a.group : 0);
 
-    const float cap = a.softcap * kLog2e, inv_cap = GEN && cap > 0.0f ? 1.0f / cap : 0.0f;
+    const float cap = a.softcap * kLog2e, inv_cap = GEN ? inverse_cap(cap) : 0.0f;
     const bool use_pos = GEN && (a.window > 0 || a.slopes || a.first || a.prefix);
     const int all_see = a.causal ? q.len - q.n + 1 : q.len;
     const int32_t* table = b.pages + (size_t)s * b.max_pages;
@@ -235,7 +235,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void score_prompt_kern
     const int per = (r_hi - r_lo + parts - 1) / parts;
     const int r0 = min(r_lo + part * per, r_hi), r1 = min(r0 + per, r_hi);
 
-    const float cap = a.softcap * kLog2e, inv_cap = GEN && cap > 0.0f ? 1.0f / cap : 0.0f;
+    const float cap = a.softcap * kLog2e, inv_cap = GEN ? inverse_cap(cap) : 0.0f;
     const int prefix = a.prefix ? a.prefix[s] : -0x7FFFFFFF - 1, window = a.window > 0 ? a.window : 0x7FFFFFFF;
     float v[kEach];
     Kv8Row in{};

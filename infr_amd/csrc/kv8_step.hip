@@ -62,7 +62,7 @@ __global__ __launch_bounds__(64 * kWaves<TOK>, DP == 64 ? 3 : DP == 128 || (DP =
     const int i = live ? rr / a.group : q.n - 1, head = h * a.group + (live ? rr % a.group : 0);
 
     const Kv8Row row = kv8_row(b, a, q, s, i, head);
-    const float cap = a.softcap * kLog2e, inv_cap = GEN && cap > 0.0f ? 1.0f / cap : 0.0f;
+    const float cap = a.softcap * kLog2e, inv_cap = GEN ? inverse_cap(cap) : 0.0f;
     const bool use_pos = GEN && (a.window > 0 || a.slopes || a.first || a.prefix);
     // tokens below this one are seen by every row of the tile (without masks by position)
     const int all_see = a.causal ? q.len - q.n + rt * ROWS / a.group + 1 : q.len;

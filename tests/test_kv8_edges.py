@@ -189,3 +189,29 @@ def test_values_next_to_the_largest(be, type_, dim, size, form, news, n_len):
     want, want_l, tol, ltol = orc.attention(c, b, m, q)
     close(out, want, tol)
     close(lse, want_l, ltol)
+
+
+# ---------------------------------------------------------------- caps and positions of any size
+
+@gpu
+@pytest.mark.parametrize("softcap,scale_q", [(1e-10, 1.0), (1e-25, 1.0), (1e-37, 1.0), (1e-44, 1.0), (1e25, 1e22), (3e38, 1e30)])
+@pytest.mark.parametrize("form,news", [("few rows", 3), ("64 rows", 140), ("128 rows", 140)])
+def test_caps_of_any_size(be, softcap, scale_q, form, news):
+    """c * tanh(s / c) is a number for every finite score and every cap, scores of 0 among them."""
+    rng = np.random.default_rng(45)
+    n_len = 150
+    c, pages, _ = filled(rng, "i8", 16, 2, 64, (n_len,))
+    c.sums[...] = 0.5
+    b = batch_in_form(form, (news,), (n_len,), pages)
+    m = orc.Mode(4, softcap=float(np.float32(softcap)))
+    q = (scale_q * rng.standard_normal((b.rows, 4 * 64))).astype(np.float32)
+    q[::2] = 0
+    dev = Dev(be, c)
+    out, lse = dev.attention(b, m, q)
+    want, want_l, tol, ltol = orc.attention(c, b, m, q)
+    close(out, want, tol)
+    close(lse, want_l, ltol)
+    if scale_q == 1.0:  # (beyond, an lse's own rounding is more than an exponential bears)
+        sums, stol = orc.score(c, b, m, q, lse, 1.0)
+        dev.score(b, m, q, lse)
+        assert (np.abs(dev.pull().sums - sums) <= stol).all()
