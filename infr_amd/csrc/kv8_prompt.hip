@@ -37,7 +37,6 @@ struct Stage {
     _Float16 v[DC][kPage + 8];
     float ks[4], vs[4];    // scales of the four runs of 16 tokens
     int32_t pos[kPage];
-    float rel[kPage];      // positions from the workgroup's first row's on: exact as far as 2^24
 };
 
 // DC: the columns that are computed with, head_dim rounded up to 32.
@@ -138,9 +137,6 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
     const float cap = a.softcap * kLog2e, inv_cap = GEN ? inverse_cap(cap) : 0.0f;
     const bool use_pos = GEN && (a.window > 0 || a.slopes || a.first || a.prefix);
 
-    const int ref = use_pos ? b.pos[min(q.r0 + rt * kRows / a.group, b.rows - 1)] : 0;
-    const float my_rel = (float)(row.pos - ref);
-
     f16x o[kOut];
 #pragma unroll
     for (int k = 0; k < kOut; ++k) o[k] = (f16x)(0.0f);
@@ -198,10 +194,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
         }
         if (tid < 4) st.ks[tid] = sr;
         else if (tid < 8) st.vs[tid - 4] = sr;
-        if (use_pos && tid < kPage) {
-            st.pos[tid] = pr;
-            st.rel[tid] = (float)(pr - ref);
-        }
+        if (use_pos && tid < kPage) st.pos[tid] = pr;
     };
 
     if (p0 < p1) {
@@ -247,9 +240,11 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void prompt_kernel(Kv8
                 if (GEN && a.slopes)
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) {
-                        const f4 y = *reinterpret_cast<const f4*>(&st.rel[(half0 + t) * 32 + hf * 16 + e]);
+                        const int4 y = *reinterpret_cast<const int4*>(&st.pos[(half0 + t) * 32 + hf * 16 + e]);
+                        const int kpos[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) x[t][e + n] = __builtin_fmaf(-row.slope, fabsf(my_rel - y[n]), x[t][e + n]);
+                        for (int n = 0; n < 4; ++n)  // (the difference is taken in integers: positions may be any)
+                            x[t][e + n] = __builtin_fmaf(-row.slope, fabsf((float)(row.pos - kpos[n])), x[t][e + n]);
                     }
                 if (masked) {
                     const int tok0 = p * kPage + (half0 + t) * 32 + hf * 16;

@@ -215,3 +215,29 @@ def test_caps_of_any_size(be, softcap, scale_q, form, news):
         sums, stol = orc.score(c, b, m, q, lse, 1.0)
         dev.score(b, m, q, lse)
         assert (np.abs(dev.pull().sums - sums) <= stol).all()
+
+
+@gpu
+@pytest.mark.parametrize("form,news", [("few rows", 3), ("64 rows", 250), ("128 rows", 250), ("128 rows in parts", 250)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_the_bias_by_distance_is_exact_at_far_positions(be, form, news, causal):
+    """Two documents in one sequence, the second at positions from 2^27 on: distances within it are small numbers. Its rows
+    see nothing of the first one, so their scores are of ordinary size, and the oracle's tolerances are."""
+    rng = np.random.default_rng(46)
+    n_len, cut = 250, 100
+    pos = np.concatenate([np.arange(cut), 2 ** 27 + 1 + 3 * np.arange(n_len - cut)]).astype(np.int32)
+    c, pages, _ = filled(rng, "i8", 16, 2, 64, (n_len,), pos=pos)
+    c.sums[...] = 0.5
+    b = batch_in_form(form, (news,), (n_len,), pages, pos=pos[n_len - news:])
+    first = np.where(np.arange(n_len) < cut, 0, pos[cut])[n_len - news:]
+    m = orc.Mode(4, slopes=2.0 ** -np.arange(1, 5), first=padded(first, b.rows), causal=causal)
+    q = rng.standard_normal((b.rows, 4 * 64)).astype(np.float32)
+    dev = Dev(be, c)
+    out, lse = dev.attention(b, m, q)
+    want, want_l, tol, ltol = orc.attention(c, b, m, q)
+    assert ltol[max(0, news - (n_len - cut)):news].max() < 1e-3
+    close(out, want, tol)
+    close(lse, want_l, ltol)
+    sums, stol = orc.score(c, b, m, q, lse, 1.0)
+    dev.score(b, m, q, lse)
+    assert (np.abs(dev.pull().sums - sums) <= stol).all()
