@@ -3,7 +3,8 @@
 Each case is one call of one operator on inputs a decoder has at that point: a cache of pages of 64
 tokens whose keys and values are int8 or e4m3 codes with an f32 scale for each block of tokens and
 KV head, and a batch of sequences described by device tables. With ``own`` false the operators are
-computed by elementary torch operations in 32 bits, with ``own`` true by this package."""
+computed by elementary torch operations in 32 bits, with ``own`` true by this package: `run` then enqueues on
+the backend's stream, and its outputs are there once that stream (``HipBackend.sync``) or the device was waited for."""
 import math
 
 import numpy as np
@@ -257,6 +258,8 @@ def prepare(case, seed):
         st["kept"] = torch.zeros(n_seq, n_kv, keep, dtype=torch.int32, device=dev)
     if own:
         _handles(st)
+        # the backend has a stream of its own, which does not wait for torch's: what is in hand is finished
+        torch.cuda.current_stream().synchronize()
     return st
 
 
