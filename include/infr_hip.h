@@ -295,7 +295,8 @@ int infr_hip_embed_gather(infr_hip_t *be, int dtype, const infr_hip_buffer_t *ta
  *   slots   [n_seq]      tail slot of each sequence (WriteKv8), one sequence's own as long as it lives. A sequence that
  *                        begins with a partly filled block another one wrote has its slot's tags set to -1 first
  * Sequences may share pages that none of them writes in the call; a page that a call writes stands once in its tables.
- * `max_q` bounds the rows of one sequence.
+ * `max_q` bounds the rows of one sequence. `max_pages` is the tables' width and what the launches are cut for: a table
+ * much wider than the sequences are long is right but can be slower.
  * Nothing outside the buffers is touched whatever the tables hold. A sequence whose tables contradict each other
  * or the shapes (len < n, n > max_q, q_start outside [0, rows], len > 64 max_pages) gets nothing written, and its rows
  * (up to max_q of them) read as NaN. Tokens on a page outside [0, n_pages) are not written and have no sums; rows whose
@@ -445,7 +446,8 @@ void infr_hip_plan_free(infr_hip_t *be, infr_hip_plan_t *plan);
 int infr_hip_execute(infr_hip_t *be, infr_hip_plan_t *plan, infr_hip_buffer_t *const *bindings,
                      size_t n_bindings);
 /* Number of kernel launches one execute of this plan issues for the bindings it last ran with
- * (0 before the first execute). Independent decode ops of one dependency level share a launch. */
+ * (0 before the first execute). Independent decode ops of one dependency level share a launch. With INFR_HIP_GRAPH=0,
+ * where nothing is recorded, the count is of the ops' common forms. */
 size_t infr_hip_plan_launches(const infr_hip_plan_t *plan);
 
 /* ---- shutdown latch (crates/infr-core/src/shutdown.rs:30-60): once requested, compute entry

@@ -10,7 +10,8 @@ namespace {
 // of a KV head the latter, and up to 256 as long as its tiles are no more than two for a compute unit, and their pages 32
 // (8 KV heads of 128, few / many: 64 rows behind 3000 tokens 15 / 28 us, behind 16000 33 / 42, 256 behind 3000 25 / 31,
 // 128 of each of 4 sequences of 600 to 1000 20 / 26, a prompt of 60 tokens, 4 heads to each, 8.0 / 10.1; but 64 of each of
-// 8 sequences of 500 to 8000 49 / 44, and three packed prompts of 250 tokens, 16 heads, 22 / 16).
+// 8 sequences of 500 to 8000 49 / 44, and three packed prompts of 250 tokens, 16 heads, 22 / 16). Pages are counted by the page table's
+// width: with a table of 2048 pages the prompt of 60 tokens takes 28 us, the 256 rows behind 3000 tokens 36.
 bool prompt_takes(int cus, int n_kv, int group, int n_seq, int max_q, int max_pages) {
     const int64_t rows = (int64_t)max_q * group, tiles = (rows + 15) / 16 * n_seq * n_kv;
     return rows > 32 && (rows > 256 || tiles > (int64_t)2 * cus || tiles * max_pages > (int64_t)32 * cus);

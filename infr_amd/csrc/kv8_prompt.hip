@@ -7,9 +7,11 @@
 // page's codes are requested before the current page is multiplied and written behind it, one barrier a page); a
 // wave's scores, softmax and output stay in its registers. Tokens are dealt to the MFMA's rows so that a lane holds
 // 16 neighbours: one block's scale, and P.V's operand as it stands.
-// Measured: 4096 tokens, 32 heads of 128, 8 KV heads: 278 us, 495 TFLOP/s, twice that in f16 products (a large f16 product
-// of the library: 1260). The matrix instructions and the softmax's take about as long and overlap little: a compute unit's
-// eight waves keep its clock at 1.95 GHz. Three packed prompts of 700 to 2501 tokens, 16 heads of 80: 65 us.
+// Measured: 4096 tokens, 32 heads of 128, 8 KV heads: 278 us one call behind the other for 0.15 s, 495 TFLOP/s, twice that
+// in f16 products (a large f16 product of the library: 1260); the kernel alone in short bursts, on a card less warmed up,
+// 299 to 328. By its counters there, at 1.96 GHz, matrix instructions take 45 % of the time and vector instructions 46 %,
+// and a third of either overlaps. Three packed prompts of 700 to 2501 tokens, 16 heads of 80: 63 to 77 us by the machine,
+// 11 % matrix and 35 % vector instructions: a tile's pages follow one another, and between them it waits.
 // With few row tiles a workgroup takes 64 rows instead, two waves to 32 of them, each with half of every page's tokens, and
 // joins their results in LDS at the end.
 // Pages no row of the workgroup sees are not visited; pages all rows of a wave see take no mask.
@@ -433,7 +435,7 @@ struct Cut {
     int ks, tiles, parts;
 };
 // Row tiles for waves that share rows by ks, and the parts their pages are cut into: enough for two workgroups on each
-// compute unit, of at least eight pages.
+// compute unit, of at least eight pages where sequences are as long as the page table is wide.
 Cut cut_for(int ks, int cus, int n_kv, int group, int n_seq, int max_q, int max_pages) {
     Cut c;
     c.ks = ks;
@@ -444,7 +446,7 @@ Cut cut_for(int ks, int cus, int n_kv, int group, int n_seq, int max_q, int max_
 }
 // Two waves to 32 rows halve a workgroup's time per page and double what is spent on bringing pages into LDS: better while
 // the time is that of the longest row tiles, which is up to four tiles of 128 rows for a compute unit (one / two ways, 32
-// heads of 128, 8 KV heads: 512 tokens 30 / 22 us, 1024 51 / 40, 2048 104 / 99, four times 1024 109 / 125, 4096 300 / 328;
+// heads of 128, 8 KV heads, short bursts: 512 tokens 30 / 22 us, 1024 51 / 40, 2048 104 / 99, four times 1024 109 / 125, 4096 300 / 328;
 // three packed prompts, 16 heads of 80: 88 / 67), two with more than 128 columns, where a compute unit holds one workgroup
 // (256 columns: 1024 tokens 96 / 80, 2048 197 / 252). Not where the twice as many tiles leave less than half the parts
 // (300 rows each behind 3000 and 1500 tokens, three parts / one: 82 / 98).

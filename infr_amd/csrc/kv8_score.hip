@@ -9,8 +9,9 @@
 // once for the four waves (two buffers, one barrier a step). Where pages are few, the rows are cut into parts whose
 // sums a second kernel adds in their order, so that the same call gives the same bits.
 // Measured: one token of 32 sequences of 1000 to 8000 tokens (8 KV heads of 128) 26 us, 4.6 TB/s; 1000 rows behind a
-// prompt of 4001 tokens, 32 heads of 128, 4 KV heads, capped scores: 168 us, 171 TFLOP/s - there the cap's series and the
-// exponential take two thirds of the instructions' time.
+// prompt of 4001 tokens, 32 heads of 128, 4 KV heads, capped scores: 164 to 173 us, 170 TFLOP/s - by the kernel's counters
+// vector instructions, the cap's series and the exponential above all, take 42 % of the time and matrix instructions 14 %; a
+// compute unit has work for 59 % of it, since the first pages are seen by more rows than the last.
 #include "kv8_attn.hpp"
 #include "kv8_device.hpp"
 
@@ -399,9 +400,12 @@ __global__ __launch_bounds__(64) void score_join_kernel(Kv8Cache c, Kv8Batch b, 
     *out = (decay != 0.0f ? decay * *out : 0.0f) + x;
 }
 
+// The form for few rows has one column tile.
 bool few_rows(int max_q, int group) { return (int64_t)max_q * group <= kStepRows; }
 
-// Parts of the rows: enough workgroups for two on each compute unit, four steps of rows at least in a part.
+// Parts of the rows: enough workgroups for two on each compute unit, four steps of rows at least in a part. The workgroups
+// are counted by the page table's width: a table far wider than the sequences are long leaves the rows in one part (1000 rows
+// behind 4001 tokens, 64 / 2048 pages: 166 / 720 us).
 int parts_of(int cus, int n_kv, int group, int n_seq, int max_q, int max_pages) {
     const int64_t wgs = (int64_t)n_seq * n_kv * ((max_pages + kWaves - 1) / kWaves);
     const int64_t steps = ((int64_t)max_q * group + kTile - 1) / kTile;

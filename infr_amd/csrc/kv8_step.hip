@@ -1,17 +1,17 @@
 // AttentionKv8 for few rows per sequence: decode steps and drafts. Bound by reading the cache once.
 //
 // Up to 16 query rows of one (sequence, KV head) - its rows times the heads of the group - are one column tile of
-// the 16x16x32 f16 MFMA; up to 8 of them take its other 8 columns for their low parts, and half the products. A wave takes one page at a time: 64 tokens as four row tiles chosen so that lane group g
-// holds tokens 16 g .. 16 g + 15 of its query row, which is what P.V wants side by side from V^T's 16-byte pieces.
+// the 16x16x32 f16 MFMA; up to 8 of them take its other 8 columns for their low parts, and half the products. A wave
+// takes one page at a time: 64 tokens as four row tiles chosen so that lane group g holds tokens 16 g .. 16 g + 15 of its query row, which is what P.V wants side by side from V^T's 16-byte pieces.
 // Key and value codes go from HBM to registers in 16-byte loads (whole lines per instruction), become f16 there and
 // feed the MFMA; the next page's keys are requested before the current page's softmax, its values before its scores.
 //
 // The pages of all sequences are cut into pieces of one size, found on the device from the lengths: long sequences
 // get many workgroups, short ones one, and no piece is empty. A sequence in one piece writes its result; the pieces
 // of others are joined by a second kernel, in their order.
-// Measured (8 KV heads of 128, 32 heads): one token of 64 sequences of 500 to 8000 tokens 69 us, 5.2 TB/s, 63 us and 5.7
-// TB/s of it the first kernel (a pass that only reads: 7.1 TB/s); two sequences of 115000 tokens, 4 KV heads, 45 us, 5.2
-// TB/s; one of 700 tokens 9.8 us, launch and dependent loads; drafts of 4 tokens of 16 sequences, window 1024, capped, 8
+// Measured (8 KV heads of 128, 32 heads): one token of 64 sequences of 500 to 8000 tokens 71 us, 5.1 TB/s, 63 us and 5.7
+// TB/s of it the first kernel (a pass that only reads: 7.1 TB/s); two sequences of 115000 tokens, 4 KV heads, 46 us, 5.2
+// TB/s; one of 700 tokens 10.3 us, launch and dependent loads; drafts of 4 tokens of 16 sequences, window 1024, capped, 8
 // KV heads of 256, 22 us, bound by what one wave does for half a page. (A join by the workgroup that comes last to its row tile
 // saves that launch but costs its own round trips past the L2, which the XCDs do not share: 53 us against 49 for two
 // sequences of 115000 tokens, 48 against 44 for drafts of four tokens.)
@@ -447,6 +447,7 @@ StepCut step_cut(int cus, int dim, bool gen, int window, int n_kv, int group, in
     c.whole = 2 * tiles > cus ? 24 : dim > 128 ? 4 : gen ? 8 : 12;
     // a window bounds the pages gone over: `window` tokens and one less than the call's rows
     const int64_t most = window > 0 ? std::min<int64_t>(max_pages, ((int64_t)window + max_q + 125) / kPage) : max_pages;
+    // (by the table's width: with one of 2048 pages a sequence of 700 tokens pays for an empty join, 13.9 us instead of 10.6)
     c.join = most > c.whole;
     // More than 128 columns leave a compute unit one wave a SIMD, and nothing to do while it waits, unless a wave takes half
     // a page; but that reads V in pieces of 32 bytes, which costs where reading is the bound: half up to 64 pages for a
