@@ -2,9 +2,10 @@
 //
 // Up to 16 query rows of one (sequence, KV head) - its rows times the heads of the group - are one column tile of
 // the 16x16x32 f16 MFMA; up to 8 of them take its other 8 columns for their low parts, and half the products. A wave
-// takes one page at a time: 64 tokens as four row tiles chosen so that lane group g holds tokens 16 g .. 16 g + 15 of its query row, which is what P.V wants side by side from V^T's 16-byte pieces.
-// Key and value codes go from HBM to registers in 16-byte loads (whole lines per instruction), become f16 there and
-// feed the MFMA; the next page's keys are requested before the current page's softmax, its values before its scores.
+// takes one page at a time: 64 tokens as four row tiles chosen so that lane group g holds tokens 16 g .. 16 g + 15 of
+// its query row, which is what P.V wants side by side from V^T's 16-byte pieces. Key and value codes go from HBM to
+// registers in 16-byte loads (whole lines per instruction), become f16 there and feed the MFMA; the next page's keys
+// are requested before the current page's softmax, its values before its scores.
 //
 // The pages of all sequences are cut into pieces of one size, found on the device from the lengths: long sequences
 // get many workgroups, short ones one, and no piece is empty. A sequence in one piece writes its result; the pieces
